@@ -11,6 +11,11 @@ single sequence, and full-context storage even for windowed layers
 
 Pool layout (one per layer of a group): ``[pages, kv_heads, PAGE_SIZE, head_dim]``.
 Page table (one per group): ``int32 [slots, pages_per_sequence]``.
+
+With ``kv_dtype`` "fp8" or "int8" keys and values are held in 8 bits: the pools hold codes (e4m3 or
+int8), and ``[pages, kv_heads, PAGE_SIZE]`` bytes hold the exponent, plus 127, of each row's
+power-of-two scale (the format: csrc/kv_quant.cuh). A windowed group then keeps every position, so that
+any step can be written before it attends.
 """
 from __future__ import annotations
 
@@ -22,6 +27,8 @@ import torch
 from ..kernels.ops import PAGE_SIZE   # one number for host and kernels; the library's own is checked when it is loaded
 from ..parts.base import KVNeed, StateNeed
 from .allocators import CacheFull, CacheStateError, PageAllocator, SlotAllocator
+
+KV_DTYPES = {"fp8": torch.float8_e4m3fn, "int8": torch.int8}   # what an 8-bit cache holds its codes as
 
 
 def pages_for(tokens: int) -> int:
@@ -39,18 +46,26 @@ class LayerCache:
     ring: int = 0
     window: Optional[int] = None
     state: Optional[torch.Tensor] = None  # [slots, *shape]
+    k_scale: Optional[torch.Tensor] = None  # an 8-bit cache: uint8 [pages, kv_heads, PAGE_SIZE]
+    v_scale: Optional[torch.Tensor] = None
 
 
 class KVGroup:
     def __init__(self, need: KVNeed, n_layers: int, n_pages: int, n_slots: int, max_seq_len: int,
                  dtype: torch.dtype, device: torch.device):
         self.need = need
-        self.ring = pages_for(need.window) * PAGE_SIZE if need.window else 0
+        quantised = dtype in KV_DTYPES.values()
+        self.ring = pages_for(need.window) * PAGE_SIZE if need.window and not quantised else 0
         self.pages_per_seq = pages_for(self.ring if self.ring else max_seq_len)
         self.ledger = PageAllocator(n_pages)
         shape = (n_layers, n_pages, need.kv_heads, PAGE_SIZE, need.head_dim)
-        self.k = torch.zeros(shape, dtype=dtype, device=device)
-        self.v = torch.zeros(shape, dtype=dtype, device=device)
+        held = torch.uint8 if quantised else dtype   # (zero bytes are zeros in every format)
+        self.k = torch.zeros(shape, dtype=held, device=device).view(dtype)
+        self.v = torch.zeros(shape, dtype=held, device=device).view(dtype)
+        self.k_scale = self.v_scale = None
+        if quantised:
+            self.k_scale = torch.zeros(shape[:-1], dtype=torch.uint8, device=device)
+            self.v_scale = torch.zeros(shape[:-1], dtype=torch.uint8, device=device)
         self.table = torch.zeros((n_slots, self.pages_per_seq), dtype=torch.int32, device=device)
         self.slot_pages: Dict[int, List[int]] = {}
         self.n_layers = n_layers
@@ -60,7 +75,8 @@ class KVGroup:
         return min(n, self.pages_per_seq) if self.ring else n
 
     def bytes_per_token(self) -> int:
-        return 2 * self.n_layers * self.need.kv_heads * self.need.head_dim * self.k.element_size()
+        row = self.need.head_dim * self.k.element_size() + (0 if self.k_scale is None else 1)
+        return 2 * self.n_layers * self.need.kv_heads * row
 
 
 class SequenceCache:
@@ -68,11 +84,15 @@ class SequenceCache:
     ``StateNeed``, ``None``, or an int naming the earlier run whose cache it reads."""
 
     def __init__(self, needs: Sequence[Union[KVNeed, StateNeed, None, int]], *, max_tokens: int, max_slots: int,
-                 max_seq_len: int, dtype: torch.dtype, device: Union[str, torch.device]):
+                 max_seq_len: int, dtype: torch.dtype, device: Union[str, torch.device], kv_dtype: Optional[str] = None):
+        if kv_dtype is not None and kv_dtype not in KV_DTYPES:
+            raise ValueError(f"kv_dtype must be one of {', '.join(sorted(KV_DTYPES))} (or None: the compute type), got {kv_dtype!r}")
         if max_tokens <= 0 or max_seq_len <= 0:
             raise ValueError("max_tokens and max_seq_len must be positive")
         self.device = torch.device(device)
         self.dtype = dtype
+        self.kv_dtype = kv_dtype
+        held = KV_DTYPES[kv_dtype] if kv_dtype is not None else dtype
         self.max_tokens = max_tokens
         self.max_seq_len = max_seq_len
         self.n_pages = pages_for(max_tokens)
@@ -103,7 +123,7 @@ class SequenceCache:
             else:
                 raise TypeError(f"run {run}: unknown cache need {need!r}")
         for need, g in sorted(group_of.items(), key=lambda kv: kv[1]):
-            self.groups.append(KVGroup(need, members[g], self.n_pages, self.max_slots, max_seq_len, dtype, self.device))
+            self.groups.append(KVGroup(need, members[g], self.n_pages, self.max_slots, max_seq_len, held, self.device))
         for kind, what, index in plan:
             if kind == "kv":
                 self._run_view.append(("kv", what, index))
@@ -192,7 +212,8 @@ class SequenceCache:
         kind, index, layer = self._run_view[run]
         if kind == "kv":
             g = self.groups[index]
-            return LayerCache("kv", g.k[layer], g.v[layer], g.table, g.ring, g.need.window)
+            k_scale, v_scale = (None, None) if g.k_scale is None else (g.k_scale[layer], g.v_scale[layer])
+            return LayerCache("kv", g.k[layer], g.v[layer], g.table, g.ring, g.need.window, k_scale=k_scale, v_scale=v_scale)
         if kind == "state":
             return LayerCache("state", state=self.states[index])
         return LayerCache("none")

@@ -130,6 +130,26 @@ SM_API int sm_kv_store(const void* k_packed, const void* v_packed, int dt, int T
     });
 }
 
+SM_API int sm_kv_quant_store(const void* k_packed, const void* v_packed, int dt, int T, int kv_heads, int head_dim, void* k_rows,
+                             void* v_rows, int fmt, void* k_pool, void* v_pool, void* k_scale, void* v_scale,
+                             long long pool_pages, const int32_t* positions, const int32_t* page_table, int slots, int table_stride,
+                             const int32_t* token_slot, void* stream) {
+    return guarded([&] {
+        sm::kv_quant_store(k_packed, v_packed, (sm::DType)dt, T, kv_heads, head_dim, k_rows, v_rows, fmt, k_pool, v_pool, k_scale,
+                           v_scale, pool_pages, positions, page_table, slots, table_stride, token_slot, (cudaStream_t)stream);
+    });
+}
+
+SM_API int sm_kv_quant_load(int fmt, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
+                            long long pool_pages, int dt, int n_seqs, int kv_heads, int head_dim, const int32_t* slot_ids,
+                            const int32_t* seq_ends, const int32_t* page_table, int slots, int table_stride, void* k_out, void* v_out, int32_t* out_table, int pages,
+                            int whole, void* stream) {
+    return guarded([&] {
+        sm::kv_quant_load(fmt, k_pool, v_pool, k_scale, v_scale, pool_pages, (sm::DType)dt, n_seqs, kv_heads, head_dim, slot_ids,
+                          seq_ends, page_table, slots, table_stride, k_out, v_out, out_table, pages, whole != 0, (cudaStream_t)stream);
+    });
+}
+
 SM_API int sm_gemm_simt(const void* x, int x_dt, const void* w, int w_dt, const void* bias, int bias_dt, void* out,
                         int out_dt, int T, int N, int K, int accumulate, void* stream) {
     return guarded([&] {

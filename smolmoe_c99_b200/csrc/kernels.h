@@ -76,6 +76,21 @@ void kv_store(const void* k_packed, const void* v_packed, DType dt, int T, int k
               void* v_pool, const int32_t* positions, const int32_t* page_table, int table_stride, int ring,
               const int32_t* token_slot, const int32_t* token_end, cudaStream_t stream);
 
+// ---- kv_quant.cu ----------------------------------------------------------------------
+// The 8-bit cache (format and pools: kv_quant.cuh; fmt: 0 e4m3, 1 int8). kv_quant_store: a step's packed keys and values
+// [T, kv_heads, head_dim] (F32 or BF16) as codes and exponents into the pages of their positions; k_rows, v_rows
+// (nullable) receive what the cache then stands for, in dt. kv_quant_load: the pages of n_seqs sequences as values of dt,
+// [n_seqs, pages, kv_heads, 64, head_dim], positions at and past seq_ends[i] as zeros (pages wholly past it only if
+// `whole`, else they are left alone), and out_table [slots, pages] to find them by slot. page_table is [slots, table_stride];
+// a place outside it or the pools (pool_pages) is left out and recorded in the error word.
+void kv_quant_store(const void* k_packed, const void* v_packed, DType dt, int T, int kv_heads, int head_dim, void* k_rows,
+                    void* v_rows, int fmt, void* k_pool, void* v_pool, void* k_scale, void* v_scale, long long pool_pages,
+                    const int32_t* positions, const int32_t* page_table, int slots, int table_stride, const int32_t* token_slot,
+                    cudaStream_t stream);
+void kv_quant_load(int fmt, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
+                   long long pool_pages, DType dt, int n_seqs, int kv_heads, int head_dim, const int32_t* slot_ids, const int32_t* seq_ends,
+                   const int32_t* page_table, int slots, int table_stride, void* k_out, void* v_out, int32_t* out_table, int pages, bool whole, cudaStream_t stream);
+
 // ---- gemm_simt.cu ---------------------------------------------------------------------
 // out[t, n] (+)= sum_k x[t, k] * w[n, k] + bias[n]; float FMA in ascending k for every
 // element, whatever T is. x: F32 or BF16; w, bias: F32 or BF16; out: F32 or BF16.

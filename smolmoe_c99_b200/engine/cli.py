@@ -55,6 +55,8 @@ def build_parser() -> argparse.ArgumentParser:
                    help="bfloat16 kernels, or the whole model in true 32-bit")
     g.add_argument("--kernels", choices=["fast", "plain"], default="fast",
                    help="plain: every product and attention on the plain kernels, for comparison")
+    g.add_argument("--kv-dtype", choices=["fp8", "int8"], default=None,
+                   help="hold the key/value cache in 8 bits a value (default: in the compute dtype)")
     g = p.add_argument_group("diagnostics")
     g.add_argument("--stats", help="JSON statistics (always printed to stderr)")
     g.add_argument("--trace", help="exact hexadecimal logits of every processed token of every prompt")
@@ -119,10 +121,10 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     try:
         if args.random:
             model = Model.from_random(config, args.seed, args.dtype, args.context, args.batch,
-                                      step_tokens=args.step_tokens, kernels=args.kernels)
+                                      step_tokens=args.step_tokens, kernels=args.kernels, kv_dtype=args.kv_dtype)
         else:
             model = Model.from_folder(model_dir, args.dtype, args.context, args.batch,
-                                      step_tokens=args.step_tokens, kernels=args.kernels)
+                                      step_tokens=args.step_tokens, kernels=args.kernels, kv_dtype=args.kv_dtype)
     except (ValueError, RuntimeError, OSError) as e:
         raise SystemExit(f"smolmoe: {e}")
     loaded = time.perf_counter()
@@ -130,6 +132,7 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     if args.profile:
         engine.start_profile()
     stats = {"version": __version__, "backend": f"cuda sm_100a {args.kernels}", "dtype": args.dtype, "batch": args.batch,
+             "kv_dtype": args.kv_dtype or args.dtype,
              "kv_bytes": engine.cache.bytes_per_token() * engine.cache.max_tokens,
              "weight_bytes": engine.weight_bytes(), "load_seconds": loaded - started}
     logits_hash = FNV_OFFSET

@@ -151,7 +151,10 @@ class _StepGraph:
 class Engine:
     def __init__(self, model_dir: str, dtype: Union[str, torch.dtype] = "bfloat16", *, max_tokens: int = 4096,
                  max_slots: Optional[int] = None, max_seq_len: Optional[int] = None, device: str = "cuda:0",
-                 use_graphs: bool = True, max_step_tokens: Optional[int] = None, kernels: str = "fast"):
+                 use_graphs: bool = True, max_step_tokens: Optional[int] = None, kernels: str = "fast",
+                 kv_dtype: Optional[str] = None):
+        # kv_dtype: what keys and values are held as: None the compute dtype, "fp8" or "int8" 8 bits a value and one scale a
+        # row (half of bfloat16's bytes, and about twice the positions in the same memory)
         self.dtype = DTYPES[dtype] if isinstance(dtype, str) else dtype
         if self.dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("dtype must be bfloat16 or float32")
@@ -166,7 +169,7 @@ class Engine:
         self.model.bind(tensors)
         self.cache = SequenceCache(cache_needs(self.spec), max_tokens=max_tokens,
                                    max_slots=max_slots if max_slots is not None else 256,
-                                   max_seq_len=self.max_seq_len, dtype=self.dtype, device=self.device)
+                                   max_seq_len=self.max_seq_len, dtype=self.dtype, device=self.device, kv_dtype=kv_dtype)
         self.vocab_size = self.spec.vocab_size
         self.use_graphs = use_graphs
         # a generation loop may launch the next one-token step before it has read the tokens just chosen (generate.py)

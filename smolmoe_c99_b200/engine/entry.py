@@ -33,24 +33,26 @@ class Model:
     # ---- opening -------------------------------------------------------------------------
     @classmethod
     def from_folder(cls, path: str, dtype: str = "bfloat16", context: Optional[int] = None, batch: int = 8,
-                    device: str = "cuda:0", step_tokens: Optional[int] = None, kernels: str = "fast") -> "Model":
+                    device: str = "cuda:0", step_tokens: Optional[int] = None, kernels: str = "fast",
+                    kv_dtype: Optional[str] = None) -> "Model":
         """``context``: positions a sequence may hold (default: the smaller of the model's limit
         and 2048); ``batch``: most sequences that start together. The cache is sized for
         ``batch`` sequences of ``context`` positions. ``step_tokens``: the most tokens one step may bring; longer
         prompts go through in portions (the reference's ``--batch``, src/main.c:106). ``kernels``: ``"fast"`` or
-        ``"plain"`` (every product and attention on the plain kernels, for comparison)."""
+        ``"plain"`` (every product and attention on the plain kernels, for comparison). ``kv_dtype``: ``"fp8"`` or
+        ``"int8"`` hold the cache in 8 bits a value (None: in the compute dtype)."""
         from ..config import load_config
 
         limit = load_config(path).model_spec().max_positions
         context = min(limit, context or DEFAULT_CONTEXT)
         rounded = -(-context // 64) * 64
         return cls(Engine(path, dtype, max_tokens=rounded * batch, max_slots=batch, max_seq_len=context, device=device,
-                          max_step_tokens=step_tokens, kernels=kernels))
+                          max_step_tokens=step_tokens, kernels=kernels, kv_dtype=kv_dtype))
 
     @classmethod
     def from_random(cls, config: Union[dict, object], seed: int, dtype: str = "bfloat16", context: Optional[int] = None,
                     batch: int = 8, device: str = "cuda:0", step_tokens: Optional[int] = None,
-                    kernels: str = "fast") -> "Model":
+                    kernels: str = "fast", kv_dtype: Optional[str] = None) -> "Model":
         """Random weights for a configuration (a ``config.json`` dictionary or a configuration
         object of a registered architecture) and a seed."""
         import tempfile
@@ -61,7 +63,7 @@ class Model:
         cfg = config_from_json(config) if isinstance(config, dict) else config
         with tempfile.TemporaryDirectory(prefix="smolmoe_b200_") as tmp:
             write_random_model(cfg, tmp, seed)
-            return cls.from_folder(tmp, dtype, context, batch, device, step_tokens, kernels)
+            return cls.from_folder(tmp, dtype, context, batch, device, step_tokens, kernels, kv_dtype)
 
     # ---- generating ----------------------------------------------------------------------
     def generate(self, prompts: Sequence[Sequence[int]], tokens: int = 64, temperature: float = 0.0, top_k: int = 40,

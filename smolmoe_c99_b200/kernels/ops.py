@@ -3,6 +3,7 @@ the C function on the current stream. Nothing here computes; there is no fallbac
 from __future__ import annotations
 
 import ctypes
+import dataclasses
 from typing import Optional
 
 import torch
@@ -14,6 +15,9 @@ PAGE_SIZE = 64  # positions per cache page; checked against the library's own nu
 KERNEL_CHOICES = ("fast", "plain")
 # activations of a gated feed-forward, by the numbers the kernels know them by (Activation in csrc/common.cuh)
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1, "gelu_pytorch_tanh": 1}
+# formats of an 8-bit cache, by the numbers the kernels know them by (QuantFormat in csrc/kv_quant.cuh)
+QUANT_FORMATS = {torch.float8_e4m3fn: 0, torch.int8: 1}
+BAD_PLACES = {31: "kv_quant_store", 32: "kv_quant_load", 33: "attention_quant"}   # (codes of the error word, csrc/kv_quant.cuh)
 # the reference's phases (src/model.h:38-41, src/model.c:312-328); the ones that have no counterpart here stay 0
 PHASES = ("embed", "norm", "qkv", "rope", "attention", "attn_out", "ffn_up", "activation", "attn_quant", "ffn_down",
           "routing", "residual", "logits")
@@ -45,6 +49,14 @@ def _need(t: torch.Tensor, what: str, dtype=None, ndim=None) -> torch.Tensor:
     if ndim is not None and t.dim() != ndim:
         raise KernelError(f"{what} must have {ndim} dimensions, got {t.dim()}")
     return t
+
+
+def _here(*tensors: torch.Tensor) -> None:
+    """The kernels run on the current device: tensors of another one are refused."""
+    device = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t.get_device() != device:
+            raise KernelError(f"a tensor lies on {t.device}, the current device is cuda:{device}")
 
 
 def _stream() -> ctypes.c_void_p:
@@ -120,6 +132,11 @@ class Ops:
                               f"the host by {PAGE_SIZE}")
         self.lib.sm_gemm_tc_workspace_bytes.restype = ctypes.c_longlong
         self.lib.sm_launch_count.restype = ctypes.c_longlong
+        # (with the argument types known, a call takes plain numbers as addresses)
+        addr, num = ctypes.c_void_p, ctypes.c_int
+        big = ctypes.c_longlong
+        self.lib.sm_kv_quant_store.argtypes = [addr, addr] + [num] * 4 + [addr, addr, num] + [addr] * 4 + [big, addr, addr, num, num, addr, addr]
+        self.lib.sm_kv_quant_load.argtypes = [num] + [addr] * 4 + [big] + [num] * 4 + [addr] * 3 + [num, num] + [addr] * 3 + [num, num, addr]
         fast = kernels == "fast"
         self.kernels = kernels
         self.phase_times: Optional[PhaseTimes] = None   # set to time the phases of the forward pass
@@ -508,6 +525,8 @@ class Ops:
             self.error_flag.zero_()
             for words in self._fused_barriers:
                 words.zero_()
+            if code in BAD_PLACES:
+                raise KernelError(f"{BAD_PLACES[code]} met a slot, position or page outside the 8-bit cache; its output is not valid")
             raise KernelError(f"a kernel's bounded wait ran out (code {code}); its output is not valid")
 
     # ---- attention ---------------------------------------------------------------------
@@ -581,6 +600,86 @@ class Ops:
                                          _ptr(cache.k_pool), _ptr(cache.v_pool), _ptr(step.positions),
                                          _ptr(cache.page_table), cache.page_table.shape[1], cache.ring,
                                          _ptr(step.token_slot), _ptr(step.token_end), _stream()))
+
+    # ---- an 8-bit cache ------------------------------------------------------------------
+    def _quant_cache(self, cache) -> tuple:
+        """Checks an 8-bit layer cache; returns (format, pages, kv heads, head size)."""
+        k, v, ks, vs = cache.k_pool, cache.v_pool, cache.k_scale, cache.v_scale
+        if cache.kind != "kv" or ks is None or vs is None:
+            raise KernelError("an 8-bit key/value cache is needed (kv_dtype fp8 or int8)")
+        fmt = QUANT_FORMATS.get(k.dtype)
+        if fmt is None or v.dtype != k.dtype:
+            raise KernelError(f"pools of an 8-bit cache are float8_e4m3fn or int8, got {k.dtype} and {v.dtype}")
+        if ks.dtype != torch.uint8 or vs.dtype != torch.uint8:
+            raise KernelError("exponents of an 8-bit cache are uint8")
+        shape = k.shape
+        if len(shape) != 4 or shape[2] != PAGE_SIZE or v.shape != shape or ks.shape != shape[:3] or vs.shape != shape[:3]:
+            raise KernelError(f"pools of an 8-bit cache are [pages, kv heads, {PAGE_SIZE}, head size] with exponents of the first three, "
+                              f"got {tuple(shape)}, {tuple(v.shape)}, {tuple(ks.shape)}, {tuple(vs.shape)}")
+        if cache.ring:
+            raise KernelError("an 8-bit cache keeps every position: it has no ring")
+        table = cache.page_table
+        if table.dtype != torch.int32 or table.dim() != 2:
+            raise KernelError("the page table must be int32 [slots, pages]")
+        if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and table.is_contiguous()):
+            raise KernelError("the pools, exponents and page table of an 8-bit cache must be contiguous")
+        _here(k, v, ks, vs, table)
+        return fmt, shape[0], shape[1], shape[3]
+
+    def kv_quant_store(self, k_packed, v_packed, step, cache, want_rows: bool = False):
+        """This step's packed keys and values [T, kv heads, head size] into an 8-bit cache, one power-of-two scale a row.
+        With ``want_rows`` returns (k, v) as the cache now stands for them, laid out like the packed tensors. A row that
+        holds an infinity or a NaN reads back as NaN whole."""
+        fmt, pool_pages, kv_heads, head_dim = self._quant_cache(cache)
+        _need(k_packed, "packed keys", ndim=3)
+        _need(v_packed, "packed values", k_packed.dtype, 3)
+        if tuple(k_packed.shape) != (step.n_tokens, kv_heads, head_dim) or v_packed.shape != k_packed.shape:
+            raise KernelError(f"packed keys and values are {tuple(k_packed.shape)} and {tuple(v_packed.shape)}, expected "
+                              f"{(step.n_tokens, kv_heads, head_dim)}")
+        _here(k_packed, v_packed, step.positions)
+        rows = (torch.empty_like(k_packed), torch.empty_like(v_packed)) if want_rows else None
+        self._check(self.lib.sm_kv_quant_store(
+            k_packed.data_ptr(), v_packed.data_ptr(), _dt(k_packed), step.n_tokens, kv_heads, head_dim,
+            rows[0].data_ptr() if rows else None, rows[1].data_ptr() if rows else None, fmt, cache.k_pool.data_ptr(),
+            cache.v_pool.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pool_pages,
+            step.positions.data_ptr(), cache.page_table.data_ptr(), cache.page_table.shape[0], cache.page_table.shape[1], step.token_slot.data_ptr(), _stream()))
+        return rows
+
+    def kv_quant_load(self, step, cache, dtype: torch.dtype, whole: bool = True):
+        """What an 8-bit cache holds of the step's sequences (their lengths after the step), as values: a ``LayerCache`` of
+        ``dtype`` whose page table has the same slots. Sequence ``i`` of the step has its pages from ``i * P`` on, ``P``
+        the pages of ``step.max_seq_len`` positions (at most the page table's width); positions past its end read as zeros, pages wholly past it too
+        (``whole`` False leaves those unwritten)."""
+        fmt, pool_pages, kv_heads, head_dim = self._quant_cache(cache)
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise KernelError(f"an 8-bit cache is read back as float32 or bfloat16, not {dtype}")
+        # (a captured step's longest sequence is a bound that may pass what the page table can hold)
+        pages = min((step.max_seq_len + PAGE_SIZE - 1) // PAGE_SIZE, cache.page_table.shape[1])
+        _here(step.slot_ids, step.seq_ends)
+        device = cache.k_pool.device
+        k = torch.empty((step.n_seqs * pages, kv_heads, PAGE_SIZE, head_dim), dtype=dtype, device=device)
+        v = torch.empty_like(k)
+        table = torch.empty((cache.page_table.shape[0], pages), dtype=torch.int32, device=device)
+        self._check(self.lib.sm_kv_quant_load(
+            fmt, cache.k_pool.data_ptr(), cache.v_pool.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pool_pages,
+            _dt(k), step.n_seqs, kv_heads, head_dim, step.slot_ids.data_ptr(), step.seq_ends.data_ptr(), cache.page_table.data_ptr(),
+            cache.page_table.shape[0], cache.page_table.shape[1], k.data_ptr(), v.data_ptr(), table.data_ptr(), pages, int(whole), _stream()))
+        return dataclasses.replace(cache, k_pool=k, v_pool=v, page_table=table, k_scale=None, v_scale=None)
+
+    def attention_quant(self, q, step, scale, window, cache):
+        """Causal attention of this step's tokens (one or any number per sequence) over an 8-bit cache, which holds their own
+        keys and values already (``kv_quant_store``). ``window``: each sees that many positions up to its own (None or
+        0: all)."""
+        _, _, kv_heads, head_dim = self._quant_cache(cache)
+        _need(q, "q", ndim=3)
+        if q.shape[0] != step.n_tokens or q.shape[2] != head_dim or q.shape[1] == 0 or q.shape[1] % kv_heads:
+            raise KernelError(f"q is {tuple(q.shape)}: expected {step.n_tokens} tokens, a multiple of {kv_heads} heads, head size {head_dim}")
+        if window and window < 0:
+            raise KernelError(f"a window of {window} positions")
+        _here(q, step.positions)
+        pages = self.kv_quant_load(step, cache, q.dtype, whole=False)
+        return self.attention_plain(q, step.positions, scale, window, k_pool=pages.k_pool, v_pool=pages.v_pool,
+                                    page_table=pages.page_table, token_slot=step.token_slot, kv_heads=kv_heads)
 
     def attention_extend(self, q, k_packed, v_packed, step, scale, window, cache, cache_written=False):
         """Causal attention of sequences that go on from the cache by any number of tokens: keys and values of

@@ -78,6 +78,9 @@ class Attention(Part):
         mode = step.mode
         if cache.kind != "kv":
             raise RuntimeError("attention needs a key/value cache")
+        if cache.k_scale is not None:
+            self._forward_quant(x, residual, step, cache, cos, sin)
+            return
         if mode == "decode" and own:
             # one token per sequence: product, bias, rotation and cache write in one launch
             q = ops.qkv_rope_store_fused(x, self.w_qkv, self.b_qkv, step.positions, cos, sin, self.heads, self.kv_heads,
@@ -124,6 +127,37 @@ class Attention(Part):
         ops.linear(att.view(T, self.heads * self.head_dim), self.w_o, None, out=residual, accumulate=True)
         ops.lap("attn_out")
 
+    def _forward_quant(self, x, residual, step, cache, cos, sin) -> None:
+        """The step over an 8-bit cache: keys and values are rounded to it as they are written, and every token attends
+        over what the cache stands for (whole prompts over the rounded rows themselves), so a prompt's logits do not
+        depend on how it is cut into steps."""
+        ops, rt = self.runtime.ops, self.runtime
+        T, own = x.shape[0], not self.kv_from_cache
+        kv_heads = self.kv_heads if own else 0
+        # many tokens or few: product, bias and rotation in one launch, keys and values packed
+        fused = ops.qkv_rope_store_many(x, self.w_qkv, self.b_qkv, step.positions, cos, sin, self.heads, kv_heads, self.head_dim,
+                                        self.position.rotary_dim, want_packed=own, page_table=cache.page_table,
+                                        token_slot=step.token_slot, token_end=step.token_end)
+        if fused is not None:
+            q, k_packed, v_packed = fused
+            ops.lap("qkv")
+        else:
+            qkv = ops.linear(x, self.w_qkv, self.b_qkv, out_dtype=torch.float32)
+            ops.lap("qkv")
+            q, k_packed, v_packed = ops.rope_store(qkv, step.positions, cos, sin, self.heads, kv_heads, self.head_dim,
+                                                   self.position.rotary_dim, rt.dtype, want_packed=own)
+            ops.lap("rope")
+        whole = own and step.mode == "prefill"
+        rows = ops.kv_quant_store(k_packed, v_packed, step, cache, want_rows=whole) if own else None
+        ops.lap("attn_quant")
+        if whole:
+            att = ops.attention_prefill(q, rows[0], rows[1], step, self.scale, self.window)
+        else:
+            att = ops.attention_quant(q, step, self.scale, self.window, cache)
+        ops.lap("attention")
+        ops.linear(att.view(T, self.heads * self.head_dim), self.w_o, None, out=residual, accumulate=True)
+        ops.lap("attn_out")
+
     def _check_ring_still_holds(self, step, cache) -> None:
         """A run that reads another run's windowed cache finds this step's rows already written: the oldest key a
         query of the step sees must not have been replaced by them."""
@@ -137,7 +171,7 @@ class Attention(Part):
     def fused_decode_record(self, cache):
         """What a kernel that runs whole layers needs of this part and its cache, or None where the part is not the
         plain case that kernel is written for (keys and values of its own, every dimension rotated)."""
-        if (type(self).forward is not Attention.forward or self.kv_from_cache or cache.kind != "kv"
+        if (type(self).forward is not Attention.forward or self.kv_from_cache or cache.kind != "kv" or cache.k_scale is not None
                 or self.position.rotary_dim != self.head_dim):
             return None
         cos, sin = self.position.tables(self.runtime.max_positions)
