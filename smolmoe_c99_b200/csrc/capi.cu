@@ -143,10 +143,11 @@ SM_API int sm_kv_quant_store(const void* k_packed, const void* v_packed, int dt,
 SM_API int sm_kv_quant_load(int fmt, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
                             long long pool_pages, int dt, int n_seqs, int kv_heads, int head_dim, const int32_t* slot_ids,
                             const int32_t* seq_ends, const int32_t* page_table, int slots, int table_stride, void* k_out, void* v_out, int32_t* out_table, int pages,
-                            int whole, void* stream) {
+                            int whole, const int32_t* cu_seqlens, int skip_new, int attend, int window, void* stream) {
     return guarded([&] {
         sm::kv_quant_load(fmt, k_pool, v_pool, k_scale, v_scale, pool_pages, (sm::DType)dt, n_seqs, kv_heads, head_dim, slot_ids,
-                          seq_ends, page_table, slots, table_stride, k_out, v_out, out_table, pages, whole != 0, (cudaStream_t)stream);
+                          seq_ends, page_table, slots, table_stride, k_out, v_out, out_table, pages, whole != 0, cu_seqlens, skip_new,
+                          attend != 0, window, (cudaStream_t)stream);
     });
 }
 
@@ -247,10 +248,30 @@ SM_API int sm_attention_extend_tc_supports(int heads, int kv_heads, int head_dim
 SM_API int sm_attention_extend_tc(const void* q, void* out, const int32_t* tiles, int n_tiles, int T, int heads, int kv_heads,
                                   int head_dim, float scale, int window, const void* k_pool, const void* v_pool,
                                   const int32_t* page_table, int table_stride, long long pool_pages, int longest, int variant,
-                                  int* error, void* stream) {
+                                  int skip_new, int* error, void* stream) {
     return guarded([&] {
         sm::attention_extend_tc(q, out, tiles, n_tiles, T, heads, kv_heads, head_dim, scale, window, k_pool, v_pool, page_table,
-                                table_stride, pool_pages, longest, variant, error, (cudaStream_t)stream);
+                                table_stride, pool_pages, longest, variant, skip_new, error, (cudaStream_t)stream);
+    });
+}
+
+SM_API int sm_attention_quant_supports(int heads, int kv_heads, int head_dim, long long pool_pages) {
+    return sm::attention_quant_supports(heads, kv_heads, head_dim, pool_pages) ? 1 : 0;
+}
+
+SM_API long long sm_attention_quant_workspace(int head_dim, int row_tiles, int direct) {
+    return sm::attention_quant_workspace(head_dim, row_tiles, direct != 0);
+}
+
+SM_API int sm_attention_quant(const void* q, void* out, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window,
+                              int fmt, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
+                              long long pool_pages, const int32_t* page_table, int slots, int table_stride, const int32_t* slot_ids,
+                              const int32_t* seq_ends, const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles,
+                              int pairs, int direct, float* workspace, long long workspace_floats, void* stream) {
+    return guarded([&] {
+        sm::attention_quant(q, out, n_seqs, heads, kv_heads, head_dim, scale, window, fmt, k_pool, v_pool, k_scale, v_scale,
+                            pool_pages, page_table, slots, table_stride, slot_ids, seq_ends, cu_seqlens, max_len, most_new,
+                            row_tiles, pairs, direct != 0, workspace, workspace_floats, (cudaStream_t)stream);
     });
 }
 

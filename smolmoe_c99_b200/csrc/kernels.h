@@ -82,14 +82,18 @@ void kv_store(const void* k_packed, const void* v_packed, DType dt, int T, int k
 // (nullable) receive what the cache then stands for, in dt. kv_quant_load: the pages of n_seqs sequences as values of dt,
 // [n_seqs, pages, kv_heads, 64, head_dim], positions at and past seq_ends[i] as zeros (pages wholly past it only if
 // `whole`, else they are left alone), and out_table [slots, pages] to find them by slot. page_table is [slots, table_stride];
-// a place outside it or the pools (pool_pages) is left out and recorded in the error word.
+// a place outside it or the pools (pool_pages) is left out and recorded in the error word. Sequences that bring at
+// most `skip_new` tokens by cu_seqlens [n_seqs + 1] are left out. `attend`: for a kernel that multiplies masked values by
+// zero weights: a value row without a scale is read as zeros and its key as NaN instead (a token that sees it is NaN either
+// way), and pages of 128 positions that no token of the step sees in `window` are left alone.
 void kv_quant_store(const void* k_packed, const void* v_packed, DType dt, int T, int kv_heads, int head_dim, void* k_rows,
                     void* v_rows, int fmt, void* k_pool, void* v_pool, void* k_scale, void* v_scale, long long pool_pages,
                     const int32_t* positions, const int32_t* page_table, int slots, int table_stride, const int32_t* token_slot,
                     cudaStream_t stream);
 void kv_quant_load(int fmt, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
                    long long pool_pages, DType dt, int n_seqs, int kv_heads, int head_dim, const int32_t* slot_ids, const int32_t* seq_ends,
-                   const int32_t* page_table, int slots, int table_stride, void* k_out, void* v_out, int32_t* out_table, int pages, bool whole, cudaStream_t stream);
+                   const int32_t* page_table, int slots, int table_stride, void* k_out, void* v_out, int32_t* out_table, int pages, bool whole,
+                   const int32_t* cu_seqlens, int skip_new, bool attend, int window, cudaStream_t stream);
 
 // ---- gemm_simt.cu ---------------------------------------------------------------------
 // out[t, n] (+)= sum_k x[t, k] * w[n, k] + bias[n]; float FMA in ascending k for every
@@ -234,11 +238,11 @@ void attention_prefill_tc(const void* q, const void* k, const void* v, void* out
 
 // The same kernel for sequences that go on from the cache by many tokens (prompt portions): keys and values come from
 // the paged pools, which must hold the step's own tokens already; `tiles` [n_tiles, 5] as attention_extend takes them,
-// `longest` the longest sequence after the step. No windowed group (its ring is written after the attention).
+// `longest` the longest sequence after the step. Sequences that bring at most `skip_new` tokens are left out. No windowed group (its ring is written after the attention).
 bool attention_extend_tc_supports(int heads, int kv_heads, int head_dim, long long pool_pages);
 void attention_extend_tc(const void* q, void* out, const int32_t* tiles, int n_tiles, int T, int heads, int kv_heads, int head_dim,
                          float scale, int window, const void* k_pool, const void* v_pool, const int32_t* page_table,
-                         int table_stride, long long pool_pages, int longest, int variant, int* error, cudaStream_t stream);
+                         int table_stride, long long pool_pages, int longest, int variant, int skip_new, int* error, cudaStream_t stream);
 
 // ---- attention_decode.cu --------------------------------------------------------------
 // One new token per sequence over the paged cache for bfloat16: a cluster of CTAs per
@@ -257,6 +261,22 @@ void attention_decode(const void* q, void* out, int B, int heads, int kv_heads, 
                       const int32_t* positions, const int32_t* slots, const void* k_pool, const void* v_pool,
                       const int32_t* page_table, int table_stride, int ring, int max_len, long long pool_pages, bool late,
                       cudaStream_t stream);
+
+// ---- attention_quant.cu ---------------------------------------------------------------
+// Attention over the 8-bit cache, which holds the step's own keys and values already, for bfloat16 queries [T, heads,
+// head_dim] of sequences that bring at most `most_new` tokens (those that bring more are skipped: nothing of theirs is
+// written). cu_seqlens [n_seqs + 1], slot_ids, seq_ends [n_seqs] (lengths after the step) are read on the device; on the
+// host: max_len, a bound of the lengths; row_tiles (1, 2, or 4 for head sizes up to 64): tiles of 8 rows of queries (token,
+// head of a group) that are worked on together; pairs = kv_heads * blocks of such rows over the sequences; direct: one CTA
+// a pair, no workspace (for short sequences), else a grid of one CTA an SM shares the tiles out evenly and a second kernel
+// joins what it cut. head_dim: multiples of 16 up to 128; at most 16 heads a kv head.
+bool attention_quant_supports(int heads, int kv_heads, int head_dim, long long pool_pages);
+long long attention_quant_workspace(int head_dim, int row_tiles, bool direct);   // floats
+void attention_quant(const void* q, void* out, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window, int fmt,
+                     const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale, long long pool_pages,
+                     const int32_t* page_table, int slots, int table_stride, const int32_t* slot_ids, const int32_t* seq_ends,
+                     const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles, int pairs, bool direct, float* workspace,
+                     long long workspace_floats, cudaStream_t stream);
 
 // ---- decode_fused.cu ------------------------------------------------------------------
 // One decode step (every sequence goes on by one token) of a stack of standard layers -- RMSNorm, attention with

@@ -116,6 +116,9 @@ struct LoadArgs {
     const int32_t* seq_ends;     // [sequences]
     QuantPages table;
     int kv_heads, head_dim, pages, whole;
+    const int32_t* cu;           // [sequences + 1] (read only where skip_new or a window asks for it)
+    int skip_new;                // sequences that bring at most this many tokens are left out
+    int attend, window;          // see kv_quant_load in kernels.h
     int* error;
 };
 
@@ -127,6 +130,7 @@ __global__ void __launch_bounds__(kThreads) kv_quant_load_kernel(LoadArgs a) {
     pdl_launch_dependents();
     const int seq = blockIdx.y, which = blockIdx.z;
     const int slot = a.slot_ids[seq], end = a.seq_ends[seq];
+    if (a.skip_new > 0 && a.cu[seq + 1] - a.cu[seq] <= a.skip_new) return;
     const int parts = a.head_dim / 8;                             // of a row
     const long long idx = (long long)blockIdx.x * kThreads + threadIdx.x;
     const int part = (int)(idx % parts);
@@ -141,19 +145,33 @@ __global__ void __launch_bounds__(kThreads) kv_quant_load_kernel(LoadArgs a) {
     }
     if (which == 0 && part == 0 && in_page == 0 && kvh == 0) a.out_table[(size_t)slot * a.pages + page] = seq * a.pages + page;
     if (page * kPageSize >= end && !a.whole) return;
+    if (a.window > 0) {
+        // pages that no token of the step sees, but for the neighbour that shares a tile of 128 positions with a seen one
+        const int lowest = end - (a.cu[seq + 1] - a.cu[seq]) - a.window + 1;
+        if (lowest > 0 && page < lowest / 128 * (128 / kPageSize)) return;
+    }
     float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const int held = page * kPageSize + in_page < end ? a.table.at(slot, page) : -1;
     if (held < 0) {
         if (page * kPageSize + in_page < end && a.error) atomicExch(a.error, kBadPlaceInLoad);
     } else {
         const size_t cell = ((size_t)held * a.kv_heads + kvh) * kPageSize + in_page;
-        const float scale = scale_of(a.scales[which][cell]);
+        int byte = a.scales[which][cell];
+        if (a.attend) {
+            if (which == 0 && a.scales[1][cell] == kNoScale) byte = kNoScale;
+            if (which == 1 && byte == kNoScale) byte = 0;
+        }
+        const float scale = scale_of(byte);
         const uint2 codes = *reinterpret_cast<const uint2*>(a.codes[which] + cell * a.head_dim + part * 8);
         float v[4], w[4];
         decode4<FMT>(codes.x, v);
         decode4<FMT>(codes.y, w);
+        const bool none = byte == kNoScale;      // (also where the codes are another row's: a key whose value has no scale)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { y[i] = v[i] * scale; y[4 + i] = w[i] * scale; }
+        for (int i = 0; i < 4; ++i) {
+            y[i] = none ? __int_as_float(0x7fffffff) : v[i] * scale;
+            y[4 + i] = none ? __int_as_float(0x7fffffff) : w[i] * scale;
+        }
     }
     const size_t out_row = (size_t)seq * a.pages * a.kv_heads * kPageSize + (size_t)row;
     store8((T*)a.out[which] + out_row * a.head_dim + part * 8, y);
@@ -188,14 +206,15 @@ void kv_quant_store(const void* k_packed, const void* v_packed, DType dt, int T,
 
 void kv_quant_load(int fmt, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
                    long long pool_pages, DType dt, int n_seqs, int kv_heads, int head_dim, const int32_t* slot_ids, const int32_t* seq_ends,
-                   const int32_t* page_table, int slots, int table_stride, void* k_out, void* v_out, int32_t* out_table, int pages, bool whole, cudaStream_t stream) {
+                   const int32_t* page_table, int slots, int table_stride, void* k_out, void* v_out, int32_t* out_table, int pages, bool whole,
+                   const int32_t* cu_seqlens, int skip_new, bool attend, int window, cudaStream_t stream) {
     if (n_seqs <= 0 || pages <= 0) return;
     check_sizes("kv_quant_load", kv_heads, head_dim, fmt);
     if (n_seqs > 65535) throw std::invalid_argument("kv_quant_load: more than 65535 sequences");
     if (((uintptr_t)k_out | (uintptr_t)v_out) & 15 || ((uintptr_t)k_pool | (uintptr_t)v_pool) & 7)
         throw std::invalid_argument("kv_quant_load: outputs must be 16-byte aligned and pools 8-byte aligned");
     LoadArgs a{{(const uint8_t*)k_pool, (const uint8_t*)v_pool}, {(const uint8_t*)k_scale, (const uint8_t*)v_scale}, {k_out, v_out}, out_table,
-               slot_ids, seq_ends, {page_table, slots, table_stride, pool_pages}, kv_heads, head_dim, pages, whole ? 1 : 0, error_word()};
+               slot_ids, seq_ends, {page_table, slots, table_stride, pool_pages}, kv_heads, head_dim, pages, whole ? 1 : 0, cu_seqlens, skip_new, attend ? 1 : 0, attend ? window : 0, error_word()};
     const long long threads = (long long)pages * kv_heads * kPageSize * (head_dim / 8);
     const long long blocks = (threads + kThreads - 1) / kThreads;
     if (blocks > 0x7fffffffll) throw std::invalid_argument("kv_quant_load: too many pages for one call");

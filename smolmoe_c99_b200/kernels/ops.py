@@ -136,7 +136,12 @@ class Ops:
         addr, num = ctypes.c_void_p, ctypes.c_int
         big = ctypes.c_longlong
         self.lib.sm_kv_quant_store.argtypes = [addr, addr] + [num] * 4 + [addr, addr, num] + [addr] * 4 + [big, addr, addr, num, num, addr, addr]
-        self.lib.sm_kv_quant_load.argtypes = [num] + [addr] * 4 + [big] + [num] * 4 + [addr] * 3 + [num, num] + [addr] * 3 + [num, num, addr]
+        self.lib.sm_kv_quant_load.argtypes = [num] + [addr] * 4 + [big] + [num] * 4 + [addr] * 3 + [num, num] + [addr] * 3 + [num, num, addr, num, num, num, addr]
+        self.lib.sm_attention_quant.argtypes = [addr, addr] + [num] * 4 + [ctypes.c_float, num, num] + [addr] * 4 + [big, addr, num, num] + \
+            [addr] * 3 + [num] * 5 + [addr, big, addr]
+        self.lib.sm_attention_quant_supports.argtypes = [num, num, num, big]
+        self.lib.sm_attention_quant_workspace.argtypes, self.lib.sm_attention_quant_workspace.restype = [num, num, num], big
+        self._quant_workspaces: dict = {}
         fast = kernels == "fast"
         self.kernels = kernels
         self.phase_times: Optional[PhaseTimes] = None   # set to time the phases of the forward pass
@@ -161,6 +166,7 @@ class Ops:
         # 8,000 6.85 against 4.43
         self.extend_rows_as_decode_tc = 176 if fast else 0
         self.extend_tc_variant = -1     # that kernel with one CTA an SM (0), two (1, head size 64), or as the launcher chooses
+        self.quant_rows_tokens = 64     # over an 8-bit cache: sequences that bring more tokens go to the tcgen05 kernel
         self.skinny_single_round_above_8 = True
         self.error_flag = torch.zeros(1, dtype=torch.int32, device="cuda")
         self.lib.sm_set_error_word.restype = None
@@ -645,17 +651,21 @@ class Ops:
             step.positions.data_ptr(), cache.page_table.data_ptr(), cache.page_table.shape[0], cache.page_table.shape[1], step.token_slot.data_ptr(), _stream()))
         return rows
 
-    def kv_quant_load(self, step, cache, dtype: torch.dtype, whole: bool = True):
+    def kv_quant_load(self, step, cache, dtype: torch.dtype):
         """What an 8-bit cache holds of the step's sequences (their lengths after the step), as values: a ``LayerCache`` of
         ``dtype`` whose page table has the same slots. Sequence ``i`` of the step has its pages from ``i * P`` on, ``P``
-        the pages of ``step.max_seq_len`` positions (at most the page table's width); positions past its end read as zeros, pages wholly past it too
-        (``whole`` False leaves those unwritten)."""
-        fmt, pool_pages, kv_heads, head_dim = self._quant_cache(cache)
+        the pages of ``step.max_seq_len`` positions (at most the page table's width); positions past its end read as
+        zeros."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise KernelError(f"an 8-bit cache is read back as float32 or bfloat16, not {dtype}")
+        return self._quant_load(step, cache, dtype, True, 0, False, 0)
+
+    def _quant_load(self, step, cache, dtype, whole, skip_new, attend, window):
+        """``whole``: pages past a sequence's end are zeroed too; the others: see kv_quant_load in csrc/kernels.h."""
+        fmt, pool_pages, kv_heads, head_dim = self._quant_cache(cache)
         # (a captured step's longest sequence is a bound that may pass what the page table can hold)
         pages = min((step.max_seq_len + PAGE_SIZE - 1) // PAGE_SIZE, cache.page_table.shape[1])
-        _here(step.slot_ids, step.seq_ends)
+        _here(step.slot_ids, step.seq_ends, step.cu_seqlens)
         device = cache.k_pool.device
         k = torch.empty((step.n_seqs * pages, kv_heads, PAGE_SIZE, head_dim), dtype=dtype, device=device)
         v = torch.empty_like(k)
@@ -663,23 +673,68 @@ class Ops:
         self._check(self.lib.sm_kv_quant_load(
             fmt, cache.k_pool.data_ptr(), cache.v_pool.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pool_pages,
             _dt(k), step.n_seqs, kv_heads, head_dim, step.slot_ids.data_ptr(), step.seq_ends.data_ptr(), cache.page_table.data_ptr(),
-            cache.page_table.shape[0], cache.page_table.shape[1], k.data_ptr(), v.data_ptr(), table.data_ptr(), pages, int(whole), _stream()))
+            cache.page_table.shape[0], cache.page_table.shape[1], k.data_ptr(), v.data_ptr(), table.data_ptr(), pages, int(whole),
+            step.cu_seqlens.data_ptr(), skip_new, int(attend), window, _stream()))
         return dataclasses.replace(cache, k_pool=k, v_pool=v, page_table=table, k_scale=None, v_scale=None)
 
     def attention_quant(self, q, step, scale, window, cache):
         """Causal attention of this step's tokens (one or any number per sequence) over an 8-bit cache, which holds their own
         keys and values already (``kv_quant_store``). ``window``: each sees that many positions up to its own (None or
         0: all)."""
-        _, _, kv_heads, head_dim = self._quant_cache(cache)
+        fmt, pool_pages, kv_heads, head_dim = self._quant_cache(cache)
         _need(q, "q", ndim=3)
         if q.shape[0] != step.n_tokens or q.shape[2] != head_dim or q.shape[1] == 0 or q.shape[1] % kv_heads:
             raise KernelError(f"q is {tuple(q.shape)}: expected {step.n_tokens} tokens, a multiple of {kv_heads} heads, head size {head_dim}")
         if window and window < 0:
             raise KernelError(f"a window of {window} positions")
         _here(q, step.positions)
-        pages = self.kv_quant_load(step, cache, q.dtype, whole=False)
-        return self.attention_plain(q, step.positions, scale, window, k_pool=pages.k_pool, v_pool=pages.v_pool,
-                                    page_table=pages.page_table, token_slot=step.token_slot, kv_heads=kv_heads)
+        heads = q.shape[1]
+        if not self.use_fast_attention or q.dtype != torch.bfloat16 or not self.lib.sm_attention_quant_supports(heads, kv_heads, head_dim, pool_pages):
+            # the plain kernel over pages that have been read back: float queries, other head sizes
+            pages = self._quant_load(step, cache, q.dtype, False, 0, False, 0)
+            return self.attention_plain(q, step.positions, scale, window, k_pool=pages.k_pool, v_pool=pages.v_pool,
+                                        page_table=pages.page_table, token_slot=step.token_slot, kv_heads=kv_heads)
+        out = torch.empty_like(q)
+        lens = step.seq_lens
+        most = max(lens)
+        limit = most
+        if (most > self.quant_rows_tokens and step.extend_tiles is not None and self.use_tcgen05_attention
+                and self.lib.sm_attention_extend_tc_supports(heads, kv_heads, head_dim, ctypes.c_longlong(step.n_seqs * cache.page_table.shape[1]))):
+            limit = self.quant_rows_tokens
+            few = [n for n in lens if n <= limit]
+            most = max(few) if few else 0
+        if most:
+            # single tokens, and sequences that bring a few: straight from the codes
+            group = heads // kv_heads
+            row_tiles = 1
+            while 8 * row_tiles < min(most * group, 32 if head_dim <= 64 else 16) or 8 * row_tiles < group:
+                row_tiles *= 2
+            tokens = 8 * row_tiles // group
+            pairs = kv_heads * (step.n_seqs if most == 1 and limit == most else sum(-(-n // tokens) for n in lens if n <= limit))
+            longest = step.max_seq_len if not window else min(step.max_seq_len, window + most)
+            direct = longest <= 256
+            floats = 0
+            if not direct:
+                key = (head_dim <= 64, row_tiles)
+                floats = self._quant_workspaces.get(key)
+                if floats is None:
+                    floats = self._quant_workspaces[key] = int(self.lib.sm_attention_quant_workspace(head_dim, row_tiles, 0))
+            workspace = torch.empty((floats,), dtype=torch.float32, device=q.device) if floats else None
+            self._check(self.lib.sm_attention_quant(
+                q.data_ptr(), out.data_ptr(), step.n_seqs, heads, kv_heads, head_dim, scale, int(window or 0), fmt, cache.k_pool.data_ptr(),
+                cache.v_pool.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pool_pages, cache.page_table.data_ptr(),
+                cache.page_table.shape[0], cache.page_table.shape[1], step.slot_ids.data_ptr(), step.seq_ends.data_ptr(),
+                step.cu_seqlens.data_ptr(), longest, limit, row_tiles, pairs, int(direct), workspace.data_ptr() if floats else None, floats,
+                _stream()))
+        if limit < max(lens):
+            # many tokens: the pages are read back as bfloat16 once (exactly), and the tcgen05 kernel reads those
+            pages = self._quant_load(step, cache, q.dtype, False, limit, True, int(window or 0))
+            self._check(self.lib.sm_attention_extend_tc(
+                _ptr(q), _ptr(out), _ptr(step.extend_tiles), step.extend_tiles.shape[0], q.shape[0], heads, kv_heads, head_dim,
+                ctypes.c_float(scale), int(window or 0), _ptr(pages.k_pool), _ptr(pages.v_pool), _ptr(pages.page_table),
+                pages.page_table.shape[1], ctypes.c_longlong(pages.k_pool.shape[0]), int(step.max_seq_len),
+                int(self.extend_tc_variant), limit, _ptr(self.error_flag), _stream()))
+        return out
 
     def attention_extend(self, q, k_packed, v_packed, step, scale, window, cache, cache_written=False):
         """Causal attention of sequences that go on from the cache by any number of tokens: keys and values of
@@ -707,7 +762,7 @@ class Ops:
                 _ptr(q), _ptr(out), _ptr(step.extend_tiles), step.extend_tiles.shape[0], q.shape[0], q.shape[1],
                 k_packed.shape[1], q.shape[2], ctypes.c_float(scale), int(window or 0), _ptr(cache.k_pool), _ptr(cache.v_pool),
                 _ptr(cache.page_table), cache.page_table.shape[1], ctypes.c_longlong(cache.k_pool.shape[0]),
-                int(step.max_seq_len), int(self.extend_tc_variant), _ptr(self.error_flag), _stream()))
+                int(step.max_seq_len), int(self.extend_tc_variant), 0, _ptr(self.error_flag), _stream()))
             return out
         if (self.use_fast_attention and q.dtype == torch.bfloat16 and step.extend_tiles is not None
                 and self.lib.sm_attention_prefill_supports(q.shape[2])):
