@@ -259,19 +259,19 @@ SM_API int sm_attention_quant_supports(int heads, int kv_heads, int head_dim, lo
     return sm::attention_quant_supports(heads, kv_heads, head_dim, pool_pages) ? 1 : 0;
 }
 
-SM_API long long sm_attention_quant_workspace(int head_dim, int row_tiles, int direct) {
-    return sm::attention_quant_workspace(head_dim, row_tiles, direct != 0);
+SM_API long long sm_attention_quant_workspace(int head_dim, int row_tiles, int pairs, int cluster) {
+    return sm::attention_quant_workspace(head_dim, row_tiles, pairs, cluster);
 }
 
 SM_API int sm_attention_quant(const void* q, void* out, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window,
                               int fmt, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
                               long long pool_pages, const int32_t* page_table, int slots, int table_stride, const int32_t* slot_ids,
                               const int32_t* seq_ends, const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles,
-                              int pairs, int direct, float* workspace, long long workspace_floats, void* stream) {
+                              int pairs, int cluster, float* workspace, long long workspace_floats, void* stream) {
     return guarded([&] {
         sm::attention_quant(q, out, n_seqs, heads, kv_heads, head_dim, scale, window, fmt, k_pool, v_pool, k_scale, v_scale,
                             pool_pages, page_table, slots, table_stride, slot_ids, seq_ends, cu_seqlens, max_len, most_new,
-                            row_tiles, pairs, direct != 0, workspace, workspace_floats, (cudaStream_t)stream);
+                            row_tiles, pairs, cluster, workspace, workspace_floats, (cudaStream_t)stream);
     });
 }
 

@@ -267,15 +267,15 @@ void attention_decode(const void* q, void* out, int B, int heads, int kv_heads, 
 // head_dim] of sequences that bring at most `most_new` tokens (those that bring more are skipped: nothing of theirs is
 // written). cu_seqlens [n_seqs + 1], slot_ids, seq_ends [n_seqs] (lengths after the step) are read on the device; on the
 // host: max_len, a bound of the lengths; row_tiles (1, 2, or 4 for head sizes up to 64): tiles of 8 rows of queries (token,
-// head of a group) that are worked on together; pairs = kv_heads * blocks of such rows over the sequences; direct: one CTA
-// a pair, no workspace (for short sequences), else a grid of one CTA an SM shares the tiles out evenly and a second kernel
-// joins what it cut. head_dim: multiples of 16 up to 128; at most 16 heads a kv head.
+// head of a group) that are worked on together; pairs = kv_heads * blocks of such rows over the sequences; cluster: 1 to 8
+// CTAs work on a pair, or 0: one CTA an SM, whose warps share the tiles of all pairs out evenly, with a second kernel that
+// joins what they cut (workspace, attention_quant.cu). head_dim: multiples of 16 up to 128; at most 16 heads a kv head.
 bool attention_quant_supports(int heads, int kv_heads, int head_dim, long long pool_pages);
-long long attention_quant_workspace(int head_dim, int row_tiles, bool direct);   // floats
+long long attention_quant_workspace(int head_dim, int row_tiles, int pairs, int cluster);   // floats
 void attention_quant(const void* q, void* out, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window, int fmt,
                      const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale, long long pool_pages,
                      const int32_t* page_table, int slots, int table_stride, const int32_t* slot_ids, const int32_t* seq_ends,
-                     const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles, int pairs, bool direct, float* workspace,
+                     const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles, int pairs, int cluster, float* workspace,
                      long long workspace_floats, cudaStream_t stream);
 
 // ---- decode_fused.cu ------------------------------------------------------------------

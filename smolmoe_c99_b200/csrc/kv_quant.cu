@@ -1,7 +1,8 @@
 // Writing the 8-bit key/value cache and reading it back (the format: kv_quant.cuh).
 //
-// Both are bound by memory: a thread takes 8 values of a row (16 or 32 bytes in, 8 out, or the other way), the lanes that
-// share a row find its largest magnitude with shuffles, so a value is read once and written once.
+// Both are bound by memory: a thread takes 8 values of a row at a time (16 or 32 bytes in, 8 out, or the other way) and
+// several rows at once; the lanes that share a row find its largest magnitude with shuffles, so a value is read once and
+// written once.
 #include <stdexcept>
 #include <string>
 
@@ -56,54 +57,70 @@ struct StoreArgs {
     int* error;
 };
 
-// One row per group of `lanes` threads (a power of two, at least head_dim / 8); blockIdx.y: keys or values.
+// One row per group of `lanes` threads (a power of two, at least head_dim / 8); blockIdx.y: keys or values. A thread does
+// kStoreRows rows, so that as many loads are under way together.
+constexpr int kStoreRows = 4;
+
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kThreads) kv_quant_store_kernel(StoreArgs a, int lanes) {
     pdl_wait();                  // the rows come from the kernel before
     pdl_launch_dependents();
     const int per_block = kThreads / lanes;
-    const long long row = (long long)blockIdx.x * per_block + threadIdx.x / lanes;
+    const long long row0 = (long long)blockIdx.x * per_block * kStoreRows + threadIdx.x / lanes;
     const int part = threadIdx.x % lanes;
     const int which = blockIdx.y;
-    const bool live = row < a.rows_of_each, mine = live && part * 8 < a.head_dim;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const size_t at = (size_t)row * a.head_dim + part * 8;
-    size_t cell = 0;             // the row's number in the pools
-    bool placed = true;
-    if (live) {
-        const int t = (int)(row / a.kv_heads), kvh = (int)(row - (long long)t * a.kv_heads);
-        const int pos = a.positions[t];
-        const int page = pos < 0 ? -1 : a.pages.at(a.token_slot[t], pos / kPageSize);
-        if (page < 0) {
-            if (a.error) atomicExch(a.error, kBadPlaceInStore);
-            placed = false;
-        }
-        cell = ((size_t)page * a.kv_heads + kvh) * kPageSize + pos % kPageSize;
-    }
-    if (mine) load8((const T*)a.packed[which] + at, x);
-    uint32_t amax = 0;
+    const T* packed = (const T*)a.packed[which];
+    float x[kStoreRows][8];
+    int at_token[kStoreRows], at_slot[kStoreRows];
+    bool mine[kStoreRows];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);
-    for (int o = lanes >> 1; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (!mine) return;
-    const int byte = scale_byte<FMT>(amax);
-    uint32_t lo = 0, hi = 0;
-    if (byte != kNoScale) {
-        const float up = power_of_two(127 - byte);
-        lo = encode4<FMT>(x[0] * up, x[1] * up, x[2] * up, x[3] * up);
-        hi = encode4<FMT>(x[4] * up, x[5] * up, x[6] * up, x[7] * up);
+    for (int u = 0; u < kStoreRows; ++u) {
+        const long long row = row0 + u * per_block;
+        const bool live = row < a.rows_of_each;
+        mine[u] = live && part * 8 < a.head_dim;
+        const int t = live ? (int)(row / a.kv_heads) : 0;
+        at_token[u] = a.positions[t];
+        at_slot[u] = a.token_slot[t];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+        if (mine[u]) load8(packed + (size_t)row * a.head_dim + part * 8, x[u]);
     }
-    if (placed) {
-        *reinterpret_cast<uint2*>(a.codes[which] + cell * a.head_dim + part * 8) = make_uint2(lo, hi);
-        if (part == 0) a.scales[which][cell] = (uint8_t)byte;
-    }
-    if (a.rows[which] != nullptr) {
-        const float scale = scale_of(byte);
-        float v[4], w[4];
-        decode4<FMT>(lo, v);
-        decode4<FMT>(hi, w);
-        const float y[8] = {v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale, w[0] * scale, w[1] * scale, w[2] * scale, w[3] * scale};
-        store8((T*)a.rows[which] + at, y);
+    int page[kStoreRows];
+#pragma unroll
+    for (int u = 0; u < kStoreRows; ++u) page[u] = at_token[u] < 0 ? -1 : a.pages.at(at_slot[u], at_token[u] / kPageSize);
+#pragma unroll
+    for (int u = 0; u < kStoreRows; ++u) {
+        const long long row = row0 + u * per_block;
+        uint32_t amax = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(x[u][i]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            if (o < lanes) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if (mine[u]) {
+            const int byte = scale_byte<FMT>(amax);
+            uint32_t lo = 0, hi = 0;
+            if (byte != kNoScale) {
+                const float up = power_of_two(127 - byte);
+                lo = encode4<FMT>(x[u][0] * up, x[u][1] * up, x[u][2] * up, x[u][3] * up);
+                hi = encode4<FMT>(x[u][4] * up, x[u][5] * up, x[u][6] * up, x[u][7] * up);
+            }
+            if (page[u] >= 0) {
+                const size_t cell = ((size_t)page[u] * a.kv_heads + (size_t)(row % a.kv_heads)) * kPageSize + at_token[u] % kPageSize;
+                *reinterpret_cast<uint2*>(a.codes[which] + cell * a.head_dim + part * 8) = make_uint2(lo, hi);
+                if (part == 0) a.scales[which][cell] = (uint8_t)byte;
+            } else if (a.error) {
+                atomicExch(a.error, kBadPlaceInStore);
+            }
+            if (a.rows[which] != nullptr) {
+                const float scale = scale_of(byte);
+                float v[4], w[4];
+                decode4<FMT>(lo, v);
+                decode4<FMT>(hi, w);
+                const float y[8] = {v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale, w[0] * scale, w[1] * scale, w[2] * scale, w[3] * scale};
+                store8((T*)a.rows[which] + (size_t)row * a.head_dim + part * 8, y);
+            }
+        }
     }
 }
 
@@ -122,59 +139,71 @@ struct LoadArgs {
     int* error;
 };
 
-// blockIdx.y: the sequence, blockIdx.z: keys or values; a thread takes 8 values. Positions at and past the sequence's end
-// read as zero; pages wholly past it are left alone unless `whole`.
+// A CTA reads one page (blockIdx.x) of one sequence (blockIdx.y), keys or values (blockIdx.z): a page's kv heads lie one
+// behind the other in the pools and in the output, so this is one run of bytes and one of values, 8 of them a thread and
+// kLoadSteps such pieces under way together. Positions at and past the sequence's end read as zero; pages wholly past it
+// are left alone unless `whole`.
+constexpr int kLoadSteps = 4;
+
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kThreads) kv_quant_load_kernel(LoadArgs a) {
     pdl_wait();                  // the cache may have been written by the kernel before
     pdl_launch_dependents();
-    const int seq = blockIdx.y, which = blockIdx.z;
+    const int page = blockIdx.x, seq = blockIdx.y, which = blockIdx.z;
     const int slot = a.slot_ids[seq], end = a.seq_ends[seq];
     if (a.skip_new > 0 && a.cu[seq + 1] - a.cu[seq] <= a.skip_new) return;
-    const int parts = a.head_dim / 8;                             // of a row
-    const long long idx = (long long)blockIdx.x * kThreads + threadIdx.x;
-    const int part = (int)(idx % parts);
-    const long long row = idx / parts;                            // page, kv head, position in the page
-    const int in_page = (int)(row % kPageSize);
-    const int kvh = (int)((row / kPageSize) % a.kv_heads);
-    const int page = (int)(row / ((long long)kPageSize * a.kv_heads));
-    if (page >= a.pages) return;
     if ((unsigned)slot >= (unsigned)a.table.slots) {
-        if (a.error) atomicExch(a.error, kBadPlaceInLoad);
+        if (a.error && threadIdx.x == 0) atomicExch(a.error, kBadPlaceInLoad);
         return;
     }
-    if (which == 0 && part == 0 && in_page == 0 && kvh == 0) a.out_table[(size_t)slot * a.pages + page] = seq * a.pages + page;
-    if (page * kPageSize >= end && !a.whole) return;
+    if (which == 0 && threadIdx.x == 0) a.out_table[(size_t)slot * a.pages + page] = seq * a.pages + page;
+    const int live = min(end - page * kPageSize, kPageSize);      // positions of the page that the sequence holds
+    if (live <= 0 && !a.whole) return;
     if (a.window > 0) {
         // pages that no token of the step sees, but for the neighbour that shares a tile of 128 positions with a seen one
         const int lowest = end - (a.cu[seq + 1] - a.cu[seq]) - a.window + 1;
         if (lowest > 0 && page < lowest / 128 * (128 / kPageSize)) return;
     }
-    float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const int held = page * kPageSize + in_page < end ? a.table.at(slot, page) : -1;
-    if (held < 0) {
-        if (page * kPageSize + in_page < end && a.error) atomicExch(a.error, kBadPlaceInLoad);
-    } else {
-        const size_t cell = ((size_t)held * a.kv_heads + kvh) * kPageSize + in_page;
-        int byte = a.scales[which][cell];
-        if (a.attend) {
-            if (which == 0 && a.scales[1][cell] == kNoScale) byte = kNoScale;
-            if (which == 1 && byte == kNoScale) byte = 0;
-        }
-        const float scale = scale_of(byte);
-        const uint2 codes = *reinterpret_cast<const uint2*>(a.codes[which] + cell * a.head_dim + part * 8);
-        float v[4], w[4];
-        decode4<FMT>(codes.x, v);
-        decode4<FMT>(codes.y, w);
-        const bool none = byte == kNoScale;      // (also where the codes are another row's: a key whose value has no scale)
+    const int held = live > 0 ? a.table.at(slot, page) : -1;
+    if (live > 0 && held < 0 && a.error && threadIdx.x == 0) atomicExch(a.error, kBadPlaceInLoad);
+    const int parts = a.head_dim / 8, total = a.kv_heads * kPageSize * parts;      // pieces of 8 values: of a row, of the page
+    const size_t cell0 = held < 0 ? 0 : (size_t)held * a.kv_heads * kPageSize;
+    const uint8_t* codes = a.codes[which] + cell0 * a.head_dim;
+    T* out = (T*)a.out[which] + ((size_t)seq * a.pages + page) * a.kv_heads * kPageSize * a.head_dim;
+    for (int base = threadIdx.x; base < total; base += kThreads * kLoadSteps) {
+        uint2 raw[kLoadSteps];
+        int byte[kLoadSteps];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            y[i] = none ? __int_as_float(0x7fffffff) : v[i] * scale;
-            y[4 + i] = none ? __int_as_float(0x7fffffff) : w[i] * scale;
+        for (int u = 0; u < kLoadSteps; ++u) {
+            const int i = base + u * kThreads, row = i / parts;
+            raw[u] = make_uint2(0, 0);
+            byte[u] = 0;
+            if (i < total && held >= 0 && row % kPageSize < live) {
+                raw[u] = *reinterpret_cast<const uint2*>(codes + (size_t)i * 8);
+                byte[u] = a.scales[which][cell0 + row];
+                if (a.attend) {
+                    if (which == 0 && a.scales[1][cell0 + row] == kNoScale) byte[u] = kNoScale;
+                    if (which == 1 && byte[u] == kNoScale) byte[u] = 0;
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kLoadSteps; ++u) {
+            const int i = base + u * kThreads;
+            if (i >= total) break;
+            const float scale = scale_of(byte[u]);
+            const bool none = byte[u] == kNoScale;      // (also where the codes are another row's: a key whose value has no scale)
+            float v[4], w[4], y[8];
+            decode4<FMT>(raw[u].x, v);
+            decode4<FMT>(raw[u].y, w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                y[e] = none ? __int_as_float(0x7fffffff) : v[e] * scale;
+                y[4 + e] = none ? __int_as_float(0x7fffffff) : w[e] * scale;
+            }
+            store8(out + (size_t)i * 8, y);
         }
     }
-    const size_t out_row = (size_t)seq * a.pages * a.kv_heads * kPageSize + (size_t)row;
-    store8((T*)a.out[which] + out_row * a.head_dim + part * 8, y);
 }
 
 void check_sizes(const char* who, int kv_heads, int head_dim, int fmt) {
@@ -196,7 +225,7 @@ void kv_quant_store(const void* k_packed, const void* v_packed, DType dt, int T,
     while (lanes * 8 < head_dim) lanes *= 2;
     StoreArgs a{{k_packed, v_packed}, {k_rows, v_rows}, {(uint8_t*)k_pool, (uint8_t*)v_pool}, {(uint8_t*)k_scale, (uint8_t*)v_scale},
                 positions, token_slot, {page_table, slots, table_stride, pool_pages}, kv_heads, head_dim, (long long)T * kv_heads, error_word()};
-    const long long per_block = kThreads / lanes;
+    const long long per_block = kThreads / lanes * kStoreRows;
     const dim3 grid((unsigned)((a.rows_of_each + per_block - 1) / per_block), 2);
     note_launch();
     auto kernel = dt == F32 ? (fmt == QUANT_FP8 ? kv_quant_store_kernel<float, QUANT_FP8> : kv_quant_store_kernel<float, QUANT_INT8>)
@@ -215,13 +244,10 @@ void kv_quant_load(int fmt, const void* k_pool, const void* v_pool, const void* 
         throw std::invalid_argument("kv_quant_load: outputs must be 16-byte aligned and pools 8-byte aligned");
     LoadArgs a{{(const uint8_t*)k_pool, (const uint8_t*)v_pool}, {(const uint8_t*)k_scale, (const uint8_t*)v_scale}, {k_out, v_out}, out_table,
                slot_ids, seq_ends, {page_table, slots, table_stride, pool_pages}, kv_heads, head_dim, pages, whole ? 1 : 0, cu_seqlens, skip_new, attend ? 1 : 0, attend ? window : 0, error_word()};
-    const long long threads = (long long)pages * kv_heads * kPageSize * (head_dim / 8);
-    const long long blocks = (threads + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffffll) throw std::invalid_argument("kv_quant_load: too many pages for one call");
     note_launch();
     auto kernel = dt == F32 ? (fmt == QUANT_FP8 ? kv_quant_load_kernel<float, QUANT_FP8> : kv_quant_load_kernel<float, QUANT_INT8>)
                             : (fmt == QUANT_FP8 ? kv_quant_load_kernel<__nv_bfloat16, QUANT_FP8> : kv_quant_load_kernel<__nv_bfloat16, QUANT_INT8>);
-    launch_kernel("kv_quant_load", kernel, dim3((unsigned)blocks, (unsigned)n_seqs, 2), dim3(kThreads), 0, stream, 1, dependent_launch_enabled(), a);
+    launch_kernel("kv_quant_load", kernel, dim3((unsigned)pages, (unsigned)n_seqs, 2), dim3(kThreads), 0, stream, 1, dependent_launch_enabled(), a);
 }
 
 }  // namespace sm

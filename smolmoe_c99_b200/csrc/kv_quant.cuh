@@ -71,19 +71,13 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
            ((uint32_t)(__float2int_rn(c) & 255) << 16) | ((uint32_t)(__float2int_rn(d) & 255) << 24);
 }
 
-// Two neighbouring codes (16 bits) as two half-precision numbers: exact in both formats.
-__device__ __forceinline__ uint32_t fp8x2_to_half2(uint32_t two) {
-    uint32_t h;
-    asm("{\n\t.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\t}" : "=r"(h) : "r"(two));
-    return h;
-}
-// Four codes (lowest byte first) as two pairs of half-precision numbers. int8: a code plus 128 put into the last bits of
+// Four codes (lowest byte first) as two pairs of half-precision numbers (exact in both formats). int8: a code plus 128 put into the last bits of
 // 1,024.0 gives 1,152 + code; the subtraction is exact.
 template <int FMT>
 __device__ __forceinline__ void decode4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
     if (FMT == QUANT_FP8) {
-        lo = fp8x2_to_half2(codes);
-        hi = fp8x2_to_half2(codes >> 16);
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+            : "=r"(lo), "=r"(hi) : "r"(codes));
     } else {
         const uint32_t u = codes ^ 0x80808080u;
         const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);

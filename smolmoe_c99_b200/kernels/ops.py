@@ -140,7 +140,7 @@ class Ops:
         self.lib.sm_attention_quant.argtypes = [addr, addr] + [num] * 4 + [ctypes.c_float, num, num] + [addr] * 4 + [big, addr, num, num] + \
             [addr] * 3 + [num] * 5 + [addr, big, addr]
         self.lib.sm_attention_quant_supports.argtypes = [num, num, num, big]
-        self.lib.sm_attention_quant_workspace.argtypes, self.lib.sm_attention_quant_workspace.restype = [num, num, num], big
+        self.lib.sm_attention_quant_workspace.argtypes, self.lib.sm_attention_quant_workspace.restype = [num, num, num, num], big
         self._quant_workspaces: dict = {}
         fast = kernels == "fast"
         self.kernels = kernels
@@ -167,6 +167,8 @@ class Ops:
         self.extend_rows_as_decode_tc = 176 if fast else 0
         self.extend_tc_variant = -1     # that kernel with one CTA an SM (0), two (1, head size 64), or as the launcher chooses
         self.quant_rows_tokens = 64     # over an 8-bit cache: sequences that bring more tokens go to the tcgen05 kernel
+        self.quant_cluster: Optional[int] = None     # (a fixed choice, for comparisons)
+        self.quant_line_tiles = 8192
         self.skinny_single_round_above_8 = True
         self.error_flag = torch.zeros(1, dtype=torch.int32, device="cuda")
         self.lib.sm_set_error_word.restype = None
@@ -712,19 +714,18 @@ class Ops:
             tokens = 8 * row_tiles // group
             pairs = kv_heads * (step.n_seqs if most == 1 and limit == most else sum(-(-n // tokens) for n in lens if n <= limit))
             longest = step.max_seq_len if not window else min(step.max_seq_len, window + most)
-            direct = longest <= 256
-            floats = 0
-            if not direct:
-                key = (head_dim <= 64, row_tiles)
+            cluster, floats = self._quant_cluster(pairs, longest, head_dim), 0
+            if not cluster:
+                key = (head_dim <= 64, row_tiles, pairs)
                 floats = self._quant_workspaces.get(key)
                 if floats is None:
-                    floats = self._quant_workspaces[key] = int(self.lib.sm_attention_quant_workspace(head_dim, row_tiles, 0))
+                    floats = self._quant_workspaces[key] = int(self.lib.sm_attention_quant_workspace(head_dim, row_tiles, pairs, 0))
             workspace = torch.empty((floats,), dtype=torch.float32, device=q.device) if floats else None
             self._check(self.lib.sm_attention_quant(
                 q.data_ptr(), out.data_ptr(), step.n_seqs, heads, kv_heads, head_dim, scale, int(window or 0), fmt, cache.k_pool.data_ptr(),
                 cache.v_pool.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pool_pages, cache.page_table.data_ptr(),
                 cache.page_table.shape[0], cache.page_table.shape[1], step.slot_ids.data_ptr(), step.seq_ends.data_ptr(),
-                step.cu_seqlens.data_ptr(), longest, limit, row_tiles, pairs, int(direct), workspace.data_ptr() if floats else None, floats,
+                step.cu_seqlens.data_ptr(), longest, limit, row_tiles, pairs, cluster, workspace.data_ptr() if floats else None, floats,
                 _stream()))
         if limit < max(lens):
             # many tokens: the pages are read back as bfloat16 once (exactly), and the tcgen05 kernel reads those
@@ -735,6 +736,18 @@ class Ops:
                 pages.page_table.shape[1], ctypes.c_longlong(pages.k_pool.shape[0]), int(step.max_seq_len),
                 int(self.extend_tc_variant), limit, _ptr(self.error_flag), _stream()))
         return out
+
+    def _quant_cluster(self, pairs: int, longest: int, head_dim: int) -> int:
+        """CTAs that share a pair (a block of rows of queries and its kv head), or 0 for the line (csrc/attention_quant.cu)."""
+        if self.quant_cluster is not None:
+            return self.quant_cluster
+        tiles = -(-longest // 32)
+        if pairs * tiles > self.quant_line_tiles:
+            return 0
+        cluster = 1
+        while cluster < 8 and 2 * cluster * pairs <= 148 and tiles > 8 * cluster:
+            cluster *= 2
+        return cluster
 
     def attention_extend(self, q, k_packed, v_packed, step, scale, window, cache, cache_written=False):
         """Causal attention of sequences that go on from the cache by any number of tokens: keys and values of
