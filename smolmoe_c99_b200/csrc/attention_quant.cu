@@ -1,7 +1,7 @@
 // Attention over the paged 8-bit cache (kv_quant.cuh) for one or a few new tokens per sequence, bfloat16 queries.
 //
 // What bounds it: reading the cache, and for little of it the trips to memory one after the other. The unit of work is a
-// tile of 32 positions of one kv head, worked on by one warp for a block of rows of queries: (token, head of the group). A
+// tile of 32 or 64 positions of one kv head, worked on by one warp for a block of rows of queries: (token, head of the group). A
 // pair is a block of rows and its kv head; its tiles are its sequence's. Two ways of sharing the tiles out:
 //  - clusters (little work): the eight warps of each of 1 to 8 CTAs share the tiles of one pair and put their results
 //    together through shared memory, the CTAs through the leader's (distributed shared memory). One launch, no workspace.
@@ -46,7 +46,9 @@ namespace {
 
 using namespace tc5;
 
-constexpr int kTile = 32;                // positions
+// Positions of a tile: in clusters, and of the line, where a page (64) gives a warp twice the independent work at once.
+constexpr int kClusterTile = 32;
+__host__ __device__ constexpr int line_tile(int row_tiles) { return row_tiles == 1 ? 64 : 32; }
 constexpr int kWarps = 8;                // of a CTA of a cluster
 constexpr int kMaxCluster = 8;
 constexpr int kWaitCode = 34;            // error word: a wait ran out
@@ -73,7 +75,7 @@ struct AttnArgs {
     int seqs, heads, kv_heads, head_dim, window;
     int most_new;                        // sequences with more new tokens are not this kernel's
     int block_tokens;                    // tokens of a block of rows
-    int cluster, stages;                 // CTAs of a cluster (0: the line); tiles a warp keeps in flight
+    int cluster, stages, tile;           // CTAs of a cluster (0: the line); tiles a warp keeps in flight; positions of a tile
     float scale_log2;
     Cut* cuts;                           // the line: [pairs]
     float* parts;                        // the line: [warps][2][rows][padded head size + 4]: values, then maximum and sum
@@ -97,8 +99,8 @@ __device__ __forceinline__ Seq seq_from(const AttnArgs& a, int start, int n) {
     s.n = n;
     s.start = start;
     s.blocks = n <= 0 || n > a.most_new || start < 0 ? 0 : (n + a.block_tokens - 1) / a.block_tokens;
-    s.first_tile = (a.window > 0 ? max(0, start - a.window + 1) : 0) / kTile;
-    s.tiles = (start + n - 1) / kTile - s.first_tile + 1;
+    s.first_tile = (a.window > 0 ? max(0, start - a.window + 1) : 0) / a.tile;
+    s.tiles = (start + n - 1) / a.tile - s.first_tile + 1;
     return s;
 }
 
@@ -175,6 +177,14 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
+__device__ __forceinline__ int lds_u8(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr));
+    return (int)v;
+}
+__device__ __forceinline__ void sts_zero16(uint32_t addr) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
+}
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -187,15 +197,16 @@ __device__ __forceinline__ int row_position(int r) { return r < 8 ? r : 8 + ((r 
 // What a warp knows of the pair it works on, and what it has added up. NB: blocks of 64 of the head dimension; NHT: tiles
 // of 8 rows of queries; BOX: head_dim is 64 * NB. A thread holds, of each tile of rows, rows 2 q4 and 2 q4 + 1 (q4 = lane % 4)
 // and, of each 16 positions or dimensions, two (of positions: row_position(g) and row_position(g + 8), g = lane / 4).
-template <int NB, int NHT, int FMT, bool BOX>
+template <int NB, int NHT, int FMT, bool BOX, int KT>
 struct Rows {
-    static constexpr int HDP = NB * 64, CH = HDP / 16, MT = kTile / 16;    // padded head size, pieces of 16 dimensions
+    static constexpr int HDP = NB * 64, CH = HDP / 16, MT = KT / 16;       // padded head size, pieces of 16 dimensions
     uint32_t qf[CH][NHT][2];             // queries as half precision, scaled by a power of two to at most 2^11
     float q_scale[NHT][2];               // undoes the power of two, times scale * log2(e)
     float ot[CH][NHT][4];
     float run_m[NHT][2], run_l[NHT][2];
     int top_exponent;                    // E, as a byte; 0: none yet
     int first_pos, tokens, lowest;       // position of the first row's token, tokens, the lowest position that any sees
+    uint32_t k_lane, v_lane;             // offsets in a tile of what this lane names in an ldmatrix of keys, of values
 
     // Row 0's place in q is `row0` (of rows of head_dim), row r's r / group tokens of `heads` rows and r % group further.
     __device__ __forceinline__ void begin(const AttnArgs& a, size_t row0, int first, int n_tokens) {
@@ -205,6 +216,11 @@ struct Rows {
         tokens = n_tokens;
         lowest = a.window > 0 ? max(0, first - a.window + 1) : 0;
         top_exponent = 0;
+        // the row this lane names of 16 keys, and of a 16 x 16 block of values; lanes from 16 on name the next piece
+        const int which = lane >> 4, at = lane & 15;
+        const int k_row = row_position((lane & 7) + ((lane >> 3) & 1) * 8), v_row = row_position(2 * (at >> 2) + (at & 1) + ((at >> 1) & 1) * 8);
+        k_lane = piece_at(hd, k_row, which);
+        v_lane = (uint32_t)(KT * hd) + piece_at(hd, v_row, which);
 #pragma unroll
         for (int nh = 0; nh < NHT; ++nh) {
             const int r = nh * 8 + g;
@@ -246,40 +262,38 @@ struct Rows {
         return (uint32_t)(row * hd + (piece << 4));
     }
 
-    // One tile: positions key0 .. key0 + 31, codes of keys and values at `slot`, exponents at ks and vs.
-    __device__ __forceinline__ void tile(const AttnArgs& a, int key0, unsigned char* slot, const uint8_t* ks, const uint8_t* vs) {
+    // One tile: positions key0 .. key0 + KT - 1; shared-memory addresses of its codes (keys, then values) and exponents.
+    __device__ __forceinline__ void tile(const AttnArgs& a, int key0, uint32_t codes, uint32_t exponents) {
         const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
-        const int hd = BOX ? HDP : a.head_dim, pieces = hd / 16, tile_bytes = kTile * hd;
+        const int hd = BOX ? HDP : a.head_dim, pieces = hd / 16;
         const int last_pos = first_pos + tokens - 1;
-        const int pos_lo = g, pos_hi = 8 + (g ^ 4);
-        // the row this lane names in an ldmatrix of keys, and its piece; of a 16 x 16 block of values
-        const int k_row = row_position((lane & 7) + ((lane >> 3) & 1) * 8), which = lane >> 4, v_at = lane & 15;
-        const int v_row = row_position(2 * (v_at >> 2) + (v_at & 1) + ((v_at >> 1) & 1) * 8);
-        const uint32_t kt = smem_u32(slot);
-        const uint32_t ka = kt + piece_at(hd, k_row, which), va = kt + (uint32_t)tile_bytes + piece_at(hd, v_row, which);
-        // ... of pieces c and c + 1 (c even) of the 16 rows from 16 mt on. In a box the pieces of a row are exchanged by an
-        // exclusive or with bits of the row that 16 mt does not change.
+        const uint32_t ks_lo = exponents + (uint32_t)g, ks_hi = exponents + (uint32_t)(8 + (g ^ 4));   // of the positions this thread holds
+        const uint32_t ka = codes + k_lane, va = codes + v_lane;
+        // The address for pieces c and c + 1 (c even) of the 16 rows from 16 mt on. In a box the pieces of a row are exchanged
+        // by an exclusive or with bits of the row that 16 mt does not change.
         auto fragment_at = [&](uint32_t lane_at, int mt, int c) -> uint32_t {
             if (BOX) return (lane_at ^ (uint32_t)(c << 4)) + (uint32_t)(mt * 16 * HDP);
+            const int which = lane >> 4;
             return lane_at + (uint32_t)(mt * 16 * hd) + (uint32_t)((min(c + which, pieces - 1) - which) << 4);     // (an odd last piece is read twice)
         };
         // every row sees every position of the tile, or a mask is needed
-        const bool masked = key0 + kTile - 1 > first_pos || (a.window > 0 && key0 <= last_pos - a.window);
-        int top = vs[lane];
+        const bool masked = key0 + KT - 1 > first_pos || (a.window > 0 && key0 <= last_pos - a.window);
+        int top = lds_u8(exponents + KT + lane), top2 = KT == 64 ? lds_u8(exponents + KT + 32 + lane) : 0;
         if (masked) {
             const int from = max(lowest - key0, 0), to = last_pos + 1 - key0;    // positions some row sees: [from, to)
             if (lane < from || lane >= to) top = 0;
-            if (from > 0 || to < kTile) {
+            if (lane + 32 < from || lane + 32 >= to) top2 = 0;
+            if (from > 0 || to < KT) {
                 // value rows that no row sees may hold bytes that were never written: zeros (times zero weights)
-                for (int idx = lane; idx < kTile * pieces; idx += 32) {
+                for (int idx = lane; idx < KT * pieces; idx += 32) {
                     const int row = idx / pieces, piece = idx - row * pieces;
-                    if (row < from || row >= to) *reinterpret_cast<uint4*>(slot + tile_bytes + piece_at(hd, row, piece)) = make_uint4(0, 0, 0, 0);
+                    if (row < from || row >= to) sts_zero16(codes + (uint32_t)(KT * hd) + piece_at(hd, row, piece));
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             }
         }
-        if (top == kNoScale) top = 0;
+        top = max(top == kNoScale ? 0 : top, top2 == kNoScale ? 0 : top2);
         // S^T = K Q^T
         float st[MT][NHT][4];
 #pragma unroll
@@ -304,29 +318,48 @@ struct Rows {
                 }
             }
         }
-        // scores (in powers of two), mask, and whether any exceeds its row's maximum so far
-        bool moved = top > top_exponent;
-        const int group = a.heads / a.kv_heads;
+        // scores (in powers of two)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            const float f0 = scale_of(ks[mt * 16 + pos_lo]), f1 = scale_of(ks[mt * 16 + pos_hi]);
+            const float f0 = scale_of(lds_u8(ks_lo + mt * 16)), f1 = scale_of(lds_u8(ks_hi + mt * 16));
+#pragma unroll
+            for (int nh = 0; nh < NHT; ++nh) {
+                st[mt][nh][0] *= f0 * q_scale[nh][0];
+                st[mt][nh][1] *= f0 * q_scale[nh][1];
+                st[mt][nh][2] *= f1 * q_scale[nh][0];
+                st[mt][nh][3] *= f1 * q_scale[nh][1];
+            }
+        }
+        if (masked) {
+            const int group = a.heads / a.kv_heads;
 #pragma unroll
             for (int nh = 0; nh < NHT; ++nh)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x = st[mt][nh][e] * ((e & 2) ? f1 : f0) * q_scale[nh][e & 1];
-                    if (masked) {
-                        const int key = key0 + mt * 16 + ((e & 2) ? pos_hi : pos_lo);
-                        const int pos = first_pos + min((nh * 8 + 2 * q4 + (e & 1)) / group, tokens - 1);
-                        if (key > pos || (a.window > 0 && key <= pos - a.window)) x = -CUDART_INF_F;
+                for (int e = 0; e < 2; ++e) {
+                    // the row sees the positions of the tile from `lo` to `hi`
+                    const int hi = first_pos + min((nh * 8 + 2 * q4 + e) / group, tokens - 1) - key0, lo = a.window > 0 ? hi - a.window + 1 : 0;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        const int x = mt * 16 + g, y = mt * 16 + 8 + (g ^ 4);
+                        if (x > hi || x < lo) st[mt][nh][e] = -CUDART_INF_F;
+                        if (y > hi || y < lo) st[mt][nh][e + 2] = -CUDART_INF_F;
                     }
-                    st[mt][nh][e] = x;
-                    moved |= x > run_m[nh][e & 1];
                 }
         }
+        // whether any score exceeds its row's maximum so far
+        bool moved = top > top_exponent;
+#pragma unroll
+        for (int nh = 0; nh < NHT; ++nh)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x = fmaxf(st[0][nh][e], st[0][nh][e + 2]);
+#pragma unroll
+                for (int mt = 1; mt < MT; ++mt) x = fmax3(x, st[mt][nh][e], st[mt][nh][e + 2]);
+                moved |= x > run_m[nh][e];
+            }
         if (__any_sync(0xffffffffu, moved)) {
             // a larger maximum or exponent: what has been added up is put on the new footing (most tiles of a long
-            // sequence bring neither, and then no maximum is looked for)
+            // sequence bring neither, and then no maximum is looked for among the threads)
             top = max((int)__reduce_max_sync(0xffffffffu, (unsigned)top), top_exponent);
             const float less = top_exponent == 0 ? 0.f : power_of_two(-min(top - top_exponent, 126));
             top_exponent = top;
@@ -337,7 +370,7 @@ struct Rows {
                 for (int e = 0; e < 2; ++e) {
                     float x = run_m[nh][e];
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) x = fmaxf(x, fmaxf(st[mt][nh][e], st[mt][nh][e + 2]));
+                    for (int mt = 0; mt < MT; ++mt) x = fmax3(x, st[mt][nh][e], st[mt][nh][e + 2]);
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -350,28 +383,38 @@ struct Rows {
                 for (int c = 0; c < CH; ++c) { ot[c][nh][0] *= f[0]; ot[c][nh][1] *= f[1]; ot[c][nh][2] *= f[0]; ot[c][nh][3] *= f[1]; }
             }
         }
-        // P = 2^(score - maximum), and the weights P * 2^(e - E + 15) as the B operand
-        uint32_t pb[MT][NHT][2];
+        // P = 2^(score - maximum), summed up
+        float ref[NHT][2];
+#pragma unroll
+        for (int nh = 0; nh < NHT; ++nh)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) ref[nh][e] = run_m[nh][e] == -CUDART_INF_F ? 0.f : run_m[nh][e];
+        const int shift = 142 - top_exponent;        // 127 + 15 - E
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            const int b0 = vs[mt * 16 + pos_lo], b1 = vs[mt * 16 + pos_hi];
-            const float w0 = b0 == kNoScale ? CUDART_NAN_F : __int_as_float(max(b0 - top_exponent + 142, 0) << 23);
-            const float w1 = b1 == kNoScale ? CUDART_NAN_F : __int_as_float(max(b1 - top_exponent + 142, 0) << 23);
+            // the weights P * 2^(e - E + 15)
+            const int b0 = lds_u8(ks_lo + KT + mt * 16), b1 = lds_u8(ks_hi + KT + mt * 16);
+            const float w0 = b0 == kNoScale ? CUDART_NAN_F : __int_as_float(max(b0 + shift, 0) << 23);
+            const float w1 = b1 == kNoScale ? CUDART_NAN_F : __int_as_float(max(b1 + shift, 0) << 23);
 #pragma unroll
-            for (int nh = 0; nh < NHT; ++nh) {
-                float p[4];
+            for (int nh = 0; nh < NHT; ++nh)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float x = st[mt][nh][e];
-                    const float ref = run_m[nh][e & 1] == -CUDART_INF_F ? 0.f : run_m[nh][e & 1];
-                    const float v = ex2_approx(x - ref);
+                    const float v = ex2_approx(st[mt][nh][e] - ref[nh][e & 1]);
                     run_l[nh][e & 1] += v;
-                    p[e] = masked && x == -CUDART_INF_F ? 0.f : v * ((e & 2) ? w1 : w0);
+                    // (a weight of zero stays zero whatever the byte of a position that is not seen says)
+                    st[mt][nh][e] = masked && st[mt][nh][e] == -CUDART_INF_F ? 0.f : v * ((e & 2) ? w1 : w0);
                 }
-                pb[mt][nh][0] = movmatrix_trans(pack_half2(p[0], p[1]));
-                pb[mt][nh][1] = movmatrix_trans(pack_half2(p[2], p[3]));
-            }
         }
+        // ... as the B operand
+        uint32_t pb[MT][NHT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int nh = 0; nh < NHT; ++nh) {
+                pb[mt][nh][0] = movmatrix_trans(pack_half2(st[mt][nh][0], st[mt][nh][1]));
+                pb[mt][nh][1] = movmatrix_trans(pack_half2(st[mt][nh][2], st[mt][nh][3]));
+            }
         // O^T += V^T P^T
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -409,30 +452,40 @@ struct Rows {
 };
 
 // A warp's tiles: places, copies and waits. A place is a row of the pools: pages of kv heads of 64 positions.
-template <bool BOX>
+template <bool BOX, int KT>
 struct Ring {
     const CUtensorMap *map_k, *map_v;
-    unsigned char* slots;                // [stages][keys | values]
-    unsigned char* scales;               // [stages][exponents of keys, of values]
     uint64_t* bars;                      // [stages]
-    int stages, tile_bytes, hd, tiles;   // tiles: the warp's
+    uint32_t slots;                      // shared-memory address of [stages][keys | values]
+    uint32_t scales;                     // ... of [stages][exponents of keys, of values]
+    int stages, hd, tiles;               // tiles: the warp's
     int issued, used, stage;
     uint32_t parity;
 
+    __device__ __forceinline__ uint32_t codes_at(int s) const { return slots + (uint32_t)(s * 2 * KT * hd); }
+    __device__ __forceinline__ uint32_t scales_at(int s) const { return scales + (uint32_t)(s * 2 * KT); }
     __device__ __forceinline__ void request(const AttnArgs& a, int place, int into) {
-        const int lane = threadIdx.x & 31;
-        unsigned char* slot = slots + (size_t)into * 2 * tile_bytes;
-        uint64_t* bar = &bars[into];
-        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(2 * tile_bytes + 2 * kTile));
-        __syncwarp();
-        if (lane < 2) {
-            unsigned char* dst = slot + lane * tile_bytes;
-            if (BOX) tma_load_2d(dst, lane ? map_v : map_k, 0, place, bar);
-            else bulk_load(dst, (lane ? a.v_codes : a.k_codes) + (size_t)place * hd, (uint32_t)tile_bytes, bar);
-        } else if (lane < 4) {
-            bulk_load(scales + (into * 2 + lane - 2) * kTile, (lane == 3 ? a.v_scale : a.k_scale) + place, kTile, bar);
+        // (one lane for all four copies: those of several lanes would be issued one lane after the other)
+        if ((threadIdx.x & 31) == 0) {
+            const uint32_t bar = smem_u32(&bars[into]), dst = codes_at(into), sc = scales_at(into), bytes = (uint32_t)(KT * hd);
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2 * bytes + 2 * KT) : "memory");
+            if (BOX) {
+                asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                             ::"r"(dst), "l"(map_k), "r"(0), "r"(place), "r"(bar) : "memory");
+                asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                             ::"r"(dst + bytes), "l"(map_v), "r"(0), "r"(place), "r"(bar) : "memory");
+            } else {
+                bulk(dst, a.k_codes + (size_t)place * hd, bytes, bar);
+                bulk(dst + bytes, a.v_codes + (size_t)place * hd, bytes, bar);
+            }
+            bulk(sc, a.k_scale + place, KT, bar);
+            bulk(sc + KT, a.v_scale + place, KT, bar);
         }
         ++issued;
+    }
+    static __device__ __forceinline__ void bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
     }
     // Waits for the next tile (false: the limit ran out).
     __device__ __forceinline__ bool wait(const AttnArgs& a) {
@@ -455,7 +508,7 @@ struct Ring {
 };
 // The row of the pools of tile t (from the sequence's first) of sequence i and kv head kvh.
 __device__ __forceinline__ int place_of(const AttnArgs& a, const SeqTable& table, int i, int tile, int kvh) {
-    const int key = tile * kTile;
+    const int key = tile * a.tile;
     int page = a.pages.at(table.slot[i], key / kPageSize);
     if (page < 0) {
         if (a.error) atomicExch(a.error, kBadPlaceInAttention);
@@ -478,13 +531,13 @@ __device__ __forceinline__ float part_factor(float m, float l, float top) {
 template <int NB, int NHT, int FMT, bool BOX>
 __global__ void __launch_bounds__(kWarps * 32) attention_quant_cluster_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                               const __grid_constant__ CUtensorMap map_v, AttnArgs a) {
-    using R_ = Rows<NB, NHT, FMT, BOX>;
+    using R_ = Rows<NB, NHT, FMT, BOX, kClusterTile>;
     constexpr int HDP = R_::HDP, CH = R_::CH, LD = HDP + 4, R = 8 * NHT, kThreads = kWarps * 32;    // LD: a row of results (conflict-free)
     extern __shared__ __align__(16) unsigned char smem_raw[];
     namespace cg = cooperative_groups;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
     const int hd = BOX ? HDP : a.head_dim, group = a.heads / a.kv_heads, S = a.stages, C = a.cluster;
-    const size_t ring_bytes = (size_t)kWarps * S * 2 * kTile * hd;
+    const size_t ring_bytes = (size_t)kWarps * S * 2 * kClusterTile * hd;
     unsigned char* ring0 = BOX ? reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023) : smem_raw;
     float* wo = reinterpret_cast<float*>(ring0 + ring_bytes);       // [warp][R][LD] values
     float* wm = wo + kWarps * R * LD;                               // [warp][R] maxima, then the warps' factors
@@ -492,11 +545,11 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_cluster_kernel(co
     float* parts = wl + kWarps * R;                                 // the leader's: [C][R][LD] values, maximum, sum
     float* end_of_parts = parts + (C > 1 ? C : 1) * R * LD;
     unsigned char* scales = reinterpret_cast<unsigned char*>(end_of_parts);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(scales + (size_t)kWarps * S * 2 * kTile);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(scales + (size_t)kWarps * S * 2 * kClusterTile);
     const SeqTable table(reinterpret_cast<int*>(bars + kWarps * S), a.seqs);
 
-    Ring<BOX> ring{&map_k, &map_v, ring0 + (size_t)warp * S * 2 * kTile * hd, scales + (size_t)warp * S * 2 * kTile, bars + warp * S,
-                   S, kTile * hd, hd, 0, 0, 0, 0, 0u};
+    Ring<BOX, kClusterTile> ring{&map_k, &map_v, bars + warp * S, smem_u32(ring0 + (size_t)warp * S * 2 * kClusterTile * hd),
+                                 smem_u32(scales + (size_t)warp * S * 2 * kClusterTile), S, hd, 0, 0, 0, 0, 0u};
     if (lane == 0) {
         for (int s = 0; s < S; ++s) mbar_init(&ring.bars[s], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -530,8 +583,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_cluster_kernel(co
     bool ok = true;
     for (int k = 0; k < ring.tiles; ++k) {
         if (!(ok = ring.wait(a))) break;
-        const uint8_t* ks = ring.scales + ring.stage * 2 * kTile;
-        state.tile(a, (t_lo + warp + kWarps * k) * kTile, ring.slots + (size_t)ring.stage * 2 * ring.tile_bytes, ks, ks + kTile);
+        state.tile(a, (t_lo + warp + kWarps * k) * kClusterTile, ring.codes_at(ring.stage), ring.scales_at(ring.stage));
         __syncwarp();            // every lane has read the slot
         if (k + S < ring.tiles) request(k + S, ring.stage);
         ring.next();
@@ -612,17 +664,18 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_cluster_kernel(co
 template <int NB, int NHT, int FMT, bool BOX>
 __global__ void __launch_bounds__(line_warps(NHT) * 32, 1) attention_quant_line_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                                        const __grid_constant__ CUtensorMap map_v, AttnArgs a) {
-    using R_ = Rows<NB, NHT, FMT, BOX>;
-    constexpr int HDP = R_::HDP, CH = R_::CH, LD = HDP + 4, R = 8 * NHT, W = line_warps(NHT);
+    constexpr int KT = line_tile(NHT), W = line_warps(NHT);
+    using R_ = Rows<NB, NHT, FMT, BOX, KT>;
+    constexpr int HDP = R_::HDP, CH = R_::CH, LD = HDP + 4, R = 8 * NHT;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
     const int hd = BOX ? HDP : a.head_dim, group = a.heads / a.kv_heads, S = a.stages;
     unsigned char* ring0 = BOX ? reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023) : smem_raw;
-    unsigned char* scales = ring0 + (size_t)W * S * 2 * kTile * hd;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(scales + (size_t)W * S * 2 * kTile);
+    unsigned char* scales = ring0 + (size_t)W * S * 2 * KT * hd;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(scales + (size_t)W * S * 2 * KT);
     const SeqTable table(reinterpret_cast<int*>(bars + W * S), a.seqs);
-    Ring<BOX> ring{&map_k, &map_v, ring0 + (size_t)warp * S * 2 * kTile * hd, scales + (size_t)warp * S * 2 * kTile, bars + warp * S,
-                   S, kTile * hd, hd, 0, 0, 0, 0, 0u};
+    Ring<BOX, KT> ring{&map_k, &map_v, bars + warp * S, smem_u32(ring0 + (size_t)warp * S * 2 * KT * hd),
+                       smem_u32(scales + (size_t)warp * S * 2 * KT), S, hd, 0, 0, 0, 0, 0u};
     if (lane == 0) {
         for (int s = 0; s < S; ++s) mbar_init(&ring.bars[s], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -663,8 +716,7 @@ __global__ void __launch_bounds__(line_warps(NHT) * 32, 1) attention_quant_line_
         state.begin(a, (size_t)first_token * a.heads + (size_t)kvh * group, s.start + token0, tokens);
         for (; u < part_end && ok; ++u) {
             if (!(ok = ring.wait(a))) break;
-            const uint8_t* ks = ring.scales + ring.stage * 2 * kTile;
-            state.tile(a, (s.first_tile + (u - pair_at)) * kTile, ring.slots + (size_t)ring.stage * 2 * ring.tile_bytes, ks, ks + kTile);
+            state.tile(a, (s.first_tile + (u - pair_at)) * KT, ring.codes_at(ring.stage), ring.scales_at(ring.stage));
             __syncwarp();        // every lane has read the slot
             if (u - u_lo + S < ring.tiles) request(u - u_lo + S, ring.stage);
             ring.next();
@@ -782,12 +834,12 @@ constexpr size_t kRoom = 226 * 1024;     // shared memory of an SM, less what th
 template <int NB, int NHT, int FMT, bool BOX>
 void launch(AttnArgs a, const CUtensorMap& mk, const CUtensorMap& mv, const LaunchSizes& sizes, cudaStream_t stream) {
     constexpr int HDP = NB * 64, R = 8 * NHT, LD = HDP + 4;
-    const size_t slot = (size_t)2 * kTile * a.head_dim + 2 * kTile + sizeof(uint64_t);      // codes, exponents, a barrier
+    const size_t slot = (size_t)2 * a.tile * (a.head_dim + 1) + sizeof(uint64_t);      // codes, exponents, a barrier
     const size_t table = (BOX ? 1024 : 0) + seq_table_bytes(a.seqs);
     if (a.cluster) {
         const size_t fixed = table + ((size_t)kWarps * R * (LD + 2) + (size_t)a.cluster * R * LD) * sizeof(float);
         // as many tiles in flight as a warp gets, at most what is left
-        const int tiles = ((sizes.max_len + kTile - 1) / kTile + 1 + a.cluster - 1) / a.cluster;
+        const int tiles = ((sizes.max_len + a.tile - 1) / a.tile + 1 + a.cluster - 1) / a.cluster;
         a.stages = std::max(1, std::min({(tiles + kWarps - 1) / kWarps, kMaxStages, (int)((kRoom - fixed) / (kWarps * slot))}));
         static bool prepared[kDevices] = {};
         auto kernel = attention_quant_cluster_kernel<NB, NHT, FMT, BOX>;
@@ -859,7 +911,8 @@ void attention_quant(const void* q, void* out, int n_seqs, int heads, int kv_hea
     if (workspace_floats < attention_quant_workspace(head_dim, row_tiles, pairs, cluster)) throw std::invalid_argument("attention_quant: the workspace is too small");
     AttnArgs a{(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)k_pool, (const uint8_t*)v_pool, (const uint8_t*)k_scale,
                (const uint8_t*)v_scale, {page_table, slots, table_stride, pool_pages}, slot_ids, seq_ends, cu_seqlens, n_seqs, heads,
-               kv_heads, head_dim, window, most_new, 8 * row_tiles / group, cluster, 0, scale * 1.4426950408889634f, (Cut*)workspace,
+               kv_heads, head_dim, window, most_new, 8 * row_tiles / group, cluster, 0,
+               cluster ? kClusterTile : line_tile(row_tiles), scale * 1.4426950408889634f, (Cut*)workspace,
                workspace + (cluster ? 0 : (long long)pairs * (long long)(sizeof(Cut) / sizeof(float))), error_word()};
     CUtensorMap mk{}, mv{};
     if (head_dim == 64 || head_dim == 128) {
@@ -867,9 +920,9 @@ void attention_quant(const void* q, void* out, int n_seqs, int heads, int kv_hea
         const CUtensorMapSwizzle swizzle = head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
         const uint64_t rows = (uint64_t)pool_pages * kv_heads * kPageSize;
         mk = tiled_map_2d("attention_quant", CU_TENSOR_MAP_DATA_TYPE_UINT8, k_pool, (uint64_t)head_dim, rows, (uint64_t)head_dim, (uint32_t)head_dim,
-                          kTile, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+                          (uint32_t)a.tile, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
         mv = tiled_map_2d("attention_quant", CU_TENSOR_MAP_DATA_TYPE_UINT8, v_pool, (uint64_t)head_dim, rows, (uint64_t)head_dim, (uint32_t)head_dim,
-                          kTile, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+                          (uint32_t)a.tile, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
     }
     const LaunchSizes sizes{pairs, a.block_tokens * group, max_len};
     if (fmt == QUANT_FP8) launch_fmt<QUANT_FP8>(a, row_tiles, mk, mv, sizes, stream);
