@@ -1,0 +1,563 @@
+// Causal attention of a chunk of new tokens per sequence over pages of bfloat16 keys and values (what an 8-bit cache stands
+// for, read back page by page), head sizes 64 and 128, on the 5th-generation tensor cores.
+//
+// Rows of queries are (token, head of the group): the heads that share keys and values share a tile, so a tile of 128 rows is
+// 128 / group tokens, keys are read once for all of them, and few rows lie beyond a tile's causal border. A CTA has two
+// such tiles, A and B, under way: while the threads of one turn scores into weights, the tensor cores work for the other.
+//   S_X = Q_X K^T    tcgen05.mma 128 x 128 x head_dim, both operands in shared memory, S (float) in tensor memory;
+//   P_X = 2^(S * scale - reference) as bfloat16, back into tensor memory over the scores (a thread per row);
+//   O_X += P_X V     tcgen05.mma 128 x head_dim x 128, P_X from tensor memory, V as it lies in memory (MN-major).
+// In order on the tensor cores: S_A S_B | P_A: PV_A, next S_A | P_B: PV_B, next S_B | ... A row's reference is lazy: it moves
+// when a tile's maximum exceeds it by more than 2^8, and only then is the accumulator rescaled; the scores of a tile come
+// after the PV of the tile before, so whoever has waited for them may touch the accumulator.
+//
+// Work is shared out as a line: the tiles of 128 keys of all pairs (two query tiles of one kv head), one after the other; each
+// CTA of a grid of one an SM takes an equal run. What a run cuts is left as float accumulators, references and sums in a
+// workspace and joined by a second kernel in the order of the line. So 512 tokens of 14 heads onto 8,000, 30 pairs, fill
+// 148 SMs. Lengths are read on the device: a captured launch follows a growing sequence.
+//
+// Every wait on an mbarrier is bounded; a wait that runs out records a code in *error and the CTA leaves without writing.
+#include <math_constants.h>
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+
+#include "common.cuh"
+#include "drain.cuh"
+#include "kernels.h"
+#include "kv_quant.cuh"
+#include "launch.cuh"
+#include "tcgen05.cuh"
+
+namespace sm {
+
+namespace {
+
+using namespace tc5;
+
+constexpr int kRows = 128, kKeys = 128;
+constexpr int kRowThreads = 256;            // one a row: warps 0-3 tile A, 4-7 tile B
+constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr int kThreads = 320;
+constexpr int kBlockBytes = 128 * 128;      // 128 rows of 128 bytes: one swizzled block of 64 bfloat16 columns
+constexpr int kMaxSeqs = 1024, kMaxBlocks = 2048;
+
+__host__ __device__ constexpr int stages_of(int head_dim) { return head_dim == 64 ? 4 : 2; }
+
+// What the CTA that begins a pair leaves for the join, by the pair's number.
+struct ChunkCut {
+    int first_token, kv_head, tokens, first, last;     // tokens 0: the pair is not cut; CTAs
+    int pad[3];
+};
+
+struct ChunkArgs {
+    __nv_bfloat16* out;                  // [T, heads, HD]
+    const int32_t* seq_ends;             // [seqs] lengths after the step
+    const int32_t* cu;                   // [seqs + 1]
+    int seqs, heads, kv_heads, window, skip_new, pages;    // pages: of each sequence in the pools
+    int tile_tokens;                     // tokens of a tile of rows
+    int blocks;                          // what the host says there are
+    float scale_log2;
+    ChunkCut* cuts;                      // [pairs]
+    float* parts;                        // [CTAs][2][2 tiles][HD + 2][128 rows]
+    int* error;
+};
+
+// The reduction dimension of V is its rows: an "MN-major" operand with 128-byte swizzle.
+__device__ __forceinline__ uint64_t smem_desc_rows(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFF) >> 4) | (uint64_t)(kBlockBytes >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// D += A B with A in tensor memory (two bfloat16 a column, a lane a row).
+__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st32_raw(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+           "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A block: two tiles of rows of one sequence, for every kv head a pair of the line. Tiles of keys it sees: first .. first + n - 1.
+struct Block {
+    int seq, token0, tokens, start;      // first token among the sequence's new ones, tokens (of both tiles), position of new token 0
+    int first_tile, tiles;
+};
+__device__ __forceinline__ Block block_of(const ChunkArgs& a, int seq, int index) {
+    Block b;
+    const int n = a.cu[seq + 1] - a.cu[seq];
+    b.seq = seq;
+    b.start = a.seq_ends[seq] - n;
+    b.token0 = index * 2 * a.tile_tokens;
+    b.tokens = min(2 * a.tile_tokens, n - b.token0);
+    const int lowest = a.window > 0 ? max(0, b.start + b.token0 - a.window + 1) : 0;
+    b.first_tile = lowest / kKeys;
+    b.tiles = (b.start + b.token0 + b.tokens - 1) / kKeys - b.first_tile + 1;
+    return b;
+}
+// The last i with before[i] <= x.
+__device__ __forceinline__ int find_last(const int* before, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (before[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+// before[i] = the sum of values 0 .. i - 1 (value(i) is asked for by one thread), before[n] the total; all threads call it.
+template <typename F>
+__device__ void prefix_sums(int* before, int n, F value) {
+    __shared__ int warp_total[kThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int carry = 0;
+    for (int base = 0; base < n; base += kThreads) {
+        const int i = base + threadIdx.x, mine = i < n ? value(i) : 0;
+        int run = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += x;
+        }
+        if (lane == 31) warp_total[warp] = run;
+        __syncthreads();
+        int at = carry;
+        for (int w = 0; w < kThreads / 32; ++w) {
+            if (w < warp) at += warp_total[w];
+            carry += warp_total[w];
+        }
+        if (i < n) before[i] = at + run - mine;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) before[n] = carry;
+    __syncthreads();
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                      const __grid_constant__ CUtensorMap map_v, ChunkArgs a, int least_run) {
+    constexpr int DB = HD / 64, NS = stages_of(HD);
+    constexpr int kTileBytes = DB * kBlockBytes;         // a tile of queries, of keys or of values
+    constexpr uint32_t kTmemO = 256;                     // columns: S_A 0, S_B 128, O_A 256, O_B 384
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* q_s = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);   // [2 tiles][DB][128 rows][128 B]
+    uint8_t* k_s = q_s + 2 * kTileBytes;                 // [NS][DB][128 keys][128 B]
+    uint8_t* v_s = k_s + NS * kTileBytes;                // [NS]
+    uint64_t* bars = (uint64_t*)(v_s + NS * kTileBytes);
+    uint64_t* q_full = bars;                             // the segment's queries have landed
+    uint64_t* s_full = bars + 1;                         // [2] scores are in tensor memory (and PV of the tile before is done)
+    uint64_t* p_full = bars + 3;                         // [2] weights are in tensor memory
+    uint64_t* o_full = bars + 5;                         // [2] the segment's last PV is done
+    uint64_t* drain_bar = bars + 7;
+    uint64_t *k_full = bars + 8, *k_empty = k_full + NS, *v_full = k_empty + NS, *v_empty = v_full + NS;
+    uint32_t* tmem_slot = (uint32_t*)(bars + 8 + 4 * NS);
+    volatile int* failed = (volatile int*)(tmem_slot + 1);
+    int* blocks_before = (int*)(tmem_slot + 2);          // [seqs + 1] blocks before a sequence
+    int* tiles_before = blocks_before + a.seqs + 1;      // [blocks + 1] tiles of the line before a block
+
+    const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads, tile_rows = a.tile_tokens * group;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 1); mbar_init(&p_full[x], kRows); mbar_init(&o_full[x], 1); }
+        mbar_init(drain_bar, 1);
+        for (int i = 0; i < 4 * NS; ++i) mbar_init(&k_full[i], 1);
+        *failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
+    // the rows of the query tiles that no copy fills: zeros
+    for (int i = threadIdx.x; i < 2 * DB * (kRows - tile_rows) * 8; i += kThreads) {
+        const int block = i / ((kRows - tile_rows) * 8), rest = i - block * (kRows - tile_rows) * 8;
+        *reinterpret_cast<uint4*>(q_s + block * kBlockBytes + tile_rows * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();              // queries, pages and lengths come from the kernels before
+    pdl_launch_dependents();
+
+    prefix_sums(blocks_before, a.seqs, [&](int i) {
+        const int n = a.cu[i + 1] - a.cu[i];
+        return n > a.skip_new && n <= a.seq_ends[i] ? (n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens) : 0;
+    });
+    // (lengths on the device that are not those on the host: nothing is done)
+    const int blocks = blocks_before[a.seqs] == a.blocks ? a.blocks : 0;
+    if (blocks == 0 && blockIdx.x == 0) {
+        if (threadIdx.x == 0 && a.error) atomicExch(a.error, kBadPlaceInAttention);
+        for (int i = threadIdx.x; i < a.blocks * a.kv_heads; i += kThreads) a.cuts[i].tokens = 0;
+    }
+    prefix_sums(tiles_before, blocks, [&](int i) {
+        const int seq = find_last(blocks_before, a.seqs, i);
+        return a.kv_heads * block_of(a, seq, i - blocks_before[seq]).tiles;
+    });
+    const int total = tiles_before[blocks], run = max((total + (int)gridDim.x - 1) / (int)gridDim.x, least_run);
+    const int u_lo = min(total, (int)blockIdx.x * run), u_hi = min(total, u_lo + run);
+
+    auto fail = [&](int code) {
+        *failed = 1;
+        if (a.error) atomicExch(a.error, code);
+    };
+    // counts of what has gone through each ring and hand-over, the same in every role: fills of K and of V, scores and
+    // weights of each tile of rows, segments
+    int fills = 0, scores[2] = {0, 0}, segments = 0, ends[2] = {0, 0};
+    bool any_mma = false;
+
+    for (int u = u_lo; u < u_hi;) {
+        // ---- one part of one pair -------------------------------------------------------------------------------------
+        const int block_number = find_last(tiles_before, blocks, u), seq = find_last(blocks_before, a.seqs, block_number);
+        const Block b = block_of(a, seq, block_number - blocks_before[seq]);
+        const int kvh = (u - tiles_before[block_number]) / b.tiles, pair_at = tiles_before[block_number] + kvh * b.tiles;
+        const int part_end = min(u_hi, pair_at + b.tiles), n_kt = part_end - u, kt0 = b.first_tile + (u - pair_at);
+        const int first_token = a.cu[seq] + b.token0;
+        const int both = b.tokens > a.tile_tokens ? 2 : 1;          // tiles of rows that hold any
+
+        if (warp == kLoadWarp) {
+            if ((threadIdx.x & 31) == 0) {
+                bool ok = true;
+                mbar_expect_tx(q_full, (uint32_t)(both * DB * tile_rows * 128));
+                for (int x = 0; x < both; ++x)
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+                        tma_load_3d(q_s + x * kTileBytes + d * kBlockBytes, &map_q, d * 64, kvh * group, first_token + x * a.tile_tokens, q_full);
+                const int last_page = (b.start + a.cu[seq + 1] - a.cu[seq] - 1) / kPageSize;
+                auto load = [&](uint8_t* dst, const CUtensorMap* map, int t, uint64_t* bar) {
+                    mbar_expect_tx(bar, (uint32_t)kTileBytes);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        // (a page the sequence does not hold is replaced by its last one: its rows are masked, but must be numbers)
+                        const int row = ((seq * a.pages + min(2 * (kt0 + t) + half, last_page)) * a.kv_heads + kvh) * kPageSize;
+#pragma unroll
+                        for (int d = 0; d < DB; ++d) tma_load_2d(dst + d * kBlockBytes + half * (kBlockBytes / 2), map, d * 64, row, bar);
+                    }
+                };
+                int t = 0;
+                for (; t < n_kt && ok; ++t) {
+                    const int f = fills + t, s = f % NS;
+                    if (f >= NS && !(ok = mbar_wait(&k_empty[s], (uint32_t)(f / NS - 1) & 1u))) { fail(41); break; }
+                    load(k_s + s * kTileBytes, &map_k, t, &k_full[s]);
+                    if (f >= NS && !(ok = mbar_wait(&v_empty[s], (uint32_t)(f / NS - 1) & 1u))) {
+                        fail(42);
+                        mbar_wait(&k_full[s], (uint32_t)(f / NS) & 1u);      // (the copy just asked for lands)
+                        break;
+                    }
+                    load(v_s + s * kTileBytes, &map_v, t, &v_full[s]);
+                }
+                if (!ok || *failed) {
+                    // the way out: what was asked for lands before the CTA gives up its shared memory
+                    mbar_wait(q_full, (uint32_t)segments & 1u);
+                    OutstandingFill left[8];
+                    const int n = outstanding_fills(fills + t, max(0, fills + t - NS), NS, left);
+                    for (int i = 0; i < n; ++i) { mbar_wait(&k_full[left[i].stage], left[i].parity); mbar_wait(&v_full[left[i].stage], left[i].parity); }
+                }
+            }
+        } else if (warp == kMmaWarp) {
+            if ((threadIdx.x & 31) == 0) {
+                const uint32_t idesc_s = instr_desc(kRows, kKeys), idesc_pv = instr_desc(kRows, HD) | (1u << 16);     // V is MN-major
+                const uint64_t desc_q = smem_desc(smem_u32(q_s)), desc_k = smem_desc(smem_u32(k_s)), desc_v = smem_desc_rows(smem_u32(v_s));
+                auto issue_s = [&](int x, int s) {
+#pragma unroll
+                    for (int ks = 0; ks < HD / 16; ++ks) {
+                        const uint64_t off = (uint64_t)(((uint32_t)(ks / 4) * kBlockBytes + (uint32_t)(ks % 4) * 32) >> 4);
+                        umma_bf16(tmem + (uint32_t)x * 128, desc_q + (uint64_t)(((uint32_t)x * kTileBytes) >> 4) + off,
+                                  desc_k + (uint64_t)(((uint32_t)s * kTileBytes) >> 4) + off, idesc_s, ks > 0 ? 1u : 0u);
+                    }
+                    umma_commit(&s_full[x]);
+                };
+                auto issue_pv = [&](int x, int s, bool first) {
+#pragma unroll
+                    for (int ks = 0; ks < kKeys / 16; ++ks)
+                        umma_bf16_ts(tmem + kTmemO + (uint32_t)x * 128, tmem + (uint32_t)x * 128 + (uint32_t)ks * 8,
+                                     desc_v + (uint64_t)(((uint32_t)s * kTileBytes + (uint32_t)ks * 16 * 128) >> 4), idesc_pv, first && ks == 0 ? 0u : 1u);
+                };
+                bool ok = mbar_wait(q_full, (uint32_t)segments & 1u) && mbar_wait(&k_full[fills % NS], (uint32_t)(fills / NS) & 1u);
+                if (ok) {
+                    any_mma = true;
+                    tc_fence_after();
+                    for (int x = 0; x < both; ++x) issue_s(x, fills % NS);
+                    umma_commit(&k_empty[fills % NS]);
+                } else {
+                    fail(43);
+                }
+                for (int t = 0; t < n_kt && ok; ++t) {
+                    const int f = fills + t, s = f % NS, next = (f + 1) % NS;
+                    for (int x = 0; x < both && ok; ++x) {
+                        if (x == 0 && !(ok = mbar_wait(&v_full[s], (uint32_t)(f / NS) & 1u))) { fail(44); break; }
+                        if (x == 0 && t + 1 < n_kt && !(ok = mbar_wait(&k_full[next], (uint32_t)((f + 1) / NS) & 1u))) { fail(45); break; }
+                        if (!(ok = mbar_wait(&p_full[x], (uint32_t)(scores[x] + t) & 1u))) { fail(46); break; }
+                        tc_fence_after();
+                        issue_pv(x, s, t == 0);
+                        if (t + 1 < n_kt) issue_s(x, next);
+                        else umma_commit(&o_full[x]);
+                    }
+                    if (ok) {
+                        umma_commit(&v_empty[s]);
+                        if (t + 1 < n_kt) umma_commit(&k_empty[next]);
+                    }
+                }
+                if ((!ok || *failed) && any_mma) {
+                    umma_commit(drain_bar);
+                    mbar_wait(drain_bar, 0);
+                }
+            }
+        } else {
+            // ---- a thread per row ----------------------------------------------------------------------------------
+            const int x = warp >> 2, row = (warp & 3) * 32 + (threadIdx.x & 31);
+            if (x < both) {
+                const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+                const uint32_t tmem_s = tmem + (uint32_t)x * 128 + lane_base, tmem_o = tmem + kTmemO + (uint32_t)x * 128 + lane_base;
+                constexpr float kLazy = 8.0f;
+                const int x_tokens = min(a.tile_tokens, b.tokens - x * a.tile_tokens);           // tokens of this tile of rows
+                const int first_pos = b.start + b.token0 + x * a.tile_tokens, last_pos = first_pos + x_tokens - 1;
+                const int token = row / group, pos = first_pos + min(token, x_tokens - 1);
+                const bool live = token < x_tokens;
+                float m = -CUDART_INF_F, l = 0.f;
+                bool ok = true;
+                for (int t = 0; t < n_kt && ok; ++t) {
+                    const int key0 = (kt0 + t) * kKeys;
+                    if (!mbar_wait(&s_full[x], (uint32_t)(scores[x] + t) & 1u)) { fail(47); ok = false; break; }
+                    tc_fence_after();
+                    float sv[128];
+                    tmem_ld128(tmem_s, sv);
+                    // every row sees every key of the tile, or a mask is needed
+                    if (key0 + kKeys - 1 > first_pos || (a.window > 0 && key0 <= last_pos - a.window)) {
+                        const int hi = pos - key0, lo = a.window > 0 ? hi - a.window + 1 : 0;
+#pragma unroll
+                        for (int j = 0; j < 128; ++j)
+                            if (j > hi || j < lo) sv[j] = -CUDART_INF_F;
+                    }
+                    // maximum of the raw scores (the scale is positive)
+                    float top8[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top8[e] = sv[e];
+#pragma unroll
+                    for (int j = 8; j + 8 < 128; j += 16)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) top8[e] = fmax3(top8[e], sv[j + e], sv[j + 8 + e]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top8[e] = fmaxf(top8[e], sv[120 + e]);
+                    const float top = fmaxf(fmax3(top8[0], top8[1], top8[2]), fmax3(fmax3(top8[3], top8[4], top8[5]), top8[6], top8[7])) * a.scale_log2;
+                    if (__any_sync(0xffffffffu, top > m + kLazy)) {
+                        const float mx = fmaxf(m, top), corr = mx == -CUDART_INF_F ? 1.0f : ex2_approx(m - mx);
+                        if (t > 0) {         // (PV of the tile before is done: the scores came after it)
+#pragma unroll
+                            for (int c = 0; c < HD / 32; ++c) {
+                                float acc[32];
+                                tmem_ld32(tmem_o + (uint32_t)(c * 32), acc);
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) acc[j] *= corr;
+                                tmem_st32(tmem_o + (uint32_t)(c * 32), acc);
+                            }
+                        }
+                        l *= corr;
+                        m = mx;
+                    }
+                    const float ref = m == -CUDART_INF_F ? 0.f : m;
+                    const uint64_t scale2 = pack_f32x2(a.scale_log2, a.scale_log2), ref2 = pack_f32x2(-ref, -ref);
+                    uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};      // (the bits of two float zeros)
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int j = 0; j < 64; j += 2) {
+                            float x0, x1;
+                            unpack_f32x2(fma_f32x2(pack_f32x2(sv[part * 64 + j], sv[part * 64 + j + 1]), scale2, ref2), x0, x1);
+                            const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                            sum2[(j / 2) & 3] = add_f32x2(sum2[(j / 2) & 3], pack_f32x2(p0, p1));
+                            pk[j / 2] = pack_bf16(p0, p1);
+                        }
+                        tmem_st32_raw(tmem_s + (uint32_t)(part * 32), pk);
+                    }
+                    float lo, hi;
+                    unpack_f32x2(add_f32x2(add_f32x2(sum2[0], sum2[1]), add_f32x2(sum2[2], sum2[3])), lo, hi);
+                    l += lo + hi;
+                    tmem_st_wait();
+                    tc_fence_before();
+                    mbar_arrive(&p_full[x]);
+                }
+                if (ok && !mbar_wait(&o_full[x], (uint32_t)ends[x] & 1u)) { fail(48); ok = false; }
+                tc_fence_after();
+                const bool whole = u == pair_at && part_end == pair_at + b.tiles;
+                if (__all_sync(0xffffffffu, ok && !*failed)) {
+                    if (whole) {
+                        const float inv = 1.0f / l;
+                        __nv_bfloat16* dst = a.out + ((size_t)(first_token + x * a.tile_tokens + token) * a.heads + (size_t)kvh * group + (row - token * group)) * HD;
+#pragma unroll
+                        for (int c = 0; c < HD / 32; ++c) {
+                            float o[32];
+                            tmem_ld32(tmem_o + (uint32_t)(c * 32), o);
+                            if (live) {
+#pragma unroll
+                                for (int i = 0; i < 32; i += 8)
+                                    *reinterpret_cast<uint4*>(dst + c * 32 + i) =
+                                        make_uint4(pack_bf16(o[i] * inv, o[i + 1] * inv), pack_bf16(o[i + 2] * inv, o[i + 3] * inv),
+                                                   pack_bf16(o[i + 4] * inv, o[i + 5] * inv), pack_bf16(o[i + 6] * inv, o[i + 7] * inv));
+                            }
+                        }
+                    } else {
+                        float* part = a.parts + (((size_t)blockIdx.x * 2 + (pair_at < u_lo ? 0 : 1)) * 2 + x) * (HD + 2) * kRows + row;
+#pragma unroll
+                        for (int c = 0; c < HD / 32; ++c) {
+                            float o[32];
+                            tmem_ld32(tmem_o + (uint32_t)(c * 32), o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) part[(size_t)(c * 32 + i) * kRows] = o[i];
+                        }
+                        part[(size_t)HD * kRows] = m;
+                        part[(size_t)(HD + 1) * kRows] = l;
+                    }
+                }
+                tc_fence_before();      // (this segment's reads of tensor memory come before the next one's writes)
+            }
+        }
+        __syncwarp();
+        __syncthreads();
+        tc_fence_after();
+        if (*failed) break;
+        if (threadIdx.x == 0 && pair_at >= u_lo) {
+            const bool whole = part_end == pair_at + b.tiles;
+            a.cuts[block_number * a.kv_heads + kvh] =
+                ChunkCut{first_token, kvh, whole ? 0 : b.tokens, (int)blockIdx.x, (pair_at + b.tiles - 1) / run, {0, 0, 0}};
+        }
+        fills += n_kt;
+        ++segments;
+        for (int x = 0; x < both; ++x) { scores[x] += n_kt; ++ends[x]; }
+        u = part_end;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+// Puts the parts of a cut pair together, in the order of the line: blockIdx.x the pair, blockIdx.y 32 of its dimensions, a
+// thread a row.
+template <int HD>
+__global__ void __launch_bounds__(2 * kRows) attention_chunk_join_kernel(ChunkArgs a) {
+    pdl_wait();              // (every CTA waits: this kernel must not end before the one it follows)
+    pdl_launch_dependents();
+    const ChunkCut cut = a.cuts[blockIdx.x];
+    const int group = a.heads / a.kv_heads, x = threadIdx.x / kRows, row = threadIdx.x - x * kRows, token = row / group;
+    if (token >= min(a.tile_tokens, cut.tokens - x * a.tile_tokens)) return;
+    const float* first = a.parts + (size_t)x * (HD + 2) * kRows + row;
+    const size_t stride = (size_t)2 * (HD + 2) * kRows;                 // of a part of both tiles; two a CTA
+    float m = -CUDART_INF_F;
+    for (int c = cut.first; c <= cut.last; ++c) m = fmaxf(m, first[((size_t)c * 2 + (c == cut.first ? 1 : 0)) * stride + (size_t)HD * kRows]);
+    float l = 0.f, o[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) o[i] = 0.f;
+    for (int c = cut.first; c <= cut.last; ++c) {
+        const float* part = first + ((size_t)c * 2 + (c == cut.first ? 1 : 0)) * stride;
+        const float pm = part[(size_t)HD * kRows], pl = part[(size_t)(HD + 1) * kRows];
+        // (no key seen: 0; no maximum, because every score is NaN: 1, and the sum is NaN)
+        const float f = pm == -CUDART_INF_F ? (pl == 0.f ? 0.f : 1.f) : ex2_approx(pm - m);
+        if (f == 0.f) continue;
+        l += pl * f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = fmaf(part[(size_t)(blockIdx.y * 32 + i) * kRows], f, o[i]);
+    }
+    const float inv = 1.0f / l;
+    __nv_bfloat16* dst = a.out + ((size_t)(cut.first_token + x * a.tile_tokens + token) * a.heads + (size_t)cut.kv_head * group + (row - token * group)) * HD + blockIdx.y * 32;
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        *reinterpret_cast<uint4*>(dst + i) = make_uint4(pack_bf16(o[i] * inv, o[i + 1] * inv), pack_bf16(o[i + 2] * inv, o[i + 3] * inv),
+                                                        pack_bf16(o[i + 4] * inv, o[i + 5] * inv), pack_bf16(o[i + 6] * inv, o[i + 7] * inv));
+}
+
+constexpr int kDevices = 64;
+int this_device() {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= kDevices) throw std::runtime_error("attention_chunk: more devices than it knows");
+    return dev;
+}
+int sm_count() {
+    static int known[kDevices] = {};
+    const int dev = this_device();
+    if (!known[dev]) cudaDeviceGetAttribute(&known[dev], cudaDevAttrMultiProcessorCount, dev);
+    return known[dev];
+}
+
+template <int HD>
+void launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkArgs& a, int blocks, int least_run, cudaStream_t stream) {
+    constexpr int NS = stages_of(HD);
+    const size_t smem = 1024 + (size_t)(2 + 2 * NS) * (HD / 64) * kBlockBytes + (8 + 4 * NS) * sizeof(uint64_t) + 8 + (size_t)(a.seqs + blocks + 2) * sizeof(int);
+    auto kernel = attention_chunk_kernel<HD>;
+    static bool prepared[kDevices] = {};
+    const int dev = this_device();
+    if (!prepared[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+        if (e != cudaSuccess) throw std::runtime_error(std::string("attention_chunk: ") + cudaGetErrorString(e));
+        prepared[dev] = true;
+    }
+    note_launch(2);
+    launch_kernel("attention_chunk", kernel, dim3((unsigned)sm_count()), dim3(kThreads), smem, stream, 1, dependent_launch_enabled(), mq, mk, mv, a, least_run);
+    launch_kernel("attention_chunk", attention_chunk_join_kernel<HD>, dim3((unsigned)(blocks * a.kv_heads), HD / 32), dim3(2 * kRows), 0, stream, 1,
+                  dependent_launch_enabled(), a);
+}
+
+}  // namespace
+
+bool attention_chunk_supports(int heads, int kv_heads, int head_dim, long long pool_pages, int n_seqs, int blocks) {
+    return (head_dim == 64 || head_dim == 128) && kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= 64 && pool_pages > 0 &&
+           pool_pages * kv_heads * kPageSize < (1ll << 31) && n_seqs <= kMaxSeqs && blocks <= kMaxBlocks;
+}
+
+long long attention_chunk_workspace(int head_dim, int kv_heads, int blocks) {
+    return (long long)blocks * kv_heads * (long long)(sizeof(ChunkCut) / sizeof(float)) + (long long)sm_count() * 2 * 2 * (head_dim + 2) * kRows;
+}
+
+void attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window, const void* k_pages,
+                     const void* v_pages, int pages, const int32_t* seq_ends, const int32_t* cu_seqlens, int skip_new, int blocks, float* workspace,
+                     long long workspace_floats, cudaStream_t stream) {
+    if (n_seqs <= 0 || blocks <= 0 || T <= 0) return;
+    if (!attention_chunk_supports(heads, kv_heads, head_dim, (long long)n_seqs * pages, n_seqs, blocks))
+        throw std::invalid_argument("attention_chunk: " + std::to_string(heads) + " heads on " + std::to_string(kv_heads) + " of size " +
+                                    std::to_string(head_dim) + " (64 or 128, at most 64 heads a kv head), " + std::to_string(n_seqs) + " sequences, " +
+                                    std::to_string(blocks) + " blocks of queries");
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15)
+        throw std::invalid_argument("attention_chunk: operands must be 16-byte aligned");
+    if (workspace_floats < attention_chunk_workspace(head_dim, kv_heads, blocks)) throw std::invalid_argument("attention_chunk: the workspace is too small");
+    const int group = heads / kv_heads, tile_tokens = kRows / group;
+    // queries as [T][heads][head_dim]: a box is 64 columns of a group's heads of a tile's tokens
+    CUtensorMap mq;
+    cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)T};
+    cuuint64_t strides[2] = {(cuuint64_t)head_dim * 2, (cuuint64_t)heads * head_dim * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)tile_tokens}, step[3] = {1, 1, 1};
+    const CUresult r = tensor_map_encoder()(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw std::runtime_error("attention_chunk: cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+    // pages [n_seqs * pages, kv heads, 64 positions, head_dim] as rows of head_dim: a box is 64 columns of a page of one kv head
+    const uint64_t rows = (uint64_t)n_seqs * pages * kv_heads * kPageSize;
+    const CUtensorMap mk = tiled_map_2d("attention_chunk", CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, k_pages, (uint64_t)head_dim, rows, (uint64_t)head_dim * 2, 64,
+                                        kPageSize, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    const CUtensorMap mv = tiled_map_2d("attention_chunk", CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, v_pages, (uint64_t)head_dim, rows, (uint64_t)head_dim * 2, 64,
+                                        kPageSize, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    ChunkCut* cuts = (ChunkCut*)workspace;
+    ChunkArgs a{(__nv_bfloat16*)out, seq_ends, cu_seqlens, n_seqs, heads, kv_heads, window, skip_new, pages, tile_tokens, blocks, scale * 1.4426950408889634f, cuts,
+                workspace + (long long)blocks * kv_heads * (long long)(sizeof(ChunkCut) / sizeof(float)), error_word()};
+    // a run is at least this many tiles: a part costs about as much as two to leave and join
+    const int least_run = 4;
+    if (head_dim == 64) launch<64>(mq, mk, mv, a, blocks, least_run, stream);
+    else launch<128>(mq, mk, mv, a, blocks, least_run, stream);
+}
+
+}  // namespace sm

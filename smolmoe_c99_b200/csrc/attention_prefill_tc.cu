@@ -63,7 +63,6 @@ struct PrefillTcArgs {
     int* error;
     const int32_t* page_table;    // over the cache: [slots][table_stride]
     int table_stride;
-    int skip_new;             // over the cache: sequences that bring at most this many tokens are another kernel's
 };
 
 // Descriptor of an "MN-major" operand tile with 128-byte swizzle: rows of the reduction dimension are 128
@@ -110,7 +109,6 @@ __global__ void __launch_bounds__(kThreads, TWO ? 2 : 1) prefill_attention_tc_ke
     const int seq_start = a.tiles[TW * tile], seq_len = a.tiles[TW * tile + 1], q0 = a.tiles[TW * tile + 2];
     const int pos0 = CACHED ? a.tiles[TW * tile + 3] : 0, slot = CACHED ? a.tiles[TW * tile + 4] : 0;
     if (q0 % kBM) return;                             // the second half of a tile of 128 queries
-    if (CACHED && seq_len <= a.skip_new) { pdl_wait(); return; }
     const int kvh = h / (a.heads / a.kv_heads);
 
     extern __shared__ uint8_t smem_raw[];
@@ -548,7 +546,7 @@ void attention_prefill_tc(const void* q, const void* k, const void* v, void* out
     const CUtensorMap mq = make_map(q, T, heads * head_dim);
     const CUtensorMap mk = make_map(k, T, kv_heads * head_dim);
     const CUtensorMap mv = make_map(v, T, kv_heads * head_dim);
-    PrefillTcArgs a{(__nv_bfloat16*)out, tiles, heads, kv_heads, window, scale * 1.4426950408889634f, error, nullptr, 0, 0};
+    PrefillTcArgs a{(__nv_bfloat16*)out, tiles, heads, kv_heads, window, scale * 1.4426950408889634f, error, nullptr, 0};
     note_launch();
     if (head_dim == 128) {
         launch<128, false>(mq, mk, mv, a, n_tiles, stream);
@@ -576,8 +574,7 @@ bool attention_extend_tc_supports(int heads, int kv_heads, int head_dim, long lo
 
 void attention_extend_tc(const void* q, void* out, const int32_t* tiles, int n_tiles, int T, int heads, int kv_heads, int head_dim,
                          float scale, int window, const void* k_pool, const void* v_pool, const int32_t* page_table,
-                         int table_stride, long long pool_pages, int longest, int variant, int skip_new, int* error,
-                         cudaStream_t stream) {
+                         int table_stride, long long pool_pages, int longest, int variant, int* error, cudaStream_t stream) {
     if (n_tiles <= 0) return;
     if (!attention_extend_tc_supports(heads, kv_heads, head_dim, pool_pages))
         throw std::invalid_argument("attention_extend_tc: head_dim " + std::to_string(head_dim) + " is not 64 or 128, or the pool has too many rows for a tensor map");
@@ -591,7 +588,7 @@ void attention_extend_tc(const void* q, void* out, const int32_t* tiles, int n_t
                                         (uint64_t)head_dim * 2, 64, kPageSize, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
     const CUtensorMap mv = tiled_map_2d("attention_extend_tc", CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, v_pool, (uint64_t)head_dim, rows,
                                         (uint64_t)head_dim * 2, 64, kPageSize, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
-    PrefillTcArgs a{(__nv_bfloat16*)out, tiles, heads, kv_heads, window, scale * 1.4426950408889634f, error, page_table, table_stride, skip_new};
+    PrefillTcArgs a{(__nv_bfloat16*)out, tiles, heads, kv_heads, window, scale * 1.4426950408889634f, error, page_table, table_stride};
     note_launch();
     if (head_dim == 128) {
         launch<128, false, true>(mq, mk, mv, a, n_tiles, stream);

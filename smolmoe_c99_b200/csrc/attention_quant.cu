@@ -75,6 +75,7 @@ struct AttnArgs {
     int seqs, heads, kv_heads, head_dim, window;
     int most_new;                        // sequences with more new tokens are not this kernel's
     int block_tokens;                    // tokens of a block of rows
+    int pairs;                           // what the host says there are
     int cluster, stages, tile;           // CTAs of a cluster (0: the line); tiles a warp keeps in flight; positions of a tile
     float scale_log2;
     Cut* cuts;                           // the line: [pairs]
@@ -558,7 +559,10 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_cluster_kernel(co
     pdl_launch_dependents();
     scan_sequences(a, table);
     const int pair_number = blockIdx.x / C, rank = blockIdx.x - pair_number * C;
-    if (pair_number >= table.pairs_before[a.seqs]) return;          // (the whole cluster)
+    if (table.pairs_before[a.seqs] != a.pairs) {     // lengths on the device that are not those on the host: nothing is done
+        if (threadIdx.x == 0 && a.error) atomicExch(a.error, kBadPlaceInAttention);
+        return;                                      // (every CTA)
+    }
     // (a CTA may write into the leader's memory only once the leader runs: arrived here, waited for below)
     if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const int i = find_seq(table.pairs_before, a.seqs, pair_number);
@@ -684,6 +688,13 @@ __global__ void __launch_bounds__(line_warps(NHT) * 32, 1) attention_quant_line_
     pdl_launch_dependents();
     scan_sequences(a, table);
 
+    if (table.pairs_before[a.seqs] != a.pairs) {     // lengths on the device that are not those on the host: nothing is done
+        if (blockIdx.x == 0) {
+            if (threadIdx.x == 0 && a.error) atomicExch(a.error, kBadPlaceInAttention);
+            for (int i = threadIdx.x; i < a.pairs; i += W * 32) a.cuts[i].rows = 0;
+        }
+        return;                                      // (every CTA)
+    }
     // this warp's run of the line (neighbouring runs on different SMs: the last ones may be empty)
     const int total = table.tiles_before[a.seqs], number = warp * gridDim.x + blockIdx.x, warps = W * gridDim.x;
     const int run = (total + warps - 1) / warps;
@@ -911,7 +922,7 @@ void attention_quant(const void* q, void* out, int n_seqs, int heads, int kv_hea
     if (workspace_floats < attention_quant_workspace(head_dim, row_tiles, pairs, cluster)) throw std::invalid_argument("attention_quant: the workspace is too small");
     AttnArgs a{(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)k_pool, (const uint8_t*)v_pool, (const uint8_t*)k_scale,
                (const uint8_t*)v_scale, {page_table, slots, table_stride, pool_pages}, slot_ids, seq_ends, cu_seqlens, n_seqs, heads,
-               kv_heads, head_dim, window, most_new, 8 * row_tiles / group, cluster, 0,
+               kv_heads, head_dim, window, most_new, 8 * row_tiles / group, pairs, cluster, 0,
                cluster ? kClusterTile : line_tile(row_tiles), scale * 1.4426950408889634f, (Cut*)workspace,
                workspace + (cluster ? 0 : (long long)pairs * (long long)(sizeof(Cut) / sizeof(float))), error_word()};
     CUtensorMap mk{}, mv{};

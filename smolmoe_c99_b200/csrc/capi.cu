@@ -248,10 +248,10 @@ SM_API int sm_attention_extend_tc_supports(int heads, int kv_heads, int head_dim
 SM_API int sm_attention_extend_tc(const void* q, void* out, const int32_t* tiles, int n_tiles, int T, int heads, int kv_heads,
                                   int head_dim, float scale, int window, const void* k_pool, const void* v_pool,
                                   const int32_t* page_table, int table_stride, long long pool_pages, int longest, int variant,
-                                  int skip_new, int* error, void* stream) {
+                                  int* error, void* stream) {
     return guarded([&] {
         sm::attention_extend_tc(q, out, tiles, n_tiles, T, heads, kv_heads, head_dim, scale, window, k_pool, v_pool, page_table,
-                                table_stride, pool_pages, longest, variant, skip_new, error, (cudaStream_t)stream);
+                                table_stride, pool_pages, longest, variant, error, (cudaStream_t)stream);
     });
 }
 
@@ -272,6 +272,23 @@ SM_API int sm_attention_quant(const void* q, void* out, int n_seqs, int heads, i
         sm::attention_quant(q, out, n_seqs, heads, kv_heads, head_dim, scale, window, fmt, k_pool, v_pool, k_scale, v_scale,
                             pool_pages, page_table, slots, table_stride, slot_ids, seq_ends, cu_seqlens, max_len, most_new,
                             row_tiles, pairs, cluster, workspace, workspace_floats, (cudaStream_t)stream);
+    });
+}
+
+SM_API int sm_attention_chunk_supports(int heads, int kv_heads, int head_dim, long long pool_pages, int n_seqs, int blocks) {
+    return sm::attention_chunk_supports(heads, kv_heads, head_dim, pool_pages, n_seqs, blocks) ? 1 : 0;
+}
+
+SM_API long long sm_attention_chunk_workspace(int head_dim, int kv_heads, int blocks) {
+    return sm::attention_chunk_workspace(head_dim, kv_heads, blocks);
+}
+
+SM_API int sm_attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window,
+                              const void* k_pages, const void* v_pages, int pages, const int32_t* seq_ends, const int32_t* cu_seqlens,
+                              int skip_new, int blocks, float* workspace, long long workspace_floats, void* stream) {
+    return guarded([&] {
+        sm::attention_chunk(q, out, T, n_seqs, heads, kv_heads, head_dim, scale, window, k_pages, v_pages, pages, seq_ends, cu_seqlens,
+                            skip_new, blocks, workspace, workspace_floats, (cudaStream_t)stream);
     });
 }
 

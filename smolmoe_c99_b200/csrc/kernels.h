@@ -238,11 +238,11 @@ void attention_prefill_tc(const void* q, const void* k, const void* v, void* out
 
 // The same kernel for sequences that go on from the cache by many tokens (prompt portions): keys and values come from
 // the paged pools, which must hold the step's own tokens already; `tiles` [n_tiles, 5] as attention_extend takes them,
-// `longest` the longest sequence after the step. Sequences that bring at most `skip_new` tokens are left out. No windowed group (its ring is written after the attention).
+// `longest` the longest sequence after the step. No windowed group (its ring is written after the attention).
 bool attention_extend_tc_supports(int heads, int kv_heads, int head_dim, long long pool_pages);
 void attention_extend_tc(const void* q, void* out, const int32_t* tiles, int n_tiles, int T, int heads, int kv_heads, int head_dim,
                          float scale, int window, const void* k_pool, const void* v_pool, const int32_t* page_table,
-                         int table_stride, long long pool_pages, int longest, int variant, int skip_new, int* error, cudaStream_t stream);
+                         int table_stride, long long pool_pages, int longest, int variant, int* error, cudaStream_t stream);
 
 // ---- attention_decode.cu --------------------------------------------------------------
 // One new token per sequence over the paged cache for bfloat16: a cluster of CTAs per
@@ -276,6 +276,16 @@ void attention_quant(const void* q, void* out, int n_seqs, int heads, int kv_hea
                      const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale, long long pool_pages,
                      const int32_t* page_table, int slots, int table_stride, const int32_t* slot_ids, const int32_t* seq_ends,
                      const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles, int pairs, int cluster, float* workspace,
+                     long long workspace_floats, cudaStream_t stream);
+
+// ---- attention_chunk_tc.cu ------------------------------------------------------------
+// The same attention for sequences that bring more than `skip_new` tokens, over their pages as bfloat16 values as
+// kv_quant_load (attend) leaves them: [n_seqs, pages, kv_heads, 64, head_dim], sequence by sequence. Head sizes 64 and 128.
+// `blocks`: blocks of 2 * (128 / group) new tokens over those sequences (group: heads a kv head).
+bool attention_chunk_supports(int heads, int kv_heads, int head_dim, long long pool_pages, int n_seqs, int blocks);
+long long attention_chunk_workspace(int head_dim, int kv_heads, int blocks);   // floats
+void attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window, const void* k_pages,
+                     const void* v_pages, int pages, const int32_t* seq_ends, const int32_t* cu_seqlens, int skip_new, int blocks, float* workspace,
                      long long workspace_floats, cudaStream_t stream);
 
 // ---- decode_fused.cu ------------------------------------------------------------------

@@ -141,6 +141,9 @@ class Ops:
             [addr] * 3 + [num] * 5 + [addr, big, addr]
         self.lib.sm_attention_quant_supports.argtypes = [num, num, num, big]
         self.lib.sm_attention_quant_workspace.argtypes, self.lib.sm_attention_quant_workspace.restype = [num, num, num, num], big
+        self.lib.sm_attention_chunk_supports.argtypes = [num, num, num, big, num, num]
+        self.lib.sm_attention_chunk_workspace.argtypes, self.lib.sm_attention_chunk_workspace.restype = [num, num, num], big
+        self.lib.sm_attention_chunk.argtypes = [addr, addr] + [num] * 5 + [ctypes.c_float, num, addr, addr, num, addr, addr, num, num, addr, big, addr]
         self._quant_workspaces: dict = {}
         fast = kernels == "fast"
         self.kernels = kernels
@@ -698,16 +701,20 @@ class Ops:
                                         page_table=pages.page_table, token_slot=step.token_slot, kv_heads=kv_heads)
         out = torch.empty_like(q)
         lens = step.seq_lens
-        most = max(lens)
-        limit = most
-        if (most > self.quant_rows_tokens and step.extend_tiles is not None and self.use_tcgen05_attention
-                and self.lib.sm_attention_extend_tc_supports(heads, kv_heads, head_dim, ctypes.c_longlong(step.n_seqs * cache.page_table.shape[1]))):
-            limit = self.quant_rows_tokens
-            few = [n for n in lens if n <= limit]
-            most = max(few) if few else 0
+        most = limit = max(lens)
+        group = heads // kv_heads
+        blocks = 0
+        if most > self.quant_rows_tokens and self.use_tcgen05_attention:
+            many = 2 * (128 // group)     # tokens of a block of the tcgen05 kernel
+            blocks = sum(-(-n // many) for n in lens if n > self.quant_rows_tokens)
+            if self.lib.sm_attention_chunk_supports(heads, kv_heads, head_dim, step.n_seqs * cache.page_table.shape[1], step.n_seqs, blocks):
+                limit = self.quant_rows_tokens
+                few = [n for n in lens if n <= limit]
+                most = max(few) if few else 0
+            else:
+                blocks = 0
         if most:
             # single tokens, and sequences that bring a few: straight from the codes
-            group = heads // kv_heads
             row_tiles = 1
             while 8 * row_tiles < min(most * group, 32 if head_dim <= 64 else 16) or 8 * row_tiles < group:
                 row_tiles *= 2
@@ -727,14 +734,15 @@ class Ops:
                 cache.page_table.shape[0], cache.page_table.shape[1], step.slot_ids.data_ptr(), step.seq_ends.data_ptr(),
                 step.cu_seqlens.data_ptr(), longest, limit, row_tiles, pairs, cluster, workspace.data_ptr() if floats else None, floats,
                 _stream()))
-        if limit < max(lens):
+        if blocks:
             # many tokens: the pages are read back as bfloat16 once (exactly), and the tcgen05 kernel reads those
             pages = self._quant_load(step, cache, q.dtype, False, limit, True, int(window or 0))
-            self._check(self.lib.sm_attention_extend_tc(
-                _ptr(q), _ptr(out), _ptr(step.extend_tiles), step.extend_tiles.shape[0], q.shape[0], heads, kv_heads, head_dim,
-                ctypes.c_float(scale), int(window or 0), _ptr(pages.k_pool), _ptr(pages.v_pool), _ptr(pages.page_table),
-                pages.page_table.shape[1], ctypes.c_longlong(pages.k_pool.shape[0]), int(step.max_seq_len),
-                int(self.extend_tc_variant), limit, _ptr(self.error_flag), _stream()))
+            floats = int(self.lib.sm_attention_chunk_workspace(head_dim, kv_heads, blocks))
+            workspace = torch.empty((floats,), dtype=torch.float32, device=q.device)
+            self._check(self.lib.sm_attention_chunk(
+                q.data_ptr(), out.data_ptr(), step.n_tokens, step.n_seqs, heads, kv_heads, head_dim, scale, int(window or 0),
+                pages.k_pool.data_ptr(), pages.v_pool.data_ptr(), pages.page_table.shape[1], step.seq_ends.data_ptr(), step.cu_seqlens.data_ptr(),
+                limit, blocks, workspace.data_ptr(), floats, _stream()))
         return out
 
     def _quant_cluster(self, pairs: int, longest: int, head_dim: int) -> int:
@@ -775,7 +783,7 @@ class Ops:
                 _ptr(q), _ptr(out), _ptr(step.extend_tiles), step.extend_tiles.shape[0], q.shape[0], q.shape[1],
                 k_packed.shape[1], q.shape[2], ctypes.c_float(scale), int(window or 0), _ptr(cache.k_pool), _ptr(cache.v_pool),
                 _ptr(cache.page_table), cache.page_table.shape[1], ctypes.c_longlong(cache.k_pool.shape[0]),
-                int(step.max_seq_len), int(self.extend_tc_variant), 0, _ptr(self.error_flag), _stream()))
+                int(step.max_seq_len), int(self.extend_tc_variant), _ptr(self.error_flag), _stream()))
             return out
         if (self.use_fast_attention and q.dtype == torch.bfloat16 and step.extend_tiles is not None
                 and self.lib.sm_attention_prefill_supports(q.shape[2])):
