@@ -14,7 +14,9 @@
 // Work is shared out as a line: the tiles of 128 keys of all pairs (two query tiles of one kv head), one after the other; each
 // CTA of a grid of one an SM takes an equal run. What a run cuts is left as float accumulators, references and sums in a
 // workspace and joined by a second kernel in the order of the line. So 512 tokens of 14 heads onto 8,000, 30 pairs, fill
-// 148 SMs. Lengths are read on the device: a captured launch follows a growing sequence.
+// 148 SMs. Loads, products and row threads each go through the run at their own pace and meet at mbarriers only, so the next
+// pair's queries and first scores come while the last weights of this one are under way. Lengths are read on the device: a
+// captured launch follows a growing sequence.
 //
 // Every wait on an mbarrier is bounded; a wait that runs out records a code in *error and the CTA leaves without writing.
 #include <math_constants.h>
@@ -37,9 +39,9 @@ namespace {
 using namespace tc5;
 
 constexpr int kRows = 128, kKeys = 128;
-constexpr int kRowThreads = 256;            // one a row: warps 0-3 tile A, 4-7 tile B
+constexpr int kRowWarps = 8;                // a thread a row: warps 0-3 tile A, 4-7 tile B
 constexpr int kMmaWarp = 8, kLoadWarp = 9;
-constexpr int kThreads = 320;
+constexpr int kThreads = (kRowWarps + 2) * 32;
 constexpr int kBlockBytes = 128 * 128;      // 128 rows of 128 bytes: one swizzled block of 64 bfloat16 columns
 constexpr int kMaxSeqs = 1024, kMaxBlocks = 2048;
 
@@ -86,6 +88,14 @@ __device__ __forceinline__ void tmem_st32_raw(uint32_t taddr, const uint32_t (&r
            "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+// 16 float columns of this thread's lane back into tensor memory (complete after tmem_st_wait()).
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        :: "r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]),
+           "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -98,14 +108,12 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 
 // A block: two tiles of rows of one sequence, for every kv head a pair of the line. Tiles of keys it sees: first .. first + n - 1.
 struct Block {
-    int seq, token0, tokens, start;      // first token among the sequence's new ones, tokens (of both tiles), position of new token 0
+    int token0, tokens, start;           // first token among the sequence's new ones, tokens (of both tiles), position of new token 0
     int first_tile, tiles;
 };
-__device__ __forceinline__ Block block_of(const ChunkArgs& a, int seq, int index) {
+__device__ __forceinline__ Block block_of(const ChunkArgs& a, int start, int n, int index) {
     Block b;
-    const int n = a.cu[seq + 1] - a.cu[seq];
-    b.seq = seq;
-    b.start = a.seq_ends[seq] - n;
+    b.start = start;
     b.token0 = index * 2 * a.tile_tokens;
     b.tokens = min(2 * a.tile_tokens, n - b.token0);
     const int lowest = a.window > 0 ? max(0, b.start + b.token0 - a.window + 1) : 0;
@@ -150,6 +158,37 @@ __device__ void prefix_sums(int* before, int n, F value) {
     __syncthreads();
 }
 
+// The step's sequences and the line, in shared memory.
+struct Line {
+    int *blocks_before, *tiles_before;   // [seqs + 1] blocks before a sequence, [blocks + 1] tiles of the line before a block
+    int *first, *start, *n;              // [seqs] first new token among the step's, its position, new tokens
+};
+// One part of one pair: what a run holds of it.
+struct Part {
+    int seq, kvh, number, pair_at, tiles;      // the pair's number, its place on the line, its tiles of keys
+    int kt0, n_kt;                             // the part's tiles of keys
+    int first_token, tokens, first_pos, last_page;
+    int end;                                   // where the part ends on the line
+};
+__device__ __forceinline__ Part part_at(const ChunkArgs& a, const Line& line, int blocks, int u, int u_hi) {
+    const int block_number = find_last(line.tiles_before, blocks, u), seq = find_last(line.blocks_before, a.seqs, block_number);
+    const Block b = block_of(a, line.start[seq], line.n[seq], block_number - line.blocks_before[seq]);
+    Part p;
+    p.seq = seq;
+    p.kvh = (u - line.tiles_before[block_number]) / b.tiles;
+    p.number = block_number * a.kv_heads + p.kvh;
+    p.pair_at = line.tiles_before[block_number] + p.kvh * b.tiles;
+    p.tiles = b.tiles;
+    p.end = min(u_hi, p.pair_at + b.tiles);
+    p.n_kt = p.end - u;
+    p.kt0 = b.first_tile + (u - p.pair_at);
+    p.first_token = line.first[seq] + b.token0;
+    p.tokens = b.tokens;
+    p.first_pos = b.start + b.token0;
+    p.last_page = (b.start + line.n[seq] - 1) / kPageSize;
+    return p;
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                       const __grid_constant__ CUtensorMap map_v, ChunkArgs a, int least_run) {
@@ -161,21 +200,32 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
     uint8_t* k_s = q_s + 2 * kTileBytes;                 // [NS][DB][128 keys][128 B]
     uint8_t* v_s = k_s + NS * kTileBytes;                // [NS]
     uint64_t* bars = (uint64_t*)(v_s + NS * kTileBytes);
-    uint64_t* q_full = bars;                             // the segment's queries have landed
-    uint64_t* s_full = bars + 1;                         // [2] scores are in tensor memory (and PV of the tile before is done)
-    uint64_t* p_full = bars + 3;                         // [2] weights are in tensor memory
-    uint64_t* o_full = bars + 5;                         // [2] the segment's last PV is done
-    uint64_t* drain_bar = bars + 7;
-    uint64_t *k_full = bars + 8, *k_empty = k_full + NS, *v_full = k_empty + NS, *v_empty = v_full + NS;
-    uint32_t* tmem_slot = (uint32_t*)(bars + 8 + 4 * NS);
+    uint64_t *q_full = bars, *q_empty = bars + 1;        // a part's queries have landed; its last scores are done
+    uint64_t* s_full = bars + 2;                         // [2] scores are in tensor memory (and PV of the tile before is done)
+    uint64_t* p_full = bars + 4;                         // [2] weights are in tensor memory (and the accumulator is rescaled)
+    uint64_t* o_full = bars + 6;                         // [2] the part's last PV is done
+    uint64_t* o_empty = bars + 8;                        // [2] the part's accumulator has been read
+    uint64_t* drain_bar = bars + 10;
+    uint64_t *k_full = bars + 11, *k_empty = k_full + NS, *v_full = k_empty + NS, *v_empty = v_full + NS;
+    uint32_t* tmem_slot = (uint32_t*)(v_empty + NS);
     volatile int* failed = (volatile int*)(tmem_slot + 1);
-    int* blocks_before = (int*)(tmem_slot + 2);          // [seqs + 1] blocks before a sequence
-    int* tiles_before = blocks_before + a.seqs + 1;      // [blocks + 1] tiles of the line before a block
+    Line line;
+    line.blocks_before = (int*)(tmem_slot + 2);
+    line.first = line.blocks_before + a.seqs + 1;
+    line.start = line.first + a.seqs;
+    line.n = line.start + a.seqs;
+    line.tiles_before = line.n + a.seqs;
 
     const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads, tile_rows = a.tile_tokens * group;
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
-        for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 1); mbar_init(&p_full[x], kRows); mbar_init(&o_full[x], 1); }
+        mbar_init(q_empty, 1);
+        for (int x = 0; x < 2; ++x) {
+            mbar_init(&s_full[x], 1);
+            mbar_init(&p_full[x], kRows);
+            mbar_init(&o_full[x], 1);
+            mbar_init(&o_empty[x], kRows);
+        }
         mbar_init(drain_bar, 1);
         for (int i = 0; i < 4 * NS; ++i) mbar_init(&k_full[i], 1);
         *failed = 0;
@@ -195,261 +245,282 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
     pdl_wait();              // queries, pages and lengths come from the kernels before
     pdl_launch_dependents();
 
-    prefix_sums(blocks_before, a.seqs, [&](int i) {
-        const int n = a.cu[i + 1] - a.cu[i];
-        return n > a.skip_new && n <= a.seq_ends[i] ? (n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens) : 0;
+    prefix_sums(line.blocks_before, a.seqs, [&](int i) {
+        const int first = a.cu[i], n = a.cu[i + 1] - first, end = a.seq_ends[i];
+        line.first[i] = first;
+        line.start[i] = end - n;
+        line.n[i] = n;
+        return n > a.skip_new && n <= end ? (n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens) : 0;
     });
     // (lengths on the device that are not those on the host: nothing is done)
-    const int blocks = blocks_before[a.seqs] == a.blocks ? a.blocks : 0;
+    const int blocks = line.blocks_before[a.seqs] == a.blocks ? a.blocks : 0;
     if (blocks == 0 && blockIdx.x == 0) {
         if (threadIdx.x == 0 && a.error) atomicExch(a.error, kBadPlaceInAttention);
         for (int i = threadIdx.x; i < a.blocks * a.kv_heads; i += kThreads) a.cuts[i].tokens = 0;
     }
-    prefix_sums(tiles_before, blocks, [&](int i) {
-        const int seq = find_last(blocks_before, a.seqs, i);
-        return a.kv_heads * block_of(a, seq, i - blocks_before[seq]).tiles;
+    prefix_sums(line.tiles_before, blocks, [&](int i) {
+        const int seq = find_last(line.blocks_before, a.seqs, i);
+        return a.kv_heads * block_of(a, line.start[seq], line.n[seq], i - line.blocks_before[seq]).tiles;
     });
-    const int total = tiles_before[blocks], run = max((total + (int)gridDim.x - 1) / (int)gridDim.x, least_run);
+    const int total = line.tiles_before[blocks], run = max((total + (int)gridDim.x - 1) / (int)gridDim.x, least_run);
     const int u_lo = min(total, (int)blockIdx.x * run), u_hi = min(total, u_lo + run);
 
     auto fail = [&](int code) {
         *failed = 1;
         if (a.error) atomicExch(a.error, code);
     };
-    // counts of what has gone through each ring and hand-over, the same in every role: fills of K and of V, scores and
-    // weights of each tile of rows, segments
-    int fills = 0, scores[2] = {0, 0}, segments = 0, ends[2] = {0, 0};
-    bool any_mma = false;
 
-    for (int u = u_lo; u < u_hi;) {
-        // ---- one part of one pair -------------------------------------------------------------------------------------
-        const int block_number = find_last(tiles_before, blocks, u), seq = find_last(blocks_before, a.seqs, block_number);
-        const Block b = block_of(a, seq, block_number - blocks_before[seq]);
-        const int kvh = (u - tiles_before[block_number]) / b.tiles, pair_at = tiles_before[block_number] + kvh * b.tiles;
-        const int part_end = min(u_hi, pair_at + b.tiles), n_kt = part_end - u, kt0 = b.first_tile + (u - pair_at);
-        const int first_token = a.cu[seq] + b.token0;
-        const int both = b.tokens > a.tile_tokens ? 2 : 1;          // tiles of rows that hold any
-
-        if (warp == kLoadWarp) {
-            if ((threadIdx.x & 31) == 0) {
-                bool ok = true;
+    if (warp == kLoadWarp) {
+        if ((threadIdx.x & 31) == 0) {
+            bool ok = true;
+            int f = 0, parts = 0, v_asked = 0;       // fills of K (as many of V, or one fewer), parts
+            for (int u = u_lo; u < u_hi && ok;) {
+                const Part p = part_at(a, line, blocks, u, u_hi);
+                if (parts > 0 && !(ok = mbar_wait(q_empty, (uint32_t)(parts - 1) & 1u))) { fail(49); break; }
+                const int both = p.tokens > a.tile_tokens ? 2 : 1;
                 mbar_expect_tx(q_full, (uint32_t)(both * DB * tile_rows * 128));
                 for (int x = 0; x < both; ++x)
 #pragma unroll
                     for (int d = 0; d < DB; ++d)
-                        tma_load_3d(q_s + x * kTileBytes + d * kBlockBytes, &map_q, d * 64, kvh * group, first_token + x * a.tile_tokens, q_full);
-                const int last_page = (b.start + a.cu[seq + 1] - a.cu[seq] - 1) / kPageSize;
+                        tma_load_3d(q_s + x * kTileBytes + d * kBlockBytes, &map_q, d * 64, p.kvh * group, p.first_token + x * a.tile_tokens, q_full);
+                ++parts;
                 auto load = [&](uint8_t* dst, const CUtensorMap* map, int t, uint64_t* bar) {
                     mbar_expect_tx(bar, (uint32_t)kTileBytes);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         // (a page the sequence does not hold is replaced by its last one: its rows are masked, but must be numbers)
-                        const int row = ((seq * a.pages + min(2 * (kt0 + t) + half, last_page)) * a.kv_heads + kvh) * kPageSize;
+                        const int row = ((p.seq * a.pages + min(2 * (p.kt0 + t) + half, p.last_page)) * a.kv_heads + p.kvh) * kPageSize;
 #pragma unroll
                         for (int d = 0; d < DB; ++d) tma_load_2d(dst + d * kBlockBytes + half * (kBlockBytes / 2), map, d * 64, row, bar);
                     }
                 };
-                int t = 0;
-                for (; t < n_kt && ok; ++t) {
-                    const int f = fills + t, s = f % NS;
+                for (int t = 0; t < p.n_kt; ++t, ++f) {
+                    const int s = f % NS;
                     if (f >= NS && !(ok = mbar_wait(&k_empty[s], (uint32_t)(f / NS - 1) & 1u))) { fail(41); break; }
                     load(k_s + s * kTileBytes, &map_k, t, &k_full[s]);
-                    if (f >= NS && !(ok = mbar_wait(&v_empty[s], (uint32_t)(f / NS - 1) & 1u))) {
-                        fail(42);
-                        mbar_wait(&k_full[s], (uint32_t)(f / NS) & 1u);      // (the copy just asked for lands)
-                        break;
-                    }
+                    if (f >= NS && !(ok = mbar_wait(&v_empty[s], (uint32_t)(f / NS - 1) & 1u))) { fail(42); ++f; break; }
                     load(v_s + s * kTileBytes, &map_v, t, &v_full[s]);
+                    ++v_asked;
                 }
-                if (!ok || *failed) {
-                    // the way out: what was asked for lands before the CTA gives up its shared memory
-                    mbar_wait(q_full, (uint32_t)segments & 1u);
-                    OutstandingFill left[8];
-                    const int n = outstanding_fills(fills + t, max(0, fills + t - NS), NS, left);
-                    for (int i = 0; i < n; ++i) { mbar_wait(&k_full[left[i].stage], left[i].parity); mbar_wait(&v_full[left[i].stage], left[i].parity); }
-                }
+                u = p.end;
             }
-        } else if (warp == kMmaWarp) {
-            if ((threadIdx.x & 31) == 0) {
-                const uint32_t idesc_s = instr_desc(kRows, kKeys), idesc_pv = instr_desc(kRows, HD) | (1u << 16);     // V is MN-major
-                const uint64_t desc_q = smem_desc(smem_u32(q_s)), desc_k = smem_desc(smem_u32(k_s)), desc_v = smem_desc_rows(smem_u32(v_s));
-                auto issue_s = [&](int x, int s) {
-#pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks) {
-                        const uint64_t off = (uint64_t)(((uint32_t)(ks / 4) * kBlockBytes + (uint32_t)(ks % 4) * 32) >> 4);
-                        umma_bf16(tmem + (uint32_t)x * 128, desc_q + (uint64_t)(((uint32_t)x * kTileBytes) >> 4) + off,
-                                  desc_k + (uint64_t)(((uint32_t)s * kTileBytes) >> 4) + off, idesc_s, ks > 0 ? 1u : 0u);
-                    }
-                    umma_commit(&s_full[x]);
-                };
-                auto issue_pv = [&](int x, int s, bool first) {
-#pragma unroll
-                    for (int ks = 0; ks < kKeys / 16; ++ks)
-                        umma_bf16_ts(tmem + kTmemO + (uint32_t)x * 128, tmem + (uint32_t)x * 128 + (uint32_t)ks * 8,
-                                     desc_v + (uint64_t)(((uint32_t)s * kTileBytes + (uint32_t)ks * 16 * 128) >> 4), idesc_pv, first && ks == 0 ? 0u : 1u);
-                };
-                bool ok = mbar_wait(q_full, (uint32_t)segments & 1u) && mbar_wait(&k_full[fills % NS], (uint32_t)(fills / NS) & 1u);
-                if (ok) {
-                    any_mma = true;
-                    tc_fence_after();
-                    for (int x = 0; x < both; ++x) issue_s(x, fills % NS);
-                    umma_commit(&k_empty[fills % NS]);
-                } else {
-                    fail(43);
-                }
-                for (int t = 0; t < n_kt && ok; ++t) {
-                    const int f = fills + t, s = f % NS, next = (f + 1) % NS;
-                    for (int x = 0; x < both && ok; ++x) {
-                        if (x == 0 && !(ok = mbar_wait(&v_full[s], (uint32_t)(f / NS) & 1u))) { fail(44); break; }
-                        if (x == 0 && t + 1 < n_kt && !(ok = mbar_wait(&k_full[next], (uint32_t)((f + 1) / NS) & 1u))) { fail(45); break; }
-                        if (!(ok = mbar_wait(&p_full[x], (uint32_t)(scores[x] + t) & 1u))) { fail(46); break; }
-                        tc_fence_after();
-                        issue_pv(x, s, t == 0);
-                        if (t + 1 < n_kt) issue_s(x, next);
-                        else umma_commit(&o_full[x]);
-                    }
-                    if (ok) {
-                        umma_commit(&v_empty[s]);
-                        if (t + 1 < n_kt) umma_commit(&k_empty[next]);
-                    }
-                }
-                if ((!ok || *failed) && any_mma) {
-                    umma_commit(drain_bar);
-                    mbar_wait(drain_bar, 0);
-                }
+            if (!ok || *failed) {
+                // the way out: what was asked for lands before the CTA gives up its shared memory
+                if (parts > 0) mbar_wait(q_full, (uint32_t)(parts - 1) & 1u);
+                OutstandingFill left[8];
+                int n = outstanding_fills(f, max(0, f - NS), NS, left);
+                for (int i = 0; i < n; ++i) mbar_wait(&k_full[left[i].stage], left[i].parity);
+                n = outstanding_fills(v_asked, max(0, v_asked - NS), NS, left);
+                for (int i = 0; i < n; ++i) mbar_wait(&v_full[left[i].stage], left[i].parity);
             }
-        } else {
-            // ---- a thread per row ----------------------------------------------------------------------------------
-            const int x = warp >> 2, row = (warp & 3) * 32 + (threadIdx.x & 31);
-            if (x < both) {
-                const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-                const uint32_t tmem_s = tmem + (uint32_t)x * 128 + lane_base, tmem_o = tmem + kTmemO + (uint32_t)x * 128 + lane_base;
-                constexpr float kLazy = 8.0f;
-                const int x_tokens = min(a.tile_tokens, b.tokens - x * a.tile_tokens);           // tokens of this tile of rows
-                const int first_pos = b.start + b.token0 + x * a.tile_tokens, last_pos = first_pos + x_tokens - 1;
-                const int token = row / group, pos = first_pos + min(token, x_tokens - 1);
-                const bool live = token < x_tokens;
-                float m = -CUDART_INF_F, l = 0.f;
-                bool ok = true;
-                for (int t = 0; t < n_kt && ok; ++t) {
-                    const int key0 = (kt0 + t) * kKeys;
-                    if (!mbar_wait(&s_full[x], (uint32_t)(scores[x] + t) & 1u)) { fail(47); ok = false; break; }
-                    tc_fence_after();
-                    float sv[128];
-                    tmem_ld128(tmem_s, sv);
-                    // every row sees every key of the tile, or a mask is needed
-                    if (key0 + kKeys - 1 > first_pos || (a.window > 0 && key0 <= last_pos - a.window)) {
-                        const int hi = pos - key0, lo = a.window > 0 ? hi - a.window + 1 : 0;
+        }
+    } else if (warp == kMmaWarp) {
+        // One thread issues all products, the tiles' strictly in turn: issued by a thread each, they mix on the tensor cores,
+        // and both tiles then turn scores into weights at the same time (333 against 270 us at 1,024 x 28 heads onto 16,000).
+        if ((threadIdx.x & 31) == 0 && u_lo < u_hi) {
+            const uint32_t idesc_s = instr_desc(kRows, kKeys), idesc_pv = instr_desc(kRows, HD) | (1u << 16);     // V is MN-major
+            const uint64_t desc_q = smem_desc(smem_u32(q_s)), desc_k = smem_desc(smem_u32(k_s)), desc_v = smem_desc_rows(smem_u32(v_s));
+            auto issue_s = [&](int x, int s) {
+                const uint64_t q = desc_q + (uint64_t)(((uint32_t)x * kTileBytes) >> 4), k = desc_k + (uint64_t)(((uint32_t)s * kTileBytes) >> 4);
 #pragma unroll
-                        for (int j = 0; j < 128; ++j)
-                            if (j > hi || j < lo) sv[j] = -CUDART_INF_F;
-                    }
-                    // maximum of the raw scores (the scale is positive)
-                    float top8[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) top8[e] = sv[e];
-#pragma unroll
-                    for (int j = 8; j + 8 < 128; j += 16)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) top8[e] = fmax3(top8[e], sv[j + e], sv[j + 8 + e]);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) top8[e] = fmaxf(top8[e], sv[120 + e]);
-                    const float top = fmaxf(fmax3(top8[0], top8[1], top8[2]), fmax3(fmax3(top8[3], top8[4], top8[5]), top8[6], top8[7])) * a.scale_log2;
-                    if (__any_sync(0xffffffffu, top > m + kLazy)) {
-                        const float mx = fmaxf(m, top), corr = mx == -CUDART_INF_F ? 1.0f : ex2_approx(m - mx);
-                        if (t > 0) {         // (PV of the tile before is done: the scores came after it)
-#pragma unroll
-                            for (int c = 0; c < HD / 32; ++c) {
-                                float acc[32];
-                                tmem_ld32(tmem_o + (uint32_t)(c * 32), acc);
-#pragma unroll
-                                for (int j = 0; j < 32; ++j) acc[j] *= corr;
-                                tmem_st32(tmem_o + (uint32_t)(c * 32), acc);
-                            }
-                        }
-                        l *= corr;
-                        m = mx;
-                    }
-                    const float ref = m == -CUDART_INF_F ? 0.f : m;
-                    const uint64_t scale2 = pack_f32x2(a.scale_log2, a.scale_log2), ref2 = pack_f32x2(-ref, -ref);
-                    uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};      // (the bits of two float zeros)
-#pragma unroll
-                    for (int part = 0; part < 2; ++part) {
-                        uint32_t pk[32];
-#pragma unroll
-                        for (int j = 0; j < 64; j += 2) {
-                            float x0, x1;
-                            unpack_f32x2(fma_f32x2(pack_f32x2(sv[part * 64 + j], sv[part * 64 + j + 1]), scale2, ref2), x0, x1);
-                            const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-                            sum2[(j / 2) & 3] = add_f32x2(sum2[(j / 2) & 3], pack_f32x2(p0, p1));
-                            pk[j / 2] = pack_bf16(p0, p1);
-                        }
-                        tmem_st32_raw(tmem_s + (uint32_t)(part * 32), pk);
-                    }
-                    float lo, hi;
-                    unpack_f32x2(add_f32x2(add_f32x2(sum2[0], sum2[1]), add_f32x2(sum2[2], sum2[3])), lo, hi);
-                    l += lo + hi;
-                    tmem_st_wait();
-                    tc_fence_before();
-                    mbar_arrive(&p_full[x]);
+                for (int ks = 0; ks < HD / 16; ++ks) {
+                    const uint64_t off = (uint64_t)(((uint32_t)(ks / 4) * kBlockBytes + (uint32_t)(ks % 4) * 32) >> 4);
+                    umma_bf16(tmem + (uint32_t)x * 128, q + off, k + off, idesc_s, ks > 0 ? 1u : 0u);
                 }
-                if (ok && !mbar_wait(&o_full[x], (uint32_t)ends[x] & 1u)) { fail(48); ok = false; }
+                umma_commit(&s_full[x]);
+            };
+            auto issue_pv = [&](int x, int s, bool first) {
+                const uint64_t v = desc_v + (uint64_t)(((uint32_t)s * kTileBytes) >> 4);
+#pragma unroll
+                for (int ks = 0; ks < kKeys / 16; ++ks)
+                    umma_bf16_ts(tmem + kTmemO + (uint32_t)x * 128, tmem + (uint32_t)x * 128 + (uint32_t)ks * 8,
+                                 v + (uint64_t)(((uint32_t)ks * 16 * 128) >> 4), idesc_pv, first && ks == 0 ? 0u : 1u);
+            };
+            // fills gone through; weights and parts of each tile of rows; parts (of queries)
+            int f = 0, weights[2] = {0, 0}, ends[2] = {0, 0}, parts = 1;
+            Part p = part_at(a, line, blocks, u_lo, u_hi);
+            int both = p.tokens > a.tile_tokens ? 2 : 1;
+            bool ok = mbar_wait(q_full, 0) && mbar_wait(&k_full[0], 0), any = ok;
+            if (ok) {
                 tc_fence_after();
-                const bool whole = u == pair_at && part_end == pair_at + b.tiles;
-                if (__all_sync(0xffffffffu, ok && !*failed)) {
-                    if (whole) {
-                        const float inv = 1.0f / l;
-                        __nv_bfloat16* dst = a.out + ((size_t)(first_token + x * a.tile_tokens + token) * a.heads + (size_t)kvh * group + (row - token * group)) * HD;
-#pragma unroll
-                        for (int c = 0; c < HD / 32; ++c) {
-                            float o[32];
-                            tmem_ld32(tmem_o + (uint32_t)(c * 32), o);
-                            if (live) {
-#pragma unroll
-                                for (int i = 0; i < 32; i += 8)
-                                    *reinterpret_cast<uint4*>(dst + c * 32 + i) =
-                                        make_uint4(pack_bf16(o[i] * inv, o[i + 1] * inv), pack_bf16(o[i + 2] * inv, o[i + 3] * inv),
-                                                   pack_bf16(o[i + 4] * inv, o[i + 5] * inv), pack_bf16(o[i + 6] * inv, o[i + 7] * inv));
+                for (int x = 0; x < both; ++x) issue_s(x, 0);
+                umma_commit(&k_empty[0]);
+                if (p.n_kt == 1) umma_commit(q_empty);
+            } else {
+                fail(43);
+            }
+            while (ok) {
+                const bool last = p.end >= u_hi;             // the run's last part
+                Part after = p;
+                int both_after = 0;
+                if (!last) { after = part_at(a, line, blocks, p.end, u_hi); both_after = after.tokens > a.tile_tokens ? 2 : 1; }
+                for (int t = 0; t < p.n_kt && ok; ++t, ++f) {
+                    const int s = f % NS, next = (f + 1) % NS;
+                    const bool more = t + 1 < p.n_kt;        // scores to follow: of this part, or of the next one's first tile
+                    const int following = more ? both : both_after;
+                    if (!(ok = mbar_wait(&v_full[s], (uint32_t)(f / NS) & 1u))) { fail(44); break; }
+                    for (int x = 0; x < 2 && ok; ++x) {
+                        if (x < both) {
+                            if (t == 0 && ends[x] > 0 && !(ok = mbar_wait(&o_empty[x], (uint32_t)(ends[x] - 1) & 1u))) { fail(50); break; }
+                            if (!(ok = mbar_wait(&p_full[x], (uint32_t)weights[x] & 1u))) { fail(46); break; }
+                            ++weights[x];
+                            tc_fence_after();
+                            issue_pv(x, s, t == 0);
+                            if (!more) { umma_commit(&o_full[x]); ++ends[x]; }
+                        }
+                        if (x < following) {
+                            if (x == 0) {
+                                if (!(ok = mbar_wait(&k_full[next], (uint32_t)((f + 1) / NS) & 1u))) { fail(45); break; }
+                                if (!more && !(ok = mbar_wait(q_full, (uint32_t)parts & 1u))) { fail(51); break; }
+                                tc_fence_after();
                             }
+                            issue_s(x, next);
                         }
-                    } else {
-                        float* part = a.parts + (((size_t)blockIdx.x * 2 + (pair_at < u_lo ? 0 : 1)) * 2 + x) * (HD + 2) * kRows + row;
-#pragma unroll
-                        for (int c = 0; c < HD / 32; ++c) {
-                            float o[32];
-                            tmem_ld32(tmem_o + (uint32_t)(c * 32), o);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) part[(size_t)(c * 32 + i) * kRows] = o[i];
-                        }
-                        part[(size_t)HD * kRows] = m;
-                        part[(size_t)(HD + 1) * kRows] = l;
+                    }
+                    if (!ok) break;
+                    umma_commit(&v_empty[s]);
+                    if (following) {
+                        umma_commit(&k_empty[next]);
+                        // the last scores of a part: its queries' memory may take the next part's
+                        if (more ? t + 2 == p.n_kt : after.n_kt == 1) umma_commit(q_empty);
                     }
                 }
-                tc_fence_before();      // (this segment's reads of tensor memory come before the next one's writes)
+                if (last) break;
+                p = after;
+                both = both_after;
+                ++parts;
+            }
+            if ((!ok || *failed) && any) {
+                umma_commit(drain_bar);
+                mbar_wait(drain_bar, 0);
             }
         }
-        __syncwarp();
-        __syncthreads();
-        tc_fence_after();
-        if (*failed) break;
-        if (threadIdx.x == 0 && pair_at >= u_lo) {
-            const bool whole = part_end == pair_at + b.tiles;
-            a.cuts[block_number * a.kv_heads + kvh] =
-                ChunkCut{first_token, kvh, whole ? 0 : b.tokens, (int)blockIdx.x, (pair_at + b.tiles - 1) / run, {0, 0, 0}};
+    } else {
+        // ---- a thread a row ---------------------------------------------------------------------------------------------
+        const int x = warp >> 2, quarter = warp & 3, row = quarter * 32 + (threadIdx.x & 31);
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+        const uint32_t tmem_s = tmem + (uint32_t)x * 128 + lane_base;                            // this tile's scores; weights over them
+        const uint32_t tmem_o = tmem + kTmemO + (uint32_t)x * 128 + lane_base;
+        constexpr float kLazy = 8.0f;
+        int scores = 0, ends = 0;
+        bool ok = true;
+        for (int u = u_lo; u < u_hi && ok;) {
+            const Part p = part_at(a, line, blocks, u, u_hi);
+            if (threadIdx.x == 0 && p.pair_at >= u_lo)
+                a.cuts[p.number] = ChunkCut{p.first_token, p.kvh, p.end == p.pair_at + p.tiles ? 0 : p.tokens, (int)blockIdx.x, (p.pair_at + p.tiles - 1) / run, {0, 0, 0}};
+            const bool whole = u == p.pair_at && p.end == p.pair_at + p.tiles;
+            const int cut_slot = p.pair_at < u_lo ? 0 : 1;
+            u = p.end;
+            const int x_tokens = min(a.tile_tokens, p.tokens - x * a.tile_tokens);               // tokens of this tile of rows
+            if (x_tokens <= 0) continue;
+            const int first_pos = p.first_pos + x * a.tile_tokens, last_pos = first_pos + x_tokens - 1;
+            const int token = row / group, pos = first_pos + min(token, x_tokens - 1);
+            float m = -CUDART_INF_F, l = 0.f;
+            for (int t = 0; t < p.n_kt; ++t) {
+                const int key0 = (p.kt0 + t) * kKeys;
+                if (!mbar_wait(&s_full[x], (uint32_t)scores & 1u)) { fail(47); ok = false; break; }
+                ++scores;
+                tc_fence_after();
+                float sv[128];
+                tmem_ld128(tmem_s, sv);
+                // every row sees every key of the tile, or a mask is needed
+                if (key0 + kKeys - 1 > first_pos || (a.window > 0 && key0 <= last_pos - a.window)) {
+                    const int hi = pos - key0, lo = a.window > 0 ? hi - a.window + 1 : 0;        // this row's keys: lo .. hi
+#pragma unroll
+                    for (int j = 0; j < 128; ++j)
+                        if (j > hi || j < lo) sv[j] = -CUDART_INF_F;
+                }
+                float top8[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top8[e] = fmaxf(sv[e], sv[8 + e]);
+#pragma unroll
+                for (int j = 16; j < 128; j += 16)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top8[e] = fmax3(top8[e], sv[j + e], sv[j + 8 + e]);
+                // maximum of the raw scores (the scale is positive)
+                const float top = fmaxf(fmax3(top8[0], top8[1], top8[2]), fmax3(fmax3(top8[3], top8[4], top8[5]), top8[6], top8[7])) * a.scale_log2;
+                if (__any_sync(0xffffffffu, top > m + kLazy)) {
+                    const float mx = fmaxf(m, top), corr = mx == -CUDART_INF_F ? 1.0f : ex2_approx(m - mx);
+                    if (t > 0) {             // (PV of the tile before is done: the scores came after it)
+#pragma unroll
+                        for (int c = 0; c < HD / 16; ++c) {
+                            float acc[16];
+                            tmem_ld16(tmem_o + (uint32_t)(c * 16), acc);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) acc[j] *= corr;
+                            tmem_st16(tmem_o + (uint32_t)(c * 16), acc);
+                        }
+                    }
+                    l *= corr;
+                    m = mx;
+                }
+                const float ref = m == -CUDART_INF_F ? 0.f : m;
+                const uint64_t scale2 = pack_f32x2(a.scale_log2, a.scale_log2), ref2 = pack_f32x2(-ref, -ref);
+                uint64_t sum2[2] = {0ull, 0ull};              // (the bits of two float zeros)
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int j = 0; j < 64; j += 2) {
+                        float x0, x1;
+                        unpack_f32x2(fma_f32x2(pack_f32x2(sv[part * 64 + j], sv[part * 64 + j + 1]), scale2, ref2), x0, x1);
+                        x0 = ex2_approx(x0);
+                        x1 = ex2_approx(x1);
+                        sum2[(j / 2) & 1] = add_f32x2(sum2[(j / 2) & 1], pack_f32x2(x0, x1));
+                        pk[j / 2] = pack_bf16(x0, x1);
+                    }
+                    tmem_st32_raw(tmem_s + (uint32_t)(part * 32), pk);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&p_full[x]);
+                float lo2, hi2;
+                unpack_f32x2(add_f32x2(sum2[0], sum2[1]), lo2, hi2);
+                l += lo2 + hi2;
+            }
+            if (ok && !mbar_wait(&o_full[x], (uint32_t)ends & 1u)) { fail(48); ok = false; }
+            ++ends;
+            tc_fence_after();
+            if (!__all_sync(0xffffffffu, ok && !*failed)) { ok = false; break; }
+            const bool live = token < x_tokens;
+            const float inv = 1.0f / l;
+            __nv_bfloat16* dst = a.out + ((size_t)(p.first_token + x * a.tile_tokens + token) * a.heads + (size_t)p.kvh * group + (row - token * group)) * HD;
+            float* part = a.parts + (((size_t)blockIdx.x * 2 + cut_slot) * 2 + x) * (HD + 2) * kRows + row;
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+                float o[32];
+                tmem_ld32(tmem_o + (uint32_t)(c * 32), o);
+                if (c == HD / 32 - 1) {      // all of it has been read
+                    tc_fence_before();
+                    mbar_arrive(&o_empty[x]);
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) part[(size_t)(c * 32 + i) * kRows] = o[i];
+                } else if (live) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+                        *reinterpret_cast<uint4*>(dst + c * 32 + i) =
+                            make_uint4(pack_bf16(o[i] * inv, o[i + 1] * inv), pack_bf16(o[i + 2] * inv, o[i + 3] * inv),
+                                       pack_bf16(o[i + 4] * inv, o[i + 5] * inv), pack_bf16(o[i + 6] * inv, o[i + 7] * inv));
+                }
+            }
+            if (!whole) {
+                part[(size_t)HD * kRows] = m;
+                part[(size_t)(HD + 1) * kRows] = l;
+            }
         }
-        fills += n_kt;
-        ++segments;
-        for (int x = 0; x < both; ++x) { scores[x] += n_kt; ++ends[x]; }
-        u = part_end;
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
-// Puts the parts of a cut pair together, in the order of the line: blockIdx.x the pair, blockIdx.y 32 of its dimensions, a
-// thread a row.
+// Puts the parts of a cut pair together, in the order of the line: blockIdx.x the pair, blockIdx.y eight of its dimensions, a
+// thread a row; the loads of four parts are under way together.
+constexpr int kJoinDims = 8;
 template <int HD>
 __global__ void __launch_bounds__(2 * kRows) attention_chunk_join_kernel(ChunkArgs a) {
     pdl_wait();              // (every CTA waits: this kernel must not end before the one it follows)
@@ -459,27 +530,38 @@ __global__ void __launch_bounds__(2 * kRows) attention_chunk_join_kernel(ChunkAr
     if (token >= min(a.tile_tokens, cut.tokens - x * a.tile_tokens)) return;
     const float* first = a.parts + (size_t)x * (HD + 2) * kRows + row;
     const size_t stride = (size_t)2 * (HD + 2) * kRows;                 // of a part of both tiles; two a CTA
-    float m = -CUDART_INF_F;
-    for (int c = cut.first; c <= cut.last; ++c) m = fmaxf(m, first[((size_t)c * 2 + (c == cut.first ? 1 : 0)) * stride + (size_t)HD * kRows]);
-    float l = 0.f, o[32];
+    float m = -CUDART_INF_F, l = 0.f, o[kJoinDims];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) o[i] = 0.f;
-    for (int c = cut.first; c <= cut.last; ++c) {
-        const float* part = first + ((size_t)c * 2 + (c == cut.first ? 1 : 0)) * stride;
-        const float pm = part[(size_t)HD * kRows], pl = part[(size_t)(HD + 1) * kRows];
-        // (no key seen: 0; no maximum, because every score is NaN: 1, and the sum is NaN)
-        const float f = pm == -CUDART_INF_F ? (pl == 0.f ? 0.f : 1.f) : ex2_approx(pm - m);
-        if (f == 0.f) continue;
-        l += pl * f;
+    for (int i = 0; i < kJoinDims; ++i) o[i] = 0.f;
+    for (int c0 = cut.first; c0 <= cut.last; c0 += 4) {
+        float pm[4], pl[4], v[4][kJoinDims];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = fmaf(part[(size_t)(blockIdx.y * 32 + i) * kRows], f, o[i]);
+        for (int k = 0; k < 4; ++k) {
+            const int c = min(c0 + k, cut.last);
+            const float* part = first + ((size_t)c * 2 + (c == cut.first ? 1 : 0)) * stride;
+            pm[k] = part[(size_t)HD * kRows];
+            pl[k] = part[(size_t)(HD + 1) * kRows];
+#pragma unroll
+            for (int i = 0; i < kJoinDims; ++i) v[k][i] = part[(size_t)(blockIdx.y * kJoinDims + i) * kRows];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (c0 + k > cut.last) break;
+            const float top = fmaxf(m, pm[k]);
+            // (no key seen: 0; no maximum, because every score is NaN: 1, and the sum is NaN)
+            const float f = m == -CUDART_INF_F ? (l == 0.f ? 0.f : 1.f) : ex2_approx(m - top);
+            const float g = pm[k] == -CUDART_INF_F ? (pl[k] == 0.f ? 0.f : 1.f) : ex2_approx(pm[k] - top);
+            m = top;
+            l = l * f + pl[k] * g;
+#pragma unroll
+            for (int i = 0; i < kJoinDims; ++i) o[i] = o[i] * f + v[k][i] * g;
+        }
     }
     const float inv = 1.0f / l;
-    __nv_bfloat16* dst = a.out + ((size_t)(cut.first_token + x * a.tile_tokens + token) * a.heads + (size_t)cut.kv_head * group + (row - token * group)) * HD + blockIdx.y * 32;
-#pragma unroll
-    for (int i = 0; i < 32; i += 8)
-        *reinterpret_cast<uint4*>(dst + i) = make_uint4(pack_bf16(o[i] * inv, o[i + 1] * inv), pack_bf16(o[i + 2] * inv, o[i + 3] * inv),
-                                                        pack_bf16(o[i + 4] * inv, o[i + 5] * inv), pack_bf16(o[i + 6] * inv, o[i + 7] * inv));
+    __nv_bfloat16* dst = a.out + ((size_t)(cut.first_token + x * a.tile_tokens + token) * a.heads + (size_t)cut.kv_head * group + (row - token * group)) * HD +
+                         blockIdx.y * kJoinDims;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv), pack_bf16(o[4] * inv, o[5] * inv),
+                                                pack_bf16(o[6] * inv, o[7] * inv));
 }
 
 constexpr int kDevices = 64;
@@ -499,7 +581,8 @@ int sm_count() {
 template <int HD>
 void launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkArgs& a, int blocks, int least_run, cudaStream_t stream) {
     constexpr int NS = stages_of(HD);
-    const size_t smem = 1024 + (size_t)(2 + 2 * NS) * (HD / 64) * kBlockBytes + (8 + 4 * NS) * sizeof(uint64_t) + 8 + (size_t)(a.seqs + blocks + 2) * sizeof(int);
+    const size_t smem = 1024 + (size_t)(2 + 2 * NS) * (HD / 64) * kBlockBytes + (11 + 4 * NS) * sizeof(uint64_t) + 8 +
+                        (size_t)(4 * a.seqs + blocks + 2) * sizeof(int);
     auto kernel = attention_chunk_kernel<HD>;
     static bool prepared[kDevices] = {};
     const int dev = this_device();
@@ -510,7 +593,7 @@ void launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
     }
     note_launch(2);
     launch_kernel("attention_chunk", kernel, dim3((unsigned)sm_count()), dim3(kThreads), smem, stream, 1, dependent_launch_enabled(), mq, mk, mv, a, least_run);
-    launch_kernel("attention_chunk", attention_chunk_join_kernel<HD>, dim3((unsigned)(blocks * a.kv_heads), HD / 32), dim3(2 * kRows), 0, stream, 1,
+    launch_kernel("attention_chunk", attention_chunk_join_kernel<HD>, dim3((unsigned)(blocks * a.kv_heads), HD / kJoinDims), dim3(2 * kRows), 0, stream, 1,
                   dependent_launch_enabled(), a);
 }
 
