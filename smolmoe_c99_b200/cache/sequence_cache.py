@@ -24,7 +24,7 @@ from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
-from ..kernels.ops import PAGE_SIZE   # one number for host and kernels; the library's own is checked when it is loaded
+from ..kernels.ops import PAGE_SIZE, QuantLayer   # PAGE_SIZE: one number for host and kernels, checked when the library is loaded
 from ..parts.base import KVNeed, StateNeed
 from .allocators import CacheFull, CacheStateError, PageAllocator, SlotAllocator
 
@@ -48,6 +48,14 @@ class LayerCache:
     state: Optional[torch.Tensor] = None  # [slots, *shape]
     k_scale: Optional[torch.Tensor] = None  # an 8-bit cache: uint8 [pages, kv_heads, PAGE_SIZE]
     v_scale: Optional[torch.Tensor] = None
+
+    def quant_layer(self) -> QuantLayer:
+        """The pools of an 8-bit cache as the kernels take them, checked when first asked for (and again where a tensor of
+        the layer has been exchanged)."""
+        layer = self.__dict__.get("_quant")
+        if layer is None or not layer.made_of(self):
+            layer = self.__dict__["_quant"] = QuantLayer(self)
+        return layer
 
 
 class KVGroup:

@@ -902,13 +902,12 @@ long long attention_quant_workspace(int head_dim, int row_tiles, int pairs, int 
     return warps * 2 * 8 * row_tiles * ((head_dim <= 64 ? 64 : 128) + 4) + (long long)pairs * (long long)(sizeof(Cut) / sizeof(float));
 }
 
-void attention_quant(const void* q, void* out, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window, int fmt,
-                     const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale, long long pool_pages,
-                     const int32_t* page_table, int slots, int table_stride, const int32_t* slot_ids, const int32_t* seq_ends,
-                     const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles, int pairs, int cluster, float* workspace,
-                     long long workspace_floats, cudaStream_t stream) {
+void attention_quant(const QuantPools& p, const void* q, void* out, int n_seqs, int heads, float scale, int window, const int32_t* slot_ids,
+                     const int32_t* seq_ends, const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles, int pairs, int cluster,
+                     float* workspace, long long workspace_floats, cudaStream_t stream) {
     if (n_seqs <= 0 || pairs <= 0) return;
-    if (!attention_quant_supports(heads, kv_heads, head_dim, pool_pages))
+    const int kv_heads = p.kv_heads, head_dim = p.head_dim;
+    if (!attention_quant_supports(heads, kv_heads, head_dim, p.pages))
         throw std::invalid_argument("attention_quant: " + std::to_string(heads) + " heads on " + std::to_string(kv_heads) + " of size " +
                                     std::to_string(head_dim) + " (multiples of 16 up to 128, at most 16 heads a kv head), or a pool of 2^31 rows");
     if (cluster < 0 || cluster > kMaxCluster) throw std::invalid_argument("attention_quant: clusters of " + std::to_string(cluster) + " CTAs");
@@ -917,11 +916,11 @@ void attention_quant(const void* q, void* out, int n_seqs, int heads, int kv_hea
     if (n_seqs > kMaxSeqs) throw std::invalid_argument("attention_quant: more than " + std::to_string(kMaxSeqs) + " sequences");
     if ((row_tiles != 1 && row_tiles != 2 && (row_tiles != 4 || head_dim > 64)) || 8 * row_tiles < group)
         throw std::invalid_argument("attention_quant: " + std::to_string(row_tiles) + " tiles of rows");
-    if (((uintptr_t)q | (uintptr_t)out) & 15 || ((uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_scale | (uintptr_t)v_scale) & 15)
+    if (((uintptr_t)q | (uintptr_t)out) & 15 || ((uintptr_t)p.k_codes | (uintptr_t)p.v_codes | (uintptr_t)p.k_scale | (uintptr_t)p.v_scale) & 15)
         throw std::invalid_argument("attention_quant: operands must be 16-byte aligned");
     if (workspace_floats < attention_quant_workspace(head_dim, row_tiles, pairs, cluster)) throw std::invalid_argument("attention_quant: the workspace is too small");
-    AttnArgs a{(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)k_pool, (const uint8_t*)v_pool, (const uint8_t*)k_scale,
-               (const uint8_t*)v_scale, {page_table, slots, table_stride, pool_pages}, slot_ids, seq_ends, cu_seqlens, n_seqs, heads,
+    AttnArgs a{(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)p.k_codes, (const uint8_t*)p.v_codes, (const uint8_t*)p.k_scale,
+               (const uint8_t*)p.v_scale, {p.page_table, p.slots, p.table_stride, p.pages}, slot_ids, seq_ends, cu_seqlens, n_seqs, heads,
                kv_heads, head_dim, window, most_new, 8 * row_tiles / group, pairs, cluster, 0,
                cluster ? kClusterTile : line_tile(row_tiles), scale * 1.4426950408889634f, (Cut*)workspace,
                workspace + (cluster ? 0 : (long long)pairs * (long long)(sizeof(Cut) / sizeof(float))), error_word()};
@@ -929,16 +928,16 @@ void attention_quant(const void* q, void* out, int n_seqs, int heads, int kv_hea
     if (head_dim == 64 || head_dim == 128) {
         // the pools as rows of codes; a box is a tile of positions of one kv head
         const CUtensorMapSwizzle swizzle = head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
-        const uint64_t rows = (uint64_t)pool_pages * kv_heads * kPageSize;
-        mk = tiled_map_2d("attention_quant", CU_TENSOR_MAP_DATA_TYPE_UINT8, k_pool, (uint64_t)head_dim, rows, (uint64_t)head_dim, (uint32_t)head_dim,
+        const uint64_t rows = (uint64_t)p.pages * kv_heads * kPageSize;
+        mk = tiled_map_2d("attention_quant", CU_TENSOR_MAP_DATA_TYPE_UINT8, p.k_codes, (uint64_t)head_dim, rows, (uint64_t)head_dim, (uint32_t)head_dim,
                           (uint32_t)a.tile, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
-        mv = tiled_map_2d("attention_quant", CU_TENSOR_MAP_DATA_TYPE_UINT8, v_pool, (uint64_t)head_dim, rows, (uint64_t)head_dim, (uint32_t)head_dim,
+        mv = tiled_map_2d("attention_quant", CU_TENSOR_MAP_DATA_TYPE_UINT8, p.v_codes, (uint64_t)head_dim, rows, (uint64_t)head_dim, (uint32_t)head_dim,
                           (uint32_t)a.tile, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
     }
     const LaunchSizes sizes{pairs, a.block_tokens * group, max_len};
-    if (fmt == QUANT_FP8) launch_fmt<QUANT_FP8>(a, row_tiles, mk, mv, sizes, stream);
-    else if (fmt == QUANT_INT8) launch_fmt<QUANT_INT8>(a, row_tiles, mk, mv, sizes, stream);
-    else throw std::invalid_argument("attention_quant: unknown format " + std::to_string(fmt));
+    if (p.fmt == QUANT_FP8) launch_fmt<QUANT_FP8>(a, row_tiles, mk, mv, sizes, stream);
+    else if (p.fmt == QUANT_INT8) launch_fmt<QUANT_INT8>(a, row_tiles, mk, mv, sizes, stream);
+    else throw std::invalid_argument("attention_quant: unknown format " + std::to_string(p.fmt));
 }
 
 }  // namespace sm

@@ -130,23 +130,21 @@ SM_API int sm_kv_store(const void* k_packed, const void* v_packed, int dt, int T
     });
 }
 
-SM_API int sm_kv_quant_store(const void* k_packed, const void* v_packed, int dt, int T, int kv_heads, int head_dim, void* k_rows,
-                             void* v_rows, int fmt, void* k_pool, void* v_pool, void* k_scale, void* v_scale,
-                             long long pool_pages, const int32_t* positions, const int32_t* page_table, int slots, int table_stride,
-                             const int32_t* token_slot, void* stream) {
+// (the 8-bit cache's functions take a layer's pools as one record: a call from Python then converts few arguments)
+SM_API int sm_quant_pools_bytes() { return (int)sizeof(sm::QuantPools); }
+
+SM_API int sm_kv_quant_store(const sm::QuantPools* pools, const void* k_packed, const void* v_packed, int dt, int T, void* k_rows, void* v_rows,
+                             const int32_t* positions, const int32_t* token_slot, void* stream) {
     return guarded([&] {
-        sm::kv_quant_store(k_packed, v_packed, (sm::DType)dt, T, kv_heads, head_dim, k_rows, v_rows, fmt, k_pool, v_pool, k_scale,
-                           v_scale, pool_pages, positions, page_table, slots, table_stride, token_slot, (cudaStream_t)stream);
+        sm::kv_quant_store(*pools, k_packed, v_packed, (sm::DType)dt, T, k_rows, v_rows, positions, token_slot, (cudaStream_t)stream);
     });
 }
 
-SM_API int sm_kv_quant_load(int fmt, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
-                            long long pool_pages, int dt, int n_seqs, int kv_heads, int head_dim, const int32_t* slot_ids,
-                            const int32_t* seq_ends, const int32_t* page_table, int slots, int table_stride, void* k_out, void* v_out, int32_t* out_table, int pages,
-                            int whole, const int32_t* cu_seqlens, int skip_new, int attend, int window, void* stream) {
+SM_API int sm_kv_quant_load(const sm::QuantPools* pools, int dt, int n_seqs, const int32_t* slot_ids, const int32_t* seq_ends, void* k_out,
+                            void* v_out, int32_t* out_table, int pages, int whole, const int32_t* cu_seqlens, int skip_new, int attend,
+                            int window, void* stream) {
     return guarded([&] {
-        sm::kv_quant_load(fmt, k_pool, v_pool, k_scale, v_scale, pool_pages, (sm::DType)dt, n_seqs, kv_heads, head_dim, slot_ids,
-                          seq_ends, page_table, slots, table_stride, k_out, v_out, out_table, pages, whole != 0, cu_seqlens, skip_new,
+        sm::kv_quant_load(*pools, (sm::DType)dt, n_seqs, slot_ids, seq_ends, k_out, v_out, out_table, pages, whole != 0, cu_seqlens, skip_new,
                           attend != 0, window, (cudaStream_t)stream);
     });
 }
@@ -263,15 +261,12 @@ SM_API long long sm_attention_quant_workspace(int head_dim, int row_tiles, int p
     return sm::attention_quant_workspace(head_dim, row_tiles, pairs, cluster);
 }
 
-SM_API int sm_attention_quant(const void* q, void* out, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window,
-                              int fmt, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
-                              long long pool_pages, const int32_t* page_table, int slots, int table_stride, const int32_t* slot_ids,
-                              const int32_t* seq_ends, const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles,
-                              int pairs, int cluster, float* workspace, long long workspace_floats, void* stream) {
+SM_API int sm_attention_quant(const sm::QuantPools* pools, const void* q, void* out, int n_seqs, int heads, float scale, int window,
+                              const int32_t* slot_ids, const int32_t* seq_ends, const int32_t* cu_seqlens, int max_len, int most_new,
+                              int row_tiles, int pairs, int cluster, float* workspace, long long workspace_floats, void* stream) {
     return guarded([&] {
-        sm::attention_quant(q, out, n_seqs, heads, kv_heads, head_dim, scale, window, fmt, k_pool, v_pool, k_scale, v_scale,
-                            pool_pages, page_table, slots, table_stride, slot_ids, seq_ends, cu_seqlens, max_len, most_new,
-                            row_tiles, pairs, cluster, workspace, workspace_floats, (cudaStream_t)stream);
+        sm::attention_quant(*pools, q, out, n_seqs, heads, scale, window, slot_ids, seq_ends, cu_seqlens, max_len, most_new, row_tiles, pairs,
+                            cluster, workspace, workspace_floats, (cudaStream_t)stream);
     });
 }
 

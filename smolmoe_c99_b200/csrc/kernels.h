@@ -77,23 +77,28 @@ void kv_store(const void* k_packed, const void* v_packed, DType dt, int T, int k
               const int32_t* token_slot, const int32_t* token_end, cudaStream_t stream);
 
 // ---- kv_quant.cu ----------------------------------------------------------------------
-// The 8-bit cache (format and pools: kv_quant.cuh; fmt: 0 e4m3, 1 int8). kv_quant_store: a step's packed keys and values
-// [T, kv_heads, head_dim] (F32 or BF16) as codes and exponents into the pages of their positions; k_rows, v_rows
-// (nullable) receive what the cache then stands for, in dt. kv_quant_load: the pages of n_seqs sequences as values of dt,
-// [n_seqs, pages, kv_heads, 64, head_dim], positions at and past seq_ends[i] as zeros (pages wholly past it only if
-// `whole`, else they are left alone), and out_table [slots, pages] to find them by slot. page_table is [slots, table_stride];
-// a place outside it or the pools (pool_pages) is left out and recorded in the error word. Sequences that bring at
-// most `skip_new` tokens by cu_seqlens [n_seqs + 1] are left out. `attend`: for a kernel that multiplies masked values by
-// zero weights: a value row without a scale is read as zeros and its key as NaN instead (a token that sees it is NaN either
-// way), and pages of 128 positions that no token of the step sees in `window` are left alone.
-void kv_quant_store(const void* k_packed, const void* v_packed, DType dt, int T, int kv_heads, int head_dim, void* k_rows,
-                    void* v_rows, int fmt, void* k_pool, void* v_pool, void* k_scale, void* v_scale, long long pool_pages,
-                    const int32_t* positions, const int32_t* page_table, int slots, int table_stride, const int32_t* token_slot,
-                    cudaStream_t stream);
-void kv_quant_load(int fmt, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
-                   long long pool_pages, DType dt, int n_seqs, int kv_heads, int head_dim, const int32_t* slot_ids, const int32_t* seq_ends,
-                   const int32_t* page_table, int slots, int table_stride, void* k_out, void* v_out, int32_t* out_table, int pages, bool whole,
-                   const int32_t* cu_seqlens, int skip_new, bool attend, int window, cudaStream_t stream);
+// One layer's 8-bit cache (format and pools: kv_quant.cuh).
+struct QuantPools {
+    void *k_codes, *v_codes;         // [pages, kv_heads, 64, head_dim]
+    void *k_scale, *v_scale;         // [pages, kv_heads, 64]
+    const int32_t* page_table;       // [slots, table_stride]
+    long long pages;
+    int fmt, kv_heads, head_dim;     // fmt: 0 e4m3, 1 int8
+    int slots, table_stride;
+};
+// kv_quant_store: a step's packed keys and values [T, kv_heads, head_dim] (F32 or BF16) as codes and exponents into the pages
+// of their positions; k_rows, v_rows (nullable) receive what the cache then stands for, in dt. kv_quant_load: the pages of
+// n_seqs sequences as values of dt, [n_seqs, pages, kv_heads, 64, head_dim], positions at and past seq_ends[i] as zeros (pages
+// wholly past it only if `whole`, else they are left alone), and out_table [slots, pages] to find them by slot. A place outside
+// the page table or the pools is left out and recorded in the error word. Sequences that bring at most `skip_new` tokens by
+// cu_seqlens [n_seqs + 1] are left out. `attend`: for a kernel that multiplies masked values by zero weights: a value row
+// without a scale is read as zeros and its key as NaN instead (a token that sees it is NaN either way), and pages of 128
+// positions that no token of the step sees in `window` are left alone.
+void kv_quant_store(const QuantPools& pools, const void* k_packed, const void* v_packed, DType dt, int T, void* k_rows, void* v_rows,
+                    const int32_t* positions, const int32_t* token_slot, cudaStream_t stream);
+void kv_quant_load(const QuantPools& pools, DType dt, int n_seqs, const int32_t* slot_ids, const int32_t* seq_ends, void* k_out, void* v_out,
+                   int32_t* out_table, int pages, bool whole, const int32_t* cu_seqlens, int skip_new, bool attend, int window,
+                   cudaStream_t stream);
 
 // ---- gemm_simt.cu ---------------------------------------------------------------------
 // out[t, n] (+)= sum_k x[t, k] * w[n, k] + bias[n]; float FMA in ascending k for every
@@ -272,11 +277,9 @@ void attention_decode(const void* q, void* out, int B, int heads, int kv_heads, 
 // joins what they cut (workspace, attention_quant.cu). head_dim: multiples of 16 up to 128; at most 16 heads a kv head.
 bool attention_quant_supports(int heads, int kv_heads, int head_dim, long long pool_pages);
 long long attention_quant_workspace(int head_dim, int row_tiles, int pairs, int cluster);   // floats
-void attention_quant(const void* q, void* out, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window, int fmt,
-                     const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale, long long pool_pages,
-                     const int32_t* page_table, int slots, int table_stride, const int32_t* slot_ids, const int32_t* seq_ends,
-                     const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles, int pairs, int cluster, float* workspace,
-                     long long workspace_floats, cudaStream_t stream);
+void attention_quant(const QuantPools& pools, const void* q, void* out, int n_seqs, int heads, float scale, int window, const int32_t* slot_ids,
+                     const int32_t* seq_ends, const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles, int pairs, int cluster,
+                     float* workspace, long long workspace_floats, cudaStream_t stream);
 
 // ---- attention_chunk_tc.cu ------------------------------------------------------------
 // The same attention for sequences that bring more than `skip_new` tokens, over their pages as bfloat16 values as

@@ -53,7 +53,7 @@ struct StoreArgs {
     const int32_t* token_slot;   // [T]
     QuantPages pages;
     int kv_heads, head_dim;
-    long long rows_of_each;      // T * kv_heads
+    unsigned rows_of_each;       // T * kv_heads
     int* error;
 };
 
@@ -66,19 +66,24 @@ __global__ void __launch_bounds__(kThreads) kv_quant_store_kernel(StoreArgs a, i
     pdl_wait();                  // the rows come from the kernel before
     pdl_launch_dependents();
     const int per_block = kThreads / lanes;
-    const long long row0 = (long long)blockIdx.x * per_block * kStoreRows + threadIdx.x / lanes;
+    const unsigned row0 = blockIdx.x * (per_block * kStoreRows) + threadIdx.x / lanes;
     const int part = threadIdx.x % lanes;
-    const int which = blockIdx.y;
-    const T* packed = (const T*)a.packed[which];
+    // (chosen, not indexed: an index that is not a constant would put the arguments into local memory)
+    const bool keys = blockIdx.y == 0;
+    const T* packed = (const T*)(keys ? a.packed[0] : a.packed[1]);
+    T* rows = (T*)(keys ? a.rows[0] : a.rows[1]);
+    uint8_t* codes = keys ? a.codes[0] : a.codes[1];
+    uint8_t* scales = keys ? a.scales[0] : a.scales[1];
     float x[kStoreRows][8];
-    int at_token[kStoreRows], at_slot[kStoreRows];
+    int at_token[kStoreRows], at_slot[kStoreRows], kv_head[kStoreRows];
     bool mine[kStoreRows];
 #pragma unroll
     for (int u = 0; u < kStoreRows; ++u) {
-        const long long row = row0 + u * per_block;
+        const unsigned row = row0 + u * per_block;
         const bool live = row < a.rows_of_each;
         mine[u] = live && part * 8 < a.head_dim;
-        const int t = live ? (int)(row / a.kv_heads) : 0;
+        const unsigned t = live ? row / (unsigned)a.kv_heads : 0;
+        kv_head[u] = (int)(row - t * (unsigned)a.kv_heads);
         at_token[u] = a.positions[t];
         at_slot[u] = a.token_slot[t];
 #pragma unroll
@@ -90,13 +95,15 @@ __global__ void __launch_bounds__(kThreads) kv_quant_store_kernel(StoreArgs a, i
     for (int u = 0; u < kStoreRows; ++u) page[u] = at_token[u] < 0 ? -1 : a.pages.at(at_slot[u], at_token[u] / kPageSize);
 #pragma unroll
     for (int u = 0; u < kStoreRows; ++u) {
-        const long long row = row0 + u * per_block;
+        const unsigned row = row0 + u * per_block;
         uint32_t amax = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(x[u][i]) & 0x7fffffffu);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-            if (o < lanes) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        for (int o = 16; o > 0; o >>= 1) {
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, amax, o);
+            if (o < lanes) amax = max(amax, other);
+        }
         if (mine[u]) {
             const int byte = scale_byte<FMT>(amax);
             uint32_t lo = 0, hi = 0;
@@ -106,19 +113,19 @@ __global__ void __launch_bounds__(kThreads) kv_quant_store_kernel(StoreArgs a, i
                 hi = encode4<FMT>(x[u][4] * up, x[u][5] * up, x[u][6] * up, x[u][7] * up);
             }
             if (page[u] >= 0) {
-                const size_t cell = ((size_t)page[u] * a.kv_heads + (size_t)(row % a.kv_heads)) * kPageSize + at_token[u] % kPageSize;
-                *reinterpret_cast<uint2*>(a.codes[which] + cell * a.head_dim + part * 8) = make_uint2(lo, hi);
-                if (part == 0) a.scales[which][cell] = (uint8_t)byte;
+                const size_t cell = ((size_t)page[u] * a.kv_heads + kv_head[u]) * kPageSize + at_token[u] % kPageSize;
+                *reinterpret_cast<uint2*>(codes + cell * a.head_dim + part * 8) = make_uint2(lo, hi);
+                if (part == 0) scales[cell] = (uint8_t)byte;
             } else if (a.error) {
                 atomicExch(a.error, kBadPlaceInStore);
             }
-            if (a.rows[which] != nullptr) {
+            if (rows != nullptr) {
                 const float scale = scale_of(byte);
                 float v[4], w[4];
                 decode4<FMT>(lo, v);
                 decode4<FMT>(hi, w);
                 const float y[8] = {v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale, w[0] * scale, w[1] * scale, w[2] * scale, w[3] * scale};
-                store8((T*)a.rows[which] + (size_t)row * a.head_dim + part * 8, y);
+                store8(rows + (size_t)row * a.head_dim + part * 8, y);
             }
         }
     }
@@ -206,47 +213,47 @@ __global__ void __launch_bounds__(kThreads) kv_quant_load_kernel(LoadArgs a) {
     }
 }
 
-void check_sizes(const char* who, int kv_heads, int head_dim, int fmt) {
-    if (kv_heads <= 0 || head_dim <= 0 || head_dim % 8 || head_dim > 256)
-        throw std::invalid_argument(std::string(who) + ": head_dim " + std::to_string(head_dim) + " is not a multiple of 8 up to 256");
-    if (fmt != QUANT_FP8 && fmt != QUANT_INT8) throw std::invalid_argument(std::string(who) + ": unknown format " + std::to_string(fmt));
+void check_pools(const char* who, const QuantPools& p) {
+    if (p.kv_heads <= 0 || p.head_dim <= 0 || p.head_dim % 8 || p.head_dim > 256)
+        throw std::invalid_argument(std::string(who) + ": head_dim " + std::to_string(p.head_dim) + " is not a multiple of 8 up to 256");
+    if (p.fmt != QUANT_FP8 && p.fmt != QUANT_INT8) throw std::invalid_argument(std::string(who) + ": unknown format " + std::to_string(p.fmt));
+    if (((uintptr_t)p.k_codes | (uintptr_t)p.v_codes) & 7) throw std::invalid_argument(std::string(who) + ": pools must be 8-byte aligned");
 }
 
 }  // namespace
 
-void kv_quant_store(const void* k_packed, const void* v_packed, DType dt, int T, int kv_heads, int head_dim, void* k_rows,
-                    void* v_rows, int fmt, void* k_pool, void* v_pool, void* k_scale, void* v_scale, long long pool_pages,
-                    const int32_t* positions, const int32_t* page_table, int slots, int table_stride, const int32_t* token_slot, cudaStream_t stream) {
+void kv_quant_store(const QuantPools& p, const void* k_packed, const void* v_packed, DType dt, int T, void* k_rows, void* v_rows,
+                    const int32_t* positions, const int32_t* token_slot, cudaStream_t stream) {
     if (T <= 0) return;
-    check_sizes("kv_quant_store", kv_heads, head_dim, fmt);
-    if (((uintptr_t)k_packed | (uintptr_t)v_packed | (uintptr_t)k_rows | (uintptr_t)v_rows) & 15 || ((uintptr_t)k_pool | (uintptr_t)v_pool) & 7)
-        throw std::invalid_argument("kv_quant_store: rows must be 16-byte aligned and pools 8-byte aligned");
+    check_pools("kv_quant_store", p);
+    if (((uintptr_t)k_packed | (uintptr_t)v_packed | (uintptr_t)k_rows | (uintptr_t)v_rows) & 15)
+        throw std::invalid_argument("kv_quant_store: rows must be 16-byte aligned");
+    if ((long long)T * p.kv_heads > 0x7fffffffll) throw std::invalid_argument("kv_quant_store: more than 2^31 rows in one call");
     int lanes = 1;
-    while (lanes * 8 < head_dim) lanes *= 2;
-    StoreArgs a{{k_packed, v_packed}, {k_rows, v_rows}, {(uint8_t*)k_pool, (uint8_t*)v_pool}, {(uint8_t*)k_scale, (uint8_t*)v_scale},
-                positions, token_slot, {page_table, slots, table_stride, pool_pages}, kv_heads, head_dim, (long long)T * kv_heads, error_word()};
-    const long long per_block = kThreads / lanes * kStoreRows;
-    const dim3 grid((unsigned)((a.rows_of_each + per_block - 1) / per_block), 2);
+    while (lanes * 8 < p.head_dim) lanes *= 2;
+    StoreArgs a{{k_packed, v_packed}, {k_rows, v_rows}, {(uint8_t*)p.k_codes, (uint8_t*)p.v_codes}, {(uint8_t*)p.k_scale, (uint8_t*)p.v_scale},
+                positions, token_slot, {p.page_table, p.slots, p.table_stride, p.pages}, p.kv_heads, p.head_dim, (unsigned)(T * p.kv_heads), error_word()};
+    const unsigned per_block = kThreads / lanes * kStoreRows;
+    const dim3 grid((a.rows_of_each + per_block - 1) / per_block, 2);
     note_launch();
-    auto kernel = dt == F32 ? (fmt == QUANT_FP8 ? kv_quant_store_kernel<float, QUANT_FP8> : kv_quant_store_kernel<float, QUANT_INT8>)
-                            : (fmt == QUANT_FP8 ? kv_quant_store_kernel<__nv_bfloat16, QUANT_FP8> : kv_quant_store_kernel<__nv_bfloat16, QUANT_INT8>);
+    auto kernel = dt == F32 ? (p.fmt == QUANT_FP8 ? kv_quant_store_kernel<float, QUANT_FP8> : kv_quant_store_kernel<float, QUANT_INT8>)
+                            : (p.fmt == QUANT_FP8 ? kv_quant_store_kernel<__nv_bfloat16, QUANT_FP8> : kv_quant_store_kernel<__nv_bfloat16, QUANT_INT8>);
     launch_kernel("kv_quant_store", kernel, grid, dim3(kThreads), 0, stream, 1, dependent_launch_enabled(), a, lanes);
 }
 
-void kv_quant_load(int fmt, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
-                   long long pool_pages, DType dt, int n_seqs, int kv_heads, int head_dim, const int32_t* slot_ids, const int32_t* seq_ends,
-                   const int32_t* page_table, int slots, int table_stride, void* k_out, void* v_out, int32_t* out_table, int pages, bool whole,
-                   const int32_t* cu_seqlens, int skip_new, bool attend, int window, cudaStream_t stream) {
+void kv_quant_load(const QuantPools& p, DType dt, int n_seqs, const int32_t* slot_ids, const int32_t* seq_ends, void* k_out, void* v_out,
+                   int32_t* out_table, int pages, bool whole, const int32_t* cu_seqlens, int skip_new, bool attend, int window,
+                   cudaStream_t stream) {
     if (n_seqs <= 0 || pages <= 0) return;
-    check_sizes("kv_quant_load", kv_heads, head_dim, fmt);
+    check_pools("kv_quant_load", p);
     if (n_seqs > 65535) throw std::invalid_argument("kv_quant_load: more than 65535 sequences");
-    if (((uintptr_t)k_out | (uintptr_t)v_out) & 15 || ((uintptr_t)k_pool | (uintptr_t)v_pool) & 7)
-        throw std::invalid_argument("kv_quant_load: outputs must be 16-byte aligned and pools 8-byte aligned");
-    LoadArgs a{{(const uint8_t*)k_pool, (const uint8_t*)v_pool}, {(const uint8_t*)k_scale, (const uint8_t*)v_scale}, {k_out, v_out}, out_table,
-               slot_ids, seq_ends, {page_table, slots, table_stride, pool_pages}, kv_heads, head_dim, pages, whole ? 1 : 0, cu_seqlens, skip_new, attend ? 1 : 0, attend ? window : 0, error_word()};
+    if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) throw std::invalid_argument("kv_quant_load: outputs must be 16-byte aligned");
+    LoadArgs a{{(const uint8_t*)p.k_codes, (const uint8_t*)p.v_codes}, {(const uint8_t*)p.k_scale, (const uint8_t*)p.v_scale}, {k_out, v_out}, out_table,
+               slot_ids, seq_ends, {p.page_table, p.slots, p.table_stride, p.pages}, p.kv_heads, p.head_dim, pages, whole ? 1 : 0, cu_seqlens, skip_new,
+               attend ? 1 : 0, attend ? window : 0, error_word()};
     note_launch();
-    auto kernel = dt == F32 ? (fmt == QUANT_FP8 ? kv_quant_load_kernel<float, QUANT_FP8> : kv_quant_load_kernel<float, QUANT_INT8>)
-                            : (fmt == QUANT_FP8 ? kv_quant_load_kernel<__nv_bfloat16, QUANT_FP8> : kv_quant_load_kernel<__nv_bfloat16, QUANT_INT8>);
+    auto kernel = dt == F32 ? (p.fmt == QUANT_FP8 ? kv_quant_load_kernel<float, QUANT_FP8> : kv_quant_load_kernel<float, QUANT_INT8>)
+                            : (p.fmt == QUANT_FP8 ? kv_quant_load_kernel<__nv_bfloat16, QUANT_FP8> : kv_quant_load_kernel<__nv_bfloat16, QUANT_INT8>);
     launch_kernel("kv_quant_load", kernel, dim3((unsigned)pages, (unsigned)n_seqs, 2), dim3(kThreads), 0, stream, 1, dependent_launch_enabled(), a);
 }
 

@@ -3,7 +3,6 @@ the C function on the current stream. Nothing here computes; there is no fallbac
 from __future__ import annotations
 
 import ctypes
-import dataclasses
 from typing import Optional
 
 import torch
@@ -65,6 +64,10 @@ def _stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
+def _raw_stream() -> int:
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
 class NormedRows:
     """The rows of a float residual under RMSNorm, not computed yet. A product over a handful
     of tokens takes the norm as its prologue; everything else asks for ``tensor()``, which
@@ -92,6 +95,53 @@ class FusedLayerRecord(ctypes.Structure):
                                                      "k_pool", "v_pool", "page_table", "cos_table", "sin_table")] + \
                [("table_stride", ctypes.c_int), ("ring", ctypes.c_int), ("window", ctypes.c_int),
                 ("eps1", ctypes.c_float), ("eps2", ctypes.c_float), ("pad_", ctypes.c_int)]
+
+
+class QuantPools(ctypes.Structure):
+    """One layer's 8-bit cache, as the kernel library lays it out (``sm::QuantPools``)."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("k_codes", "v_codes", "k_scale", "v_scale", "page_table")] + \
+               [("pages", ctypes.c_longlong)] + [(name, ctypes.c_int) for name in ("fmt", "kv_heads", "head_dim", "slots", "table_stride")]
+
+
+class QuantLayer:
+    """The pools of an 8-bit layer cache, checked once, with the record that the kernels take."""
+
+    __slots__ = ("tensors", "record", "address", "pages", "kv_heads", "head_dim", "slots", "table_stride", "device")
+
+    def __init__(self, cache):
+        k, v, ks, vs, table = cache.k_pool, cache.v_pool, cache.k_scale, cache.v_scale, cache.page_table
+        if cache.kind != "kv" or ks is None or vs is None:
+            raise KernelError("an 8-bit key/value cache is needed (kv_dtype fp8 or int8)")
+        fmt = QUANT_FORMATS.get(k.dtype)
+        if fmt is None or v.dtype != k.dtype:
+            raise KernelError(f"pools of an 8-bit cache are float8_e4m3fn or int8, got {k.dtype} and {v.dtype}")
+        if ks.dtype != torch.uint8 or vs.dtype != torch.uint8:
+            raise KernelError("exponents of an 8-bit cache are uint8")
+        shape = k.shape
+        if len(shape) != 4 or shape[2] != PAGE_SIZE or v.shape != shape or ks.shape != shape[:3] or vs.shape != shape[:3]:
+            raise KernelError(f"pools of an 8-bit cache are [pages, kv heads, {PAGE_SIZE}, head size] with exponents of the first three, "
+                              f"got {tuple(shape)}, {tuple(v.shape)}, {tuple(ks.shape)}, {tuple(vs.shape)}")
+        if cache.ring:
+            raise KernelError("an 8-bit cache keeps every position: it has no ring")
+        if table.dtype != torch.int32 or table.dim() != 2:
+            raise KernelError("the page table must be int32 [slots, pages]")
+        if not all(t.is_contiguous() for t in (k, v, ks, vs, table)):
+            raise KernelError("the pools, exponents and page table of an 8-bit cache must be contiguous")
+        self.device = k.get_device()
+        if any(t.get_device() != self.device for t in (v, ks, vs, table)):
+            raise KernelError("the pools, exponents and page table of an 8-bit cache must lie on one device")
+        self.pages, self.kv_heads, _, self.head_dim = shape
+        self.slots, self.table_stride = table.shape
+        self.record = QuantPools(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(), self.pages, fmt, self.kv_heads,
+                                 self.head_dim, self.slots, self.table_stride)
+        self.address = ctypes.addressof(self.record)
+        self.tensors = (k, v, ks, vs, table)
+
+    def made_of(self, cache) -> bool:
+        k, v, ks, vs, table = self.tensors
+        return (cache.k_pool is k and cache.v_pool is v and cache.k_scale is ks and cache.v_scale is vs and cache.page_table is table
+                and not cache.ring and cache.kind == "kv")
 
 
 class PhaseTimes:
@@ -132,19 +182,19 @@ class Ops:
                               f"the host by {PAGE_SIZE}")
         self.lib.sm_gemm_tc_workspace_bytes.restype = ctypes.c_longlong
         self.lib.sm_launch_count.restype = ctypes.c_longlong
+        if ctypes.sizeof(QuantPools) != int(self.lib.sm_quant_pools_bytes()):
+            raise KernelError("the record of an 8-bit cache's pools is laid out differently in the library")
         # (with the argument types known, a call takes plain numbers as addresses)
-        addr, num = ctypes.c_void_p, ctypes.c_int
-        big = ctypes.c_longlong
-        self.lib.sm_kv_quant_store.argtypes = [addr, addr] + [num] * 4 + [addr, addr, num] + [addr] * 4 + [big, addr, addr, num, num, addr, addr]
-        self.lib.sm_kv_quant_load.argtypes = [num] + [addr] * 4 + [big] + [num] * 4 + [addr] * 3 + [num, num] + [addr] * 3 + [num, num, addr, num, num, num, addr]
-        self.lib.sm_attention_quant.argtypes = [addr, addr] + [num] * 4 + [ctypes.c_float, num, num] + [addr] * 4 + [big, addr, num, num] + \
-            [addr] * 3 + [num] * 5 + [addr, big, addr]
+        addr, num, big, real = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+        self.lib.sm_kv_quant_store.argtypes = [addr] * 3 + [num] * 2 + [addr] * 5
+        self.lib.sm_kv_quant_load.argtypes = [addr, num, num] + [addr] * 5 + [num, num, addr, num, num, num, addr]
+        self.lib.sm_attention_quant.argtypes = [addr] * 3 + [num, num, real, num] + [addr] * 3 + [num] * 5 + [addr, big, addr]
         self.lib.sm_attention_quant_supports.argtypes = [num, num, num, big]
-        self.lib.sm_attention_quant_workspace.argtypes, self.lib.sm_attention_quant_workspace.restype = [num, num, num, num], big
+        self.lib.sm_attention_quant_workspace.argtypes, self.lib.sm_attention_quant_workspace.restype = [num] * 4, big
         self.lib.sm_attention_chunk_supports.argtypes = [num, num, num, big, num, num]
-        self.lib.sm_attention_chunk_workspace.argtypes, self.lib.sm_attention_chunk_workspace.restype = [num, num, num], big
-        self.lib.sm_attention_chunk.argtypes = [addr, addr] + [num] * 5 + [ctypes.c_float, num, addr, addr, num, addr, addr, num, num, addr, big, addr]
-        self._quant_workspaces: dict = {}
+        self.lib.sm_attention_chunk_workspace.argtypes, self.lib.sm_attention_chunk_workspace.restype = [num] * 3, big
+        self.lib.sm_attention_chunk.argtypes = [addr, addr] + [num] * 5 + [real, num, addr, addr, num, addr, addr, num, num, addr, big, addr]
+        self._quant_plans: dict = {}      # by sizes alone
         fast = kernels == "fast"
         self.kernels = kernels
         self.phase_times: Optional[PhaseTimes] = None   # set to time the phases of the forward pass
@@ -613,47 +663,29 @@ class Ops:
                                          _ptr(step.token_slot), _ptr(step.token_end), _stream()))
 
     # ---- an 8-bit cache ------------------------------------------------------------------
-    def _quant_cache(self, cache) -> tuple:
-        """Checks an 8-bit layer cache; returns (format, pages, kv heads, head size)."""
-        k, v, ks, vs = cache.k_pool, cache.v_pool, cache.k_scale, cache.v_scale
-        if cache.kind != "kv" or ks is None or vs is None:
-            raise KernelError("an 8-bit key/value cache is needed (kv_dtype fp8 or int8)")
-        fmt = QUANT_FORMATS.get(k.dtype)
-        if fmt is None or v.dtype != k.dtype:
-            raise KernelError(f"pools of an 8-bit cache are float8_e4m3fn or int8, got {k.dtype} and {v.dtype}")
-        if ks.dtype != torch.uint8 or vs.dtype != torch.uint8:
-            raise KernelError("exponents of an 8-bit cache are uint8")
-        shape = k.shape
-        if len(shape) != 4 or shape[2] != PAGE_SIZE or v.shape != shape or ks.shape != shape[:3] or vs.shape != shape[:3]:
-            raise KernelError(f"pools of an 8-bit cache are [pages, kv heads, {PAGE_SIZE}, head size] with exponents of the first three, "
-                              f"got {tuple(shape)}, {tuple(v.shape)}, {tuple(ks.shape)}, {tuple(vs.shape)}")
-        if cache.ring:
-            raise KernelError("an 8-bit cache keeps every position: it has no ring")
-        table = cache.page_table
-        if table.dtype != torch.int32 or table.dim() != 2:
-            raise KernelError("the page table must be int32 [slots, pages]")
-        if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and table.is_contiguous()):
-            raise KernelError("the pools, exponents and page table of an 8-bit cache must be contiguous")
-        _here(k, v, ks, vs, table)
-        return fmt, shape[0], shape[1], shape[3]
+    def _quant_cache(self, cache) -> "QuantLayer":
+        """An 8-bit layer cache, checked."""
+        layer = cache.quant_layer()
+        if layer.device != torch._C._cuda_getDevice():
+            raise KernelError(f"the cache lies on {cache.k_pool.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+        return layer
 
     def kv_quant_store(self, k_packed, v_packed, step, cache, want_rows: bool = False):
         """This step's packed keys and values [T, kv heads, head size] into an 8-bit cache, one power-of-two scale a row.
         With ``want_rows`` returns (k, v) as the cache now stands for them, laid out like the packed tensors. A row that
         holds an infinity or a NaN reads back as NaN whole."""
-        fmt, pool_pages, kv_heads, head_dim = self._quant_cache(cache)
-        _need(k_packed, "packed keys", ndim=3)
-        _need(v_packed, "packed values", k_packed.dtype, 3)
-        if tuple(k_packed.shape) != (step.n_tokens, kv_heads, head_dim) or v_packed.shape != k_packed.shape:
-            raise KernelError(f"packed keys and values are {tuple(k_packed.shape)} and {tuple(v_packed.shape)}, expected "
-                              f"{(step.n_tokens, kv_heads, head_dim)}")
-        _here(k_packed, v_packed, step.positions)
+        layer = self._quant_cache(cache)
+        positions, token_slot = step.positions, step.token_slot
+        if k_packed.shape != (step.n_tokens, layer.kv_heads, layer.head_dim) or v_packed.shape != k_packed.shape or v_packed.dtype != k_packed.dtype:
+            raise KernelError(f"packed keys are {tuple(k_packed.shape)} {k_packed.dtype} and packed values {tuple(v_packed.shape)} {v_packed.dtype}, "
+                              f"expected {(step.n_tokens, layer.kv_heads, layer.head_dim)} of one type")
+        if not (k_packed.is_contiguous() and v_packed.is_contiguous()):
+            raise KernelError("packed keys and values must be contiguous")
+        _here(k_packed, v_packed, positions, token_slot)
         rows = (torch.empty_like(k_packed), torch.empty_like(v_packed)) if want_rows else None
         self._check(self.lib.sm_kv_quant_store(
-            k_packed.data_ptr(), v_packed.data_ptr(), _dt(k_packed), step.n_tokens, kv_heads, head_dim,
-            rows[0].data_ptr() if rows else None, rows[1].data_ptr() if rows else None, fmt, cache.k_pool.data_ptr(),
-            cache.v_pool.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pool_pages,
-            step.positions.data_ptr(), cache.page_table.data_ptr(), cache.page_table.shape[0], cache.page_table.shape[1], step.token_slot.data_ptr(), _stream()))
+            layer.address, k_packed.data_ptr(), v_packed.data_ptr(), _dt(k_packed), step.n_tokens, rows[0].data_ptr() if rows else None,
+            rows[1].data_ptr() if rows else None, positions.data_ptr(), token_slot.data_ptr(), _raw_stream()))
         return rows
 
     def kv_quant_load(self, step, cache, dtype: torch.dtype):
@@ -661,89 +693,106 @@ class Ops:
         ``dtype`` whose page table has the same slots. Sequence ``i`` of the step has its pages from ``i * P`` on, ``P``
         the pages of ``step.max_seq_len`` positions (at most the page table's width); positions past its end read as
         zeros."""
-        if dtype not in (torch.float32, torch.bfloat16):
+        if dtype is not torch.float32 and dtype is not torch.bfloat16:
             raise KernelError(f"an 8-bit cache is read back as float32 or bfloat16, not {dtype}")
-        return self._quant_load(step, cache, dtype, True, 0, False, 0)
+        k, v, table = self._quant_load(step, self._quant_cache(cache), cache, dtype, True, 0, False, 0)
+        return type(cache)("kv", k, v, table, 0, cache.window)
 
-    def _quant_load(self, step, cache, dtype, whole, skip_new, attend, window):
-        """``whole``: pages past a sequence's end are zeroed too; the others: see kv_quant_load in csrc/kernels.h."""
-        fmt, pool_pages, kv_heads, head_dim = self._quant_cache(cache)
+    def _quant_load(self, step, layer, cache, dtype, whole, skip_new, attend, window):
+        """Values of keys, of values, and their page table. ``whole``: pages past a sequence's end are zeroed too; the
+        others: see kv_quant_load in csrc/kernels.h."""
         # (a captured step's longest sequence is a bound that may pass what the page table can hold)
-        pages = min((step.max_seq_len + PAGE_SIZE - 1) // PAGE_SIZE, cache.page_table.shape[1])
-        _here(step.slot_ids, step.seq_ends, step.cu_seqlens)
-        device = cache.k_pool.device
-        k = torch.empty((step.n_seqs * pages, kv_heads, PAGE_SIZE, head_dim), dtype=dtype, device=device)
+        pages = min((step.max_seq_len + PAGE_SIZE - 1) // PAGE_SIZE, layer.table_stride)
+        slot_ids, seq_ends, cu = step.slot_ids, step.seq_ends, step.cu_seqlens
+        _here(slot_ids, seq_ends, cu)
+        k = cache.k_pool.new_empty((step.n_seqs * pages, layer.kv_heads, PAGE_SIZE, layer.head_dim), dtype=dtype)
         v = torch.empty_like(k)
-        table = torch.empty((cache.page_table.shape[0], pages), dtype=torch.int32, device=device)
+        table = cache.page_table.new_empty((layer.slots, pages))
         self._check(self.lib.sm_kv_quant_load(
-            fmt, cache.k_pool.data_ptr(), cache.v_pool.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pool_pages,
-            _dt(k), step.n_seqs, kv_heads, head_dim, step.slot_ids.data_ptr(), step.seq_ends.data_ptr(), cache.page_table.data_ptr(),
-            cache.page_table.shape[0], cache.page_table.shape[1], k.data_ptr(), v.data_ptr(), table.data_ptr(), pages, int(whole),
-            step.cu_seqlens.data_ptr(), skip_new, int(attend), window, _stream()))
-        return dataclasses.replace(cache, k_pool=k, v_pool=v, page_table=table, k_scale=None, v_scale=None)
+            layer.address, F32 if dtype is torch.float32 else BF16, step.n_seqs, slot_ids.data_ptr(), seq_ends.data_ptr(), k.data_ptr(),
+            v.data_ptr(), table.data_ptr(), pages, whole, cu.data_ptr(), skip_new, attend, window, _raw_stream()))
+        return k, v, table
 
     def attention_quant(self, q, step, scale, window, cache):
         """Causal attention of this step's tokens (one or any number per sequence) over an 8-bit cache, which holds their own
         keys and values already (``kv_quant_store``). ``window``: each sees that many positions up to its own (None or
         0: all)."""
-        fmt, pool_pages, kv_heads, head_dim = self._quant_cache(cache)
-        _need(q, "q", ndim=3)
-        if q.shape[0] != step.n_tokens or q.shape[2] != head_dim or q.shape[1] == 0 or q.shape[1] % kv_heads:
-            raise KernelError(f"q is {tuple(q.shape)}: expected {step.n_tokens} tokens, a multiple of {kv_heads} heads, head size {head_dim}")
-        if window and window < 0:
+        layer = self._quant_cache(cache)
+        kv_heads, head_dim, dtype, shape = layer.kv_heads, layer.head_dim, q.dtype, q.shape
+        if dtype is not torch.bfloat16 and dtype is not torch.float32:
+            raise KernelError(f"unsupported dtype {dtype}: kernels take float32 and bfloat16")
+        if len(shape) != 3 or shape[0] != step.n_tokens or shape[2] != head_dim or shape[1] == 0 or shape[1] % kv_heads:
+            raise KernelError(f"q is {tuple(shape)}: expected {step.n_tokens} tokens, a multiple of {kv_heads} heads, head size {head_dim}")
+        if not q.is_contiguous():
+            raise KernelError("q must be contiguous")
+        window = int(window or 0)
+        if window < 0:
             raise KernelError(f"a window of {window} positions")
-        _here(q, step.positions)
-        heads = q.shape[1]
-        if not self.use_fast_attention or q.dtype != torch.bfloat16 or not self.lib.sm_attention_quant_supports(heads, kv_heads, head_dim, pool_pages):
+        slot_ids, seq_ends, cu = step.slot_ids, step.seq_ends, step.cu_seqlens
+        _here(q, slot_ids, seq_ends, cu)
+        heads, n_seqs = shape[1], step.n_seqs
+        plan = self._quant_plan(step.seq_lens, step.max_seq_len, heads, layer, dtype, window)
+        if plan is None:
             # the plain kernel over pages that have been read back: float queries, other head sizes
-            pages = self._quant_load(step, cache, q.dtype, False, 0, False, 0)
-            return self.attention_plain(q, step.positions, scale, window, k_pool=pages.k_pool, v_pool=pages.v_pool,
-                                        page_table=pages.page_table, token_slot=step.token_slot, kv_heads=kv_heads)
+            k, v, table = self._quant_load(step, layer, cache, dtype, False, 0, False, 0)
+            return self.attention_plain(q, step.positions, scale, window, k_pool=k, v_pool=v, page_table=table, token_slot=step.token_slot,
+                                        kv_heads=kv_heads)
+        limit, row_tiles, pairs, cluster, longest, floats, blocks, chunk_floats = plan
         out = torch.empty_like(q)
-        lens = step.seq_lens
-        most = limit = max(lens)
-        group = heads // kv_heads
-        blocks = 0
-        if most > self.quant_rows_tokens and self.use_tcgen05_attention:
-            many = 2 * (128 // group)     # tokens of a block of the tcgen05 kernel
-            blocks = sum(-(-n // many) for n in lens if n > self.quant_rows_tokens)
-            if self.lib.sm_attention_chunk_supports(heads, kv_heads, head_dim, step.n_seqs * cache.page_table.shape[1], step.n_seqs, blocks):
-                limit = self.quant_rows_tokens
-                few = [n for n in lens if n <= limit]
-                most = max(few) if few else 0
-            else:
-                blocks = 0
-        if most:
+        if pairs:
             # single tokens, and sequences that bring a few: straight from the codes
-            row_tiles = 1
-            while 8 * row_tiles < min(most * group, 32 if head_dim <= 64 else 16) or 8 * row_tiles < group:
-                row_tiles *= 2
-            tokens = 8 * row_tiles // group
-            pairs = kv_heads * (step.n_seqs if most == 1 and limit == most else sum(-(-n // tokens) for n in lens if n <= limit))
-            longest = step.max_seq_len if not window else min(step.max_seq_len, window + most)
-            cluster, floats = self._quant_cluster(pairs, longest, head_dim), 0
-            if not cluster:
-                key = (head_dim <= 64, row_tiles, pairs)
-                floats = self._quant_workspaces.get(key)
-                if floats is None:
-                    floats = self._quant_workspaces[key] = int(self.lib.sm_attention_quant_workspace(head_dim, row_tiles, pairs, 0))
-            workspace = torch.empty((floats,), dtype=torch.float32, device=q.device) if floats else None
+            workspace = q.new_empty((floats,), dtype=torch.float32) if floats else None
             self._check(self.lib.sm_attention_quant(
-                q.data_ptr(), out.data_ptr(), step.n_seqs, heads, kv_heads, head_dim, scale, int(window or 0), fmt, cache.k_pool.data_ptr(),
-                cache.v_pool.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pool_pages, cache.page_table.data_ptr(),
-                cache.page_table.shape[0], cache.page_table.shape[1], step.slot_ids.data_ptr(), step.seq_ends.data_ptr(),
-                step.cu_seqlens.data_ptr(), longest, limit, row_tiles, pairs, cluster, workspace.data_ptr() if floats else None, floats,
-                _stream()))
+                layer.address, q.data_ptr(), out.data_ptr(), n_seqs, heads, scale, window, slot_ids.data_ptr(), seq_ends.data_ptr(), cu.data_ptr(),
+                longest, limit, row_tiles, pairs, cluster, workspace.data_ptr() if floats else None, floats, _raw_stream()))
         if blocks:
             # many tokens: the pages are read back as bfloat16 once (exactly), and the tcgen05 kernel reads those
-            pages = self._quant_load(step, cache, q.dtype, False, limit, True, int(window or 0))
-            floats = int(self.lib.sm_attention_chunk_workspace(head_dim, kv_heads, blocks))
-            workspace = torch.empty((floats,), dtype=torch.float32, device=q.device)
+            k, v, table = self._quant_load(step, layer, cache, dtype, False, limit, True, window)
+            workspace = q.new_empty((chunk_floats,), dtype=torch.float32)
             self._check(self.lib.sm_attention_chunk(
-                q.data_ptr(), out.data_ptr(), step.n_tokens, step.n_seqs, heads, kv_heads, head_dim, scale, int(window or 0),
-                pages.k_pool.data_ptr(), pages.v_pool.data_ptr(), pages.page_table.shape[1], step.seq_ends.data_ptr(), step.cu_seqlens.data_ptr(),
-                limit, blocks, workspace.data_ptr(), floats, _stream()))
+                q.data_ptr(), out.data_ptr(), step.n_tokens, n_seqs, heads, kv_heads, head_dim, scale, window, k.data_ptr(), v.data_ptr(),
+                table.shape[1], seq_ends.data_ptr(), cu.data_ptr(), limit, blocks, workspace.data_ptr(), chunk_floats, _raw_stream()))
         return out
+
+    def _quant_plan(self, lens, max_len, heads, layer, dtype, window):
+        """Which kernels attend over an 8-bit cache, and how they share the work out, by sizes alone: None for the plain
+        one, else (the most new tokens of a sequence that attends straight from the codes, tiles of 8 rows of queries there,
+        pairs, CTAs of a cluster, the longest span, floats of workspace; blocks of the tcgen05 kernel for the others, floats)."""
+        switches = (self.use_fast_attention, self.use_tcgen05_attention, self.quant_rows_tokens, self.quant_cluster)
+        key = (tuple(lens), max_len, heads, layer.kv_heads, layer.head_dim, layer.pages, layer.table_stride, dtype, window, switches)
+        if key in self._quant_plans:
+            return self._quant_plans[key]
+        plan = self._make_quant_plan(lens, max_len, heads, layer, dtype, window)
+        if len(self._quant_plans) >= 256:
+            self._quant_plans.clear()
+        self._quant_plans[key] = plan
+        return plan
+
+    def _make_quant_plan(self, lens, max_len, heads, layer, dtype, window):
+        kv_heads, head_dim = layer.kv_heads, layer.head_dim
+        if not self.use_fast_attention or dtype != torch.bfloat16 or not self.lib.sm_attention_quant_supports(heads, kv_heads, head_dim, layer.pages):
+            return None
+        group, limit, blocks, chunk_floats = heads // kv_heads, max(lens), 0, 0
+        if limit > self.quant_rows_tokens and self.use_tcgen05_attention:
+            many = 2 * (128 // group)     # tokens of a block of the tcgen05 kernel
+            blocks = sum(-(-n // many) for n in lens if n > self.quant_rows_tokens)
+            if self.lib.sm_attention_chunk_supports(heads, kv_heads, head_dim, len(lens) * layer.table_stride, len(lens), blocks):
+                limit = self.quant_rows_tokens
+                chunk_floats = int(self.lib.sm_attention_chunk_workspace(head_dim, kv_heads, blocks))
+            else:
+                blocks = 0
+        few = [n for n in lens if n <= limit]
+        if not few:
+            return limit, 1, 0, 0, 0, 0, blocks, chunk_floats
+        row_tiles = 1
+        while 8 * row_tiles < min(max(few) * group, 32 if head_dim <= 64 else 16) or 8 * row_tiles < group:
+            row_tiles *= 2
+        tokens = 8 * row_tiles // group
+        pairs = kv_heads * sum(-(-n // tokens) for n in few)
+        longest = max_len if not window else min(max_len, window + max(few))
+        cluster = self._quant_cluster(pairs, longest, head_dim)
+        floats = 0 if cluster else int(self.lib.sm_attention_quant_workspace(head_dim, row_tiles, pairs, 0))
+        return limit, row_tiles, pairs, cluster, longest, floats, blocks, chunk_floats
 
     def _quant_cluster(self, pairs: int, longest: int, head_dim: int) -> int:
         """CTAs that share a pair (a block of rows of queries and its kv head), or 0 for the line (csrc/attention_quant.cu)."""
