@@ -637,8 +637,8 @@ void attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int
     ChunkCut* cuts = (ChunkCut*)workspace;
     ChunkArgs a{(__nv_bfloat16*)out, seq_ends, cu_seqlens, n_seqs, heads, kv_heads, window, skip_new, pages, tile_tokens, blocks, scale * 1.4426950408889634f, cuts,
                 workspace + (long long)blocks * kv_heads * (long long)(sizeof(ChunkCut) / sizeof(float)), error_word()};
-    // a run is at least this many tiles: a part costs about as much as two to leave and join
-    const int least_run = 4;
+    // a run is at least this many tiles: a part costs about as much as one to leave and join
+    const int least_run = 2;
     if (head_dim == 64) launch<64>(mq, mk, mv, a, blocks, least_run, stream);
     else launch<128>(mq, mk, mv, a, blocks, least_run, stream);
 }

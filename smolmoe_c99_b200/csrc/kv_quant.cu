@@ -59,7 +59,7 @@ struct StoreArgs {
 
 // One row per group of `lanes` threads (a power of two, at least head_dim / 8); blockIdx.y: keys or values. A thread does
 // kStoreRows rows, so that as many loads are under way together.
-constexpr int kStoreRows = 4;
+constexpr int kStoreRows = 2;
 
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kThreads) kv_quant_store_kernel(StoreArgs a, int lanes) {

@@ -219,9 +219,9 @@ class Ops:
         # 8,000 6.85 against 4.43
         self.extend_rows_as_decode_tc = 176 if fast else 0
         self.extend_tc_variant = -1     # that kernel with one CTA an SM (0), two (1, head size 64), or as the launcher chooses
-        self.quant_rows_tokens = 64     # over an 8-bit cache: sequences that bring more tokens go to the tcgen05 kernel
-        self.quant_cluster: Optional[int] = None     # (a fixed choice, for comparisons)
-        self.quant_line_tiles = 8192
+        # attention over an 8-bit cache: fixed choices in place of the rules, for comparisons (see _make_quant_plan)
+        self.quant_rows_tokens: Optional[int] = None
+        self.quant_cluster: Optional[int] = None
         self.skinny_single_round_above_8 = True
         self.error_flag = torch.zeros(1, dtype=torch.int32, device="cuda")
         self.lib.sm_set_error_word.restype = None
@@ -773,11 +773,18 @@ class Ops:
         if not self.use_fast_attention or dtype != torch.bfloat16 or not self.lib.sm_attention_quant_supports(heads, kv_heads, head_dim, layer.pages):
             return None
         group, limit, blocks, chunk_floats = heads // kv_heads, max(lens), 0, 0
-        if limit > self.quant_rows_tokens and self.use_tcgen05_attention:
+        # Sequences that bring up to this many tokens attend straight from the codes, the others through pages read back and
+        # the tcgen05 kernel. Measured on a B200, us a call, codes against pages: 14 heads on 2 of 64, 32 tokens onto 8,000
+        # 29 / 36, 64 onto 8,000 22 / 36, 64 onto 32,000 62 / 60; 28 heads on 4 of 128, 32 onto 8,000 33 / 45, 64 onto 8,000
+        # 52 / 48, 32 onto 32,000 89 / 85, 64 onto 32,000 165 / 90.
+        few_tokens = self.quant_rows_tokens
+        if few_tokens is None:
+            few_tokens = max(1, (448 if head_dim <= 64 else 256) // group)
+        if limit > few_tokens and self.use_tcgen05_attention:
             many = 2 * (128 // group)     # tokens of a block of the tcgen05 kernel
-            blocks = sum(-(-n // many) for n in lens if n > self.quant_rows_tokens)
+            blocks = sum(-(-n // many) for n in lens if n > few_tokens)
             if self.lib.sm_attention_chunk_supports(heads, kv_heads, head_dim, len(lens) * layer.table_stride, len(lens), blocks):
-                limit = self.quant_rows_tokens
+                limit = few_tokens
                 chunk_floats = int(self.lib.sm_attention_chunk_workspace(head_dim, kv_heads, blocks))
             else:
                 blocks = 0
@@ -795,14 +802,18 @@ class Ops:
         return limit, row_tiles, pairs, cluster, longest, floats, blocks, chunk_floats
 
     def _quant_cluster(self, pairs: int, longest: int, head_dim: int) -> int:
-        """CTAs that share a pair (a block of rows of queries and its kv head), or 0 for the line (csrc/attention_quant.cu)."""
+        """CTAs that share a pair (a block of rows of queries and its kv head), or 0 for the line (csrc/attention_quant.cu).
+        The line costs ~3 us more (the join) and wins when there are more tiles of 32 positions than clusters that fill the
+        GPU once work off quickly, or when sequences are of unequal lengths: 8 x 8,192 positions on 4 kv heads (8,192 tiles)
+        18 us either way, 64 sequences of 200 to 4,000 (32,000 tiles) 57 us in clusters of one CTA and 39 on the line."""
         if self.quant_cluster is not None:
             return self.quant_cluster
         tiles = -(-longest // 32)
-        if pairs * tiles > self.quant_line_tiles:
+        if pairs * tiles > 8192:
             return 0
         cluster = 1
-        while cluster < 8 and 2 * cluster * pairs <= 148 and tiles > 8 * cluster:
+        # (clusters of 8 large CTAs do not pack every SM: more than 14 of them would take a second turn)
+        while cluster < 8 and 2 * cluster * pairs <= (148 if cluster < 4 else 112) and tiles > 8 * cluster:
             cluster *= 2
         return cluster
 
