@@ -189,6 +189,9 @@ __device__ __forceinline__ Part part_at(const ChunkArgs& a, const Line& line, in
     return p;
 }
 
+// A wait whose outcome is the warp's, so its lanes stay together where it runs out.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                       const __grid_constant__ CUtensorMap map_v, ChunkArgs a, int least_run) {
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             float m = -CUDART_INF_F, l = 0.f;
             for (int t = 0; t < p.n_kt; ++t) {
                 const int key0 = (p.kt0 + t) * kKeys;
-                if (!mbar_wait(&s_full[x], (uint32_t)scores & 1u)) { fail(47); ok = false; break; }
+                if (!warp_wait(&s_full[x], (uint32_t)scores & 1u)) { fail(47); ok = false; break; }
                 ++scores;
                 tc_fence_after();
                 float sv[128];
@@ -478,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 unpack_f32x2(add_f32x2(sum2[0], sum2[1]), lo2, hi2);
                 l += lo2 + hi2;
             }
-            if (ok && !mbar_wait(&o_full[x], (uint32_t)ends & 1u)) { fail(48); ok = false; }
+            if (ok && !warp_wait(&o_full[x], (uint32_t)ends & 1u)) { fail(48); ok = false; }
             ++ends;
             tc_fence_after();
             if (!__all_sync(0xffffffffu, ok && !*failed)) { ok = false; break; }
