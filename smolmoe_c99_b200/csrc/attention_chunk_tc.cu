@@ -318,84 +318,105 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             }
         }
     } else if (warp == kMmaWarp) {
-        // One thread issues all products, the tiles' strictly in turn: issued by a thread each, they mix on the tensor cores,
-        // and both tiles then turn scores into weights at the same time (333 against 270 us at 1,024 x 28 heads onto 16,000).
-        if ((threadIdx.x & 31) == 0 && u_lo < u_hi) {
+        // One warp issues all products, the tiles' strictly in turn: issued by a warp each, they mix on the tensor cores, and
+        // both tiles then turn scores into weights at the same time. Its lanes go through the run together and one of them
+        // issues: the operands of tcgen05.mma then stay in the warp's uniform registers. (With one lane going through it all by
+        // itself a product took 80 cycles to issue against 64 to run, and the row threads waited for that.)
+        auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+        const int lo = same(u_lo), hi = same(u_hi);
+        if (lo < hi) {
             const uint32_t idesc_s = instr_desc(kRows, kKeys), idesc_pv = instr_desc(kRows, HD) | (1u << 16);     // V is MN-major
             const uint64_t desc_q = smem_desc(smem_u32(q_s)), desc_k = smem_desc(smem_u32(k_s)), desc_v = smem_desc_rows(smem_u32(v_s));
+            const uint32_t tm = (uint32_t)same((int)tmem);
             auto issue_s = [&](int x, int s) {
                 const uint64_t q = desc_q + (uint64_t)(((uint32_t)x * kTileBytes) >> 4), k = desc_k + (uint64_t)(((uint32_t)s * kTileBytes) >> 4);
+                if (elect_one()) {
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) {
-                    const uint64_t off = (uint64_t)(((uint32_t)(ks / 4) * kBlockBytes + (uint32_t)(ks % 4) * 32) >> 4);
-                    umma_bf16(tmem + (uint32_t)x * 128, q + off, k + off, idesc_s, ks > 0 ? 1u : 0u);
+                    for (int ks = 0; ks < HD / 16; ++ks) {
+                        const uint64_t off = (uint64_t)(((uint32_t)(ks / 4) * kBlockBytes + (uint32_t)(ks % 4) * 32) >> 4);
+                        umma_bf16(tm + (uint32_t)x * 128, q + off, k + off, idesc_s, ks > 0 ? 1u : 0u);
+                    }
+                    umma_commit(&s_full[x]);
                 }
-                umma_commit(&s_full[x]);
+                __syncwarp();
             };
             auto issue_pv = [&](int x, int s, bool first) {
                 const uint64_t v = desc_v + (uint64_t)(((uint32_t)s * kTileBytes) >> 4);
+                if (elect_one()) {
 #pragma unroll
-                for (int ks = 0; ks < kKeys / 16; ++ks)
-                    umma_bf16_ts(tmem + kTmemO + (uint32_t)x * 128, tmem + (uint32_t)x * 128 + (uint32_t)ks * 8,
-                                 v + (uint64_t)(((uint32_t)ks * 16 * 128) >> 4), idesc_pv, first && ks == 0 ? 0u : 1u);
+                    for (int ks = 0; ks < kKeys / 16; ++ks)
+                        umma_bf16_ts(tm + kTmemO + (uint32_t)x * 128, tm + (uint32_t)x * 128 + (uint32_t)ks * 8, v + (uint64_t)(((uint32_t)ks * 16 * 128) >> 4),
+                                     idesc_pv, first && ks == 0 ? 0u : 1u);
+                }
+                __syncwarp();
+            };
+            auto commit = [&](uint64_t* bar) {
+                if (elect_one()) umma_commit(bar);
+                __syncwarp();
+            };
+            struct Steps { int n_kt, both, end; };       // of a part: tiles of keys, tiles of rows, its end on the line
+            auto steps_at = [&](int u) {
+                const Part p = part_at(a, line, blocks, u, hi);
+                return Steps{same(p.n_kt), same(p.tokens) > a.tile_tokens ? 2 : 1, same(p.end)};
             };
             // fills gone through; weights and parts of each tile of rows; parts (of queries)
             int f = 0, weights[2] = {0, 0}, ends[2] = {0, 0}, parts = 1;
-            Part p = part_at(a, line, blocks, u_lo, u_hi);
-            int both = p.tokens > a.tile_tokens ? 2 : 1;
-            bool ok = mbar_wait(q_full, 0) && mbar_wait(&k_full[0], 0), any = ok;
+            Steps p = steps_at(lo);
+            bool ok = warp_wait(q_full, 0) && warp_wait(&k_full[0], 0), any = ok;
             if (ok) {
                 tc_fence_after();
-                for (int x = 0; x < both; ++x) issue_s(x, 0);
-                umma_commit(&k_empty[0]);
-                if (p.n_kt == 1) umma_commit(q_empty);
+                issue_s(0, 0);
+                if (p.both == 2) issue_s(1, 0);
+                commit(&k_empty[0]);
+                if (p.n_kt == 1) commit(q_empty);
             } else {
                 fail(43);
             }
             while (ok) {
-                const bool last = p.end >= u_hi;             // the run's last part
-                Part after = p;
-                int both_after = 0;
-                if (!last) { after = part_at(a, line, blocks, p.end, u_hi); both_after = after.tokens > a.tile_tokens ? 2 : 1; }
+                const bool last = p.end >= hi;               // the run's last part
+                Steps after = {0, 0, 0};
+                if (!last) after = steps_at(p.end);
                 for (int t = 0; t < p.n_kt && ok; ++t, ++f) {
                     const int s = f % NS, next = (f + 1) % NS;
                     const bool more = t + 1 < p.n_kt;        // scores to follow: of this part, or of the next one's first tile
-                    const int following = more ? both : both_after;
-                    if (!(ok = mbar_wait(&v_full[s], (uint32_t)(f / NS) & 1u))) { fail(44); break; }
-                    for (int x = 0; x < 2 && ok; ++x) {
-                        if (x < both) {
-                            if (t == 0 && ends[x] > 0 && !(ok = mbar_wait(&o_empty[x], (uint32_t)(ends[x] - 1) & 1u))) { fail(50); break; }
-                            if (!(ok = mbar_wait(&p_full[x], (uint32_t)weights[x] & 1u))) { fail(46); break; }
-                            ++weights[x];
-                            tc_fence_after();
-                            issue_pv(x, s, t == 0);
-                            if (!more) { umma_commit(&o_full[x]); ++ends[x]; }
+                    const int following = more ? p.both : after.both;
+                    if (!(ok = warp_wait(&v_full[s], (uint32_t)(f / NS) & 1u))) { fail(44); break; }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        if (ok && x < p.both) {
+                            if (t == 0 && ends[x] > 0 && !(ok = warp_wait(&o_empty[x], (uint32_t)(ends[x] - 1) & 1u))) fail(50);
+                            if (ok && !(ok = warp_wait(&p_full[x], (uint32_t)weights[x] & 1u))) fail(46);
+                            if (ok) {
+                                ++weights[x];
+                                tc_fence_after();
+                                issue_pv(x, s, t == 0);
+                                if (!more) { commit(&o_full[x]); ++ends[x]; }
+                            }
                         }
-                        if (x < following) {
+                        if (ok && x < following) {
                             if (x == 0) {
-                                if (!(ok = mbar_wait(&k_full[next], (uint32_t)((f + 1) / NS) & 1u))) { fail(45); break; }
-                                if (!more && !(ok = mbar_wait(q_full, (uint32_t)parts & 1u))) { fail(51); break; }
+                                if (!(ok = warp_wait(&k_full[next], (uint32_t)((f + 1) / NS) & 1u))) fail(45);
+                                if (ok && !more && !(ok = warp_wait(q_full, (uint32_t)parts & 1u))) fail(51);
                                 tc_fence_after();
                             }
-                            issue_s(x, next);
+                            if (ok) issue_s(x, next);
                         }
                     }
                     if (!ok) break;
-                    umma_commit(&v_empty[s]);
+                    commit(&v_empty[s]);
                     if (following) {
-                        umma_commit(&k_empty[next]);
+                        commit(&k_empty[next]);
                         // the last scores of a part: its queries' memory may take the next part's
-                        if (more ? t + 2 == p.n_kt : after.n_kt == 1) umma_commit(q_empty);
+                        if (more ? t + 2 == p.n_kt : after.n_kt == 1) commit(q_empty);
                     }
                 }
                 if (last) break;
                 p = after;
-                both = both_after;
                 ++parts;
             }
-            if ((!ok || *failed) && any) {
-                umma_commit(drain_bar);
-                mbar_wait(drain_bar, 0);
+            if (__any_sync(0xffffffffu, !ok || *failed) && any) {
+                commit(drain_bar);
+                warp_wait(drain_bar, 0);
             }
         }
     } else {
