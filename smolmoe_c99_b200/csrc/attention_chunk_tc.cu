@@ -191,25 +191,30 @@ __device__ __forceinline__ Part part_at(const ChunkArgs& a, const Line& line, in
 
 // A wait whose outcome is the warp's, so its lanes stay together where it runs out.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                       const __grid_constant__ CUtensorMap map_v, ChunkArgs a, int least_run) {
     constexpr int DB = HD / 64, NS = stages_of(HD);
     constexpr int kTileBytes = DB * kBlockBytes;         // a tile of queries, of keys or of values
-    constexpr uint32_t kTmemO = 256;                     // columns: S_A 0, S_B 128, O_A 256, O_B 384
+    constexpr uint32_t kTmemP = 128, kTmemO = 256;       // columns: S 0, P_A 128, P_B 192, O_A 256, O_B 384
     extern __shared__ uint8_t smem_raw[];
     uint8_t* q_s = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);   // [2 tiles][DB][128 rows][128 B]
     uint8_t* k_s = q_s + 2 * kTileBytes;                 // [NS][DB][128 keys][128 B]
     uint8_t* v_s = k_s + NS * kTileBytes;                // [NS]
     uint64_t* bars = (uint64_t*)(v_s + NS * kTileBytes);
     uint64_t *q_full = bars, *q_empty = bars + 1;        // a part's queries have landed; its last scores are done
-    uint64_t* s_full = bars + 2;                         // [2] scores are in tensor memory (and PV of the tile before is done)
+    uint64_t* s_full = bars + 2;                         // [2 tiles] scores are in tensor memory
     uint64_t* p_full = bars + 4;                         // [2] weights are in tensor memory (and the accumulator is rescaled)
-    uint64_t* o_full = bars + 6;                         // [2] the part's last PV is done
+    uint64_t* pv_done = bars + 6;                        // [2] a PV is done: its weights' place is free, the accumulator whole
     uint64_t* o_empty = bars + 8;                        // [2] the part's accumulator has been read
-    uint64_t* drain_bar = bars + 10;
-    uint64_t *k_full = bars + 11, *k_empty = k_full + NS, *v_full = k_empty + NS, *v_empty = v_full + NS;
+    uint64_t* s_empty = bars + 10;                       // the scores have been read
+    uint64_t* drain_bar = bars + 11;
+    uint64_t *k_full = bars + 12, *k_empty = k_full + NS, *v_full = k_empty + NS, *v_empty = v_full + NS;
     uint32_t* tmem_slot = (uint32_t*)(v_empty + NS);
     volatile int* failed = (volatile int*)(tmem_slot + 1);
     Line line;
@@ -225,10 +230,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
         mbar_init(q_empty, 1);
         for (int x = 0; x < 2; ++x) {
             mbar_init(&s_full[x], 1);
-            mbar_init(&p_full[x], kRows);
-            mbar_init(&o_full[x], 1);
-            mbar_init(&o_empty[x], kRows);
+            mbar_init(&p_full[x], 4);        // (a lane of each of the tile's warps)
+            mbar_init(&pv_done[x], 1);
+            mbar_init(&o_empty[x], 4);
         }
+        mbar_init(s_empty, 4);
         mbar_init(drain_bar, 1);
         for (int i = 0; i < 4 * NS; ++i) mbar_init(&k_full[i], 1);
         *failed = 0;
@@ -334,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
 #pragma unroll
                     for (int ks = 0; ks < HD / 16; ++ks) {
                         const uint64_t off = (uint64_t)(((uint32_t)(ks / 4) * kBlockBytes + (uint32_t)(ks % 4) * 32) >> 4);
-                        umma_bf16(tm + (uint32_t)x * 128, q + off, k + off, idesc_s, ks > 0 ? 1u : 0u);
+                        umma_bf16(tm, q + off, k + off, idesc_s, ks > 0 ? 1u : 0u);
                     }
                     umma_commit(&s_full[x]);
                 }
@@ -345,8 +351,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 if (elect_one()) {
 #pragma unroll
                     for (int ks = 0; ks < kKeys / 16; ++ks)
-                        umma_bf16_ts(tm + kTmemO + (uint32_t)x * 128, tm + (uint32_t)x * 128 + (uint32_t)ks * 8, v + (uint64_t)(((uint32_t)ks * 16 * 128) >> 4),
-                                     idesc_pv, first && ks == 0 ? 0u : 1u);
+                        umma_bf16_ts(tm + kTmemO + (uint32_t)x * 128, tm + kTmemP + (uint32_t)x * 64 + (uint32_t)ks * 8,
+                                     v + (uint64_t)(((uint32_t)ks * 16 * 128) >> 4), idesc_pv, first && ks == 0 ? 0u : 1u);
+                    umma_commit(&pv_done[x]);
                 }
                 __syncwarp();
             };
@@ -359,18 +366,24 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 const Part p = part_at(a, line, blocks, u, hi);
                 return Steps{same(p.n_kt), same(p.tokens) > a.tile_tokens ? 2 : 1, same(p.end)};
             };
-            // fills gone through; weights and parts of each tile of rows; parts (of queries)
-            int f = 0, weights[2] = {0, 0}, ends[2] = {0, 0}, parts = 1;
-            Steps p = steps_at(lo);
-            bool ok = warp_wait(q_full, 0) && warp_wait(&k_full[0], 0), any = ok;
-            if (ok) {
+            // fills gone through; times scores were computed; weights and parts of each tile of rows; parts (of queries)
+            int f = 0, scored = 0, weights[2] = {0, 0}, ends[2] = {0, 0}, parts = 1;
+            // The scores of tile x of rows with the keys of stage s, once those before them have been read.
+            auto scores = [&](int x, int s) {
+                if (scored > 0 && !warp_wait(s_empty, (uint32_t)(scored - 1) & 1u)) { fail(52); return false; }
+                ++scored;
                 tc_fence_after();
-                issue_s(0, 0);
-                if (p.both == 2) issue_s(1, 0);
+                issue_s(x, s);
+                return true;
+            };
+            Steps p = steps_at(lo);
+            bool ok = warp_wait(q_full, 0) && warp_wait(&k_full[0], 0);
+            const bool any = ok;
+            if (!ok) fail(43);
+            ok = ok && scores(0, 0) && (p.both == 1 || scores(1, 0));
+            if (ok) {
                 commit(&k_empty[0]);
                 if (p.n_kt == 1) commit(q_empty);
-            } else {
-                fail(43);
             }
             while (ok) {
                 const bool last = p.end >= hi;               // the run's last part
@@ -380,29 +393,27 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                     const int s = f % NS, next = (f + 1) % NS;
                     const bool more = t + 1 < p.n_kt;        // scores to follow: of this part, or of the next one's first tile
                     const int following = more ? p.both : after.both;
-                    if (!(ok = warp_wait(&v_full[s], (uint32_t)(f / NS) & 1u))) { fail(44); break; }
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        if (ok && x < p.both) {
-                            if (t == 0 && ends[x] > 0 && !(ok = warp_wait(&o_empty[x], (uint32_t)(ends[x] - 1) & 1u))) fail(50);
-                            if (ok && !(ok = warp_wait(&p_full[x], (uint32_t)weights[x] & 1u))) fail(46);
-                            if (ok) {
-                                ++weights[x];
-                                tc_fence_after();
-                                issue_pv(x, s, t == 0);
-                                if (!more) { commit(&o_full[x]); ++ends[x]; }
-                            }
-                        }
-                        if (ok && x < following) {
-                            if (x == 0) {
-                                if (!(ok = warp_wait(&k_full[next], (uint32_t)((f + 1) / NS) & 1u))) fail(45);
-                                if (ok && !more && !(ok = warp_wait(q_full, (uint32_t)parts & 1u))) fail(51);
-                                tc_fence_after();
-                            }
-                            if (ok) issue_s(x, next);
-                        }
+                    auto weighted = [&](int x) {
+                        if (t == 0 && ends[x] > 0 && !warp_wait(&o_empty[x], (uint32_t)(ends[x] - 1) & 1u)) { fail(50); return false; }
+                        if (!warp_wait(&p_full[x], (uint32_t)weights[x] & 1u)) { fail(46); return false; }
+                        ++weights[x];
+                        if (!more) ++ends[x];
+                        tc_fence_after();
+                        issue_pv(x, s, t == 0);
+                        return true;
+                    };
+                    if (following) {
+                        if (!(ok = warp_wait(&k_full[next], (uint32_t)((f + 1) / NS) & 1u))) { fail(45); break; }
+                        if (!more && !(ok = warp_wait(q_full, (uint32_t)parts & 1u))) { fail(51); break; }
+                        if (!(ok = scores(0, next))) break;
                     }
-                    if (!ok) break;
+                    if (!(ok = warp_wait(&v_full[s], (uint32_t)(f / NS) & 1u))) { fail(44); break; }
+                    if (!(ok = weighted(0))) break;
+                    // B's next scores take the place of A's, which A's threads read when they are done with this tile; at a
+                    // part's end they write its results first, so there B's weights go ahead
+                    if (!more && p.both == 2 && !(ok = weighted(1))) break;
+                    if (following == 2 && !(ok = scores(1, next))) break;
+                    if (more && p.both == 2 && !(ok = weighted(1))) break;
                     commit(&v_empty[s]);
                     if (following) {
                         commit(&k_empty[next]);
@@ -423,10 +434,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
         // ---- a thread a row ---------------------------------------------------------------------------------------------
         const int x = warp >> 2, quarter = warp & 3, row = quarter * 32 + (threadIdx.x & 31);
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        const uint32_t tmem_s = tmem + (uint32_t)x * 128 + lane_base;                            // this tile's scores; weights over them
+        const uint32_t tmem_s = tmem + lane_base, tmem_p = tmem + kTmemP + (uint32_t)x * 64 + lane_base;       // scores; this tile's weights
         const uint32_t tmem_o = tmem + kTmemO + (uint32_t)x * 128 + lane_base;
         constexpr float kLazy = 8.0f;
-        int scores = 0, ends = 0;
+        int tiles = 0;                       // of keys, of all parts
         bool ok = true;
         for (int u = u_lo; u < u_hi && ok;) {
             const Part p = part_at(a, line, blocks, u, u_hi);
@@ -440,13 +451,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             const int first_pos = p.first_pos + x * a.tile_tokens, last_pos = first_pos + x_tokens - 1;
             const int token = row / group, pos = first_pos + min(token, x_tokens - 1);
             float m = -CUDART_INF_F, l = 0.f;
-            for (int t = 0; t < p.n_kt; ++t) {
+            for (int t = 0; t < p.n_kt; ++t, ++tiles) {
                 const int key0 = (p.kt0 + t) * kKeys;
-                if (!warp_wait(&s_full[x], (uint32_t)scores & 1u)) { fail(47); ok = false; break; }
-                ++scores;
+                if (!warp_wait(&s_full[x], (uint32_t)tiles & 1u)) { fail(47); ok = false; break; }
                 tc_fence_after();
                 float sv[128];
                 tmem_ld128(tmem_s, sv);
+                tc_fence_before();
+                warp_arrive(s_empty);
                 // every row sees every key of the tile, or a mask is needed
                 if (key0 + kKeys - 1 > first_pos || (a.window > 0 && key0 <= last_pos - a.window)) {
                     const int hi = pos - key0, lo = a.window > 0 ? hi - a.window + 1 : 0;        // this row's keys: lo .. hi
@@ -463,9 +475,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                     for (int e = 0; e < 8; ++e) top8[e] = fmax3(top8[e], sv[j + e], sv[j + 8 + e]);
                 // maximum of the raw scores (the scale is positive)
                 const float top = fmaxf(fmax3(top8[0], top8[1], top8[2]), fmax3(fmax3(top8[3], top8[4], top8[5]), top8[6], top8[7])) * a.scale_log2;
+                // the PV before is done: the accumulator may be rescaled, and new weights written
+                if (t > 0) {
+                    if (!warp_wait(&pv_done[x], (uint32_t)(tiles - 1) & 1u)) { fail(49); ok = false; break; }
+                    tc_fence_after();
+                }
                 if (__any_sync(0xffffffffu, top > m + kLazy)) {
                     const float mx = fmaxf(m, top), corr = mx == -CUDART_INF_F ? 1.0f : ex2_approx(m - mx);
-                    if (t > 0) {             // (PV of the tile before is done: the scores came after it)
+                    if (t > 0) {
 #pragma unroll
                         for (int c = 0; c < HD / 16; ++c) {
                             float acc[16];
@@ -493,17 +510,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                         sum2[(j / 2) & 1] = add_f32x2(sum2[(j / 2) & 1], pack_f32x2(x0, x1));
                         pk[j / 2] = pack_bf16(x0, x1);
                     }
-                    tmem_st32_raw(tmem_s + (uint32_t)(part * 32), pk);
+                    tmem_st32_raw(tmem_p + (uint32_t)(part * 32), pk);
                 }
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(&p_full[x]);
+                warp_arrive(&p_full[x]);
                 float lo2, hi2;
                 unpack_f32x2(add_f32x2(sum2[0], sum2[1]), lo2, hi2);
                 l += lo2 + hi2;
             }
-            if (ok && !warp_wait(&o_full[x], (uint32_t)ends & 1u)) { fail(48); ok = false; }
-            ++ends;
+            if (ok && !warp_wait(&pv_done[x], (uint32_t)(tiles - 1) & 1u)) { fail(48); ok = false; }
             tc_fence_after();
             if (!__all_sync(0xffffffffu, ok && !*failed)) { ok = false; break; }
             const bool live = token < x_tokens;
@@ -516,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 tmem_ld32(tmem_o + (uint32_t)(c * 32), o);
                 if (c == HD / 32 - 1) {      // all of it has been read
                     tc_fence_before();
-                    mbar_arrive(&o_empty[x]);
+                    warp_arrive(&o_empty[x]);
                 }
                 if (!whole) {
 #pragma unroll
@@ -605,7 +621,7 @@ int sm_count() {
 template <int HD>
 void launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkArgs& a, int blocks, int least_run, cudaStream_t stream) {
     constexpr int NS = stages_of(HD);
-    const size_t smem = 1024 + (size_t)(2 + 2 * NS) * (HD / 64) * kBlockBytes + (11 + 4 * NS) * sizeof(uint64_t) + 8 +
+    const size_t smem = 1024 + (size_t)(2 + 2 * NS) * (HD / 64) * kBlockBytes + (12 + 4 * NS) * sizeof(uint64_t) + 8 +
                         (size_t)(4 * a.seqs + blocks + 2) * sizeof(int);
     auto kernel = attention_chunk_kernel<HD>;
     static bool prepared[kDevices] = {};
