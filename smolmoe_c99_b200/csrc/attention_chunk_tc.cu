@@ -40,8 +40,8 @@ using namespace tc5;
 
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kRowWarps = 8;                // a thread a row: warps 0-3 tile A, 4-7 tile B
-constexpr int kMmaWarp = 8, kLoadWarp = 9;
-constexpr int kThreads = (kRowWarps + 2) * 32;
+constexpr int kScoreWarp = 8, kSumWarp = 9, kLoadWarp = 10;     // Q K^T, P V, the copies
+constexpr int kThreads = (kRowWarps + 3) * 32;
 constexpr int kBlockBytes = 128 * 128;      // 128 rows of 128 bytes: one swizzled block of 64 bfloat16 columns
 constexpr int kMaxSeqs = 1024, kMaxBlocks = 2048;
 
@@ -213,8 +213,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
     uint64_t* pv_done = bars + 6;                        // [2] a PV is done: its weights' place is free, the accumulator whole
     uint64_t* o_empty = bars + 8;                        // [2] the part's accumulator has been read
     uint64_t* s_empty = bars + 10;                       // the scores have been read
-    uint64_t* drain_bar = bars + 11;
-    uint64_t *k_full = bars + 12, *k_empty = k_full + NS, *v_full = k_empty + NS, *v_empty = v_full + NS;
+    uint64_t* drain_bar = bars + 11;                     // [2] of each issuing warp
+    uint64_t *k_full = bars + 13, *k_empty = k_full + NS, *v_full = k_empty + NS, *v_empty = v_full + NS;
     uint32_t* tmem_slot = (uint32_t*)(v_empty + NS);
     volatile int* failed = (volatile int*)(tmem_slot + 1);
     Line line;
@@ -235,12 +235,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             mbar_init(&o_empty[x], 4);
         }
         mbar_init(s_empty, 4);
-        mbar_init(drain_bar, 1);
+        mbar_init(&drain_bar[0], 1);
+        mbar_init(&drain_bar[1], 1);
         for (int i = 0; i < 4 * NS; ++i) mbar_init(&k_full[i], 1);
         *failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
+    if (warp == kScoreWarp) tmem_alloc(tmem_slot, 512);
     // the rows of the query tiles that no copy fills: zeros
     for (int i = threadIdx.x; i < 2 * DB * (kRows - tile_rows) * 8; i += kThreads) {
         const int block = i / ((kRows - tile_rows) * 8), rest = i - block * (kRows - tile_rows) * 8;
@@ -323,112 +324,93 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 for (int i = 0; i < n; ++i) mbar_wait(&v_full[left[i].stage], left[i].parity);
             }
         }
-    } else if (warp == kMmaWarp) {
-        // One warp issues all products, the tiles' strictly in turn: issued by a warp each, they mix on the tensor cores, and
-        // both tiles then turn scores into weights at the same time. Its lanes go through the run together and one of them
-        // issues: the operands of tcgen05.mma then stay in the warp's uniform registers. (With one lane going through it all by
-        // itself a product took 80 cycles to issue against 64 to run, and the row threads waited for that.)
+    } else if (warp == kScoreWarp || warp == kSumWarp) {
+        // A warp issues the scores' products, another the sums of values, each at its own pace. A warp's lanes go through the
+        // run together and one of them issues: the operands of tcgen05.mma then stay in the warp's uniform registers. (With one
+        // lane going through it all by itself a product took 80 cycles to issue against 64 to run.)
         auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
-        const int lo = same(u_lo), hi = same(u_hi);
-        if (lo < hi) {
-            const uint32_t idesc_s = instr_desc(kRows, kKeys), idesc_pv = instr_desc(kRows, HD) | (1u << 16);     // V is MN-major
-            const uint64_t desc_q = smem_desc(smem_u32(q_s)), desc_k = smem_desc(smem_u32(k_s)), desc_v = smem_desc_rows(smem_u32(v_s));
-            const uint32_t tm = (uint32_t)same((int)tmem);
-            auto issue_s = [&](int x, int s) {
-                const uint64_t q = desc_q + (uint64_t)(((uint32_t)x * kTileBytes) >> 4), k = desc_k + (uint64_t)(((uint32_t)s * kTileBytes) >> 4);
-                if (elect_one()) {
-#pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks) {
-                        const uint64_t off = (uint64_t)(((uint32_t)(ks / 4) * kBlockBytes + (uint32_t)(ks % 4) * 32) >> 4);
-                        umma_bf16(tm, q + off, k + off, idesc_s, ks > 0 ? 1u : 0u);
-                    }
-                    umma_commit(&s_full[x]);
-                }
-                __syncwarp();
-            };
-            auto issue_pv = [&](int x, int s, bool first) {
-                const uint64_t v = desc_v + (uint64_t)(((uint32_t)s * kTileBytes) >> 4);
-                if (elect_one()) {
-#pragma unroll
-                    for (int ks = 0; ks < kKeys / 16; ++ks)
-                        umma_bf16_ts(tm + kTmemO + (uint32_t)x * 128, tm + kTmemP + (uint32_t)x * 64 + (uint32_t)ks * 8,
-                                     v + (uint64_t)(((uint32_t)ks * 16 * 128) >> 4), idesc_pv, first && ks == 0 ? 0u : 1u);
-                    umma_commit(&pv_done[x]);
-                }
-                __syncwarp();
-            };
-            auto commit = [&](uint64_t* bar) {
-                if (elect_one()) umma_commit(bar);
-                __syncwarp();
-            };
-            struct Steps { int n_kt, both, end; };       // of a part: tiles of keys, tiles of rows, its end on the line
-            auto steps_at = [&](int u) {
-                const Part p = part_at(a, line, blocks, u, hi);
-                return Steps{same(p.n_kt), same(p.tokens) > a.tile_tokens ? 2 : 1, same(p.end)};
-            };
-            // fills gone through; times scores were computed; weights and parts of each tile of rows; parts (of queries)
-            int f = 0, scored = 0, weights[2] = {0, 0}, ends[2] = {0, 0}, parts = 1;
-            // The scores of tile x of rows with the keys of stage s, once those before them have been read.
-            auto scores = [&](int x, int s) {
-                if (scored > 0 && !warp_wait(s_empty, (uint32_t)(scored - 1) & 1u)) { fail(52); return false; }
-                ++scored;
-                tc_fence_after();
-                issue_s(x, s);
-                return true;
-            };
-            Steps p = steps_at(lo);
-            bool ok = warp_wait(q_full, 0) && warp_wait(&k_full[0], 0);
-            const bool any = ok;
-            if (!ok) fail(43);
-            ok = ok && scores(0, 0) && (p.both == 1 || scores(1, 0));
-            if (ok) {
-                commit(&k_empty[0]);
-                if (p.n_kt == 1) commit(q_empty);
-            }
-            while (ok) {
-                const bool last = p.end >= hi;               // the run's last part
-                Steps after = {0, 0, 0};
-                if (!last) after = steps_at(p.end);
+        const int lo = same(u_lo), hi = same(u_hi), role = same(warp - kScoreWarp);
+        const uint32_t tm = (uint32_t)same((int)tmem);
+        auto commit = [&](uint64_t* bar) {
+            if (elect_one()) umma_commit(bar);
+            __syncwarp();
+        };
+        struct Steps { int n_kt, both, end; };           // of a part: tiles of keys, tiles of rows, its end on the line
+        auto steps_at = [&](int u) {
+            const Part p = part_at(a, line, blocks, u, hi);
+            return Steps{same(p.n_kt), same(p.tokens) > a.tile_tokens ? 2 : 1, same(p.end)};
+        };
+        bool ok = true;
+        int f = 0;                                       // fills gone through
+        if (role == 0) {
+            const uint32_t idesc = instr_desc(kRows, kKeys);
+            const uint64_t desc_q = smem_desc(smem_u32(q_s)), desc_k = smem_desc(smem_u32(k_s));
+            int scored = 0, parts = 0;                   // times scores were computed, parts
+            for (int u = lo; u < hi && ok; ++parts) {
+                const Steps p = steps_at(u);
+                u = p.end;
+                if (!(ok = warp_wait(q_full, (uint32_t)parts & 1u))) { fail(51); break; }
                 for (int t = 0; t < p.n_kt && ok; ++t, ++f) {
-                    const int s = f % NS, next = (f + 1) % NS;
-                    const bool more = t + 1 < p.n_kt;        // scores to follow: of this part, or of the next one's first tile
-                    const int following = more ? p.both : after.both;
-                    auto weighted = [&](int x) {
-                        if (t == 0 && ends[x] > 0 && !warp_wait(&o_empty[x], (uint32_t)(ends[x] - 1) & 1u)) { fail(50); return false; }
-                        if (!warp_wait(&p_full[x], (uint32_t)weights[x] & 1u)) { fail(46); return false; }
-                        ++weights[x];
-                        if (!more) ++ends[x];
+                    const int s = f % NS;
+                    if (!(ok = warp_wait(&k_full[s], (uint32_t)(f / NS) & 1u))) { fail(45); break; }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        if (x >= p.both || !ok) continue;
+                        // once the scores before these have been read
+                        if (scored > 0 && !(ok = warp_wait(s_empty, (uint32_t)(scored - 1) & 1u))) { fail(52); continue; }
+                        ++scored;
                         tc_fence_after();
-                        issue_pv(x, s, t == 0);
-                        return true;
-                    };
-                    if (following) {
-                        if (!(ok = warp_wait(&k_full[next], (uint32_t)((f + 1) / NS) & 1u))) { fail(45); break; }
-                        if (!more && !(ok = warp_wait(q_full, (uint32_t)parts & 1u))) { fail(51); break; }
-                        if (!(ok = scores(0, next))) break;
+                        const uint64_t q = desc_q + (uint64_t)(((uint32_t)x * kTileBytes) >> 4), k = desc_k + (uint64_t)(((uint32_t)s * kTileBytes) >> 4);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int ks = 0; ks < HD / 16; ++ks) {
+                                const uint64_t off = (uint64_t)(((uint32_t)(ks / 4) * kBlockBytes + (uint32_t)(ks % 4) * 32) >> 4);
+                                umma_bf16(tm, q + off, k + off, idesc, ks > 0 ? 1u : 0u);
+                            }
+                            umma_commit(&s_full[x]);
+                        }
+                        __syncwarp();
                     }
-                    if (!(ok = warp_wait(&v_full[s], (uint32_t)(f / NS) & 1u))) { fail(44); break; }
-                    if (!(ok = weighted(0))) break;
-                    // B's next scores take the place of A's, which A's threads read when they are done with this tile; at a
-                    // part's end they write its results first, so there B's weights go ahead
-                    if (!more && p.both == 2 && !(ok = weighted(1))) break;
-                    if (following == 2 && !(ok = scores(1, next))) break;
-                    if (more && p.both == 2 && !(ok = weighted(1))) break;
-                    commit(&v_empty[s]);
-                    if (following) {
-                        commit(&k_empty[next]);
-                        // the last scores of a part: its queries' memory may take the next part's
-                        if (more ? t + 2 == p.n_kt : after.n_kt == 1) commit(q_empty);
-                    }
+                    if (!ok) break;
+                    commit(&k_empty[s]);
+                    if (t + 1 == p.n_kt) commit(q_empty);
                 }
-                if (last) break;
-                p = after;
-                ++parts;
             }
-            if (__any_sync(0xffffffffu, !ok || *failed) && any) {
-                commit(drain_bar);
-                warp_wait(drain_bar, 0);
+        } else {
+            const uint32_t idesc = instr_desc(kRows, HD) | (1u << 16);     // V is MN-major
+            const uint64_t desc_v = smem_desc_rows(smem_u32(v_s));
+            int weights[2] = {0, 0}, ends[2] = {0, 0};   // tiles of keys and parts, of each tile of rows
+            for (int u = lo; u < hi && ok;) {
+                const Steps p = steps_at(u);
+                u = p.end;
+                for (int t = 0; t < p.n_kt && ok; ++t, ++f) {
+                    const int s = f % NS;
+                    if (!(ok = warp_wait(&v_full[s], (uint32_t)(f / NS) & 1u))) { fail(44); break; }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        if (x >= p.both || !ok) continue;
+                        if (t == 0 && ends[x] > 0 && !(ok = warp_wait(&o_empty[x], (uint32_t)(ends[x] - 1) & 1u))) { fail(50); continue; }
+                        if (!(ok = warp_wait(&p_full[x], (uint32_t)weights[x] & 1u))) { fail(46); continue; }
+                        ++weights[x];
+                        if (t + 1 == p.n_kt) ++ends[x];
+                        tc_fence_after();
+                        const uint64_t v = desc_v + (uint64_t)(((uint32_t)s * kTileBytes) >> 4);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int ks = 0; ks < kKeys / 16; ++ks)
+                                umma_bf16_ts(tm + kTmemO + (uint32_t)x * 128, tm + kTmemP + (uint32_t)x * 64 + (uint32_t)ks * 8,
+                                             v + (uint64_t)(((uint32_t)ks * 16 * 128) >> 4), idesc, t == 0 && ks == 0 ? 0u : 1u);
+                            umma_commit(&pv_done[x]);
+                        }
+                        __syncwarp();
+                    }
+                    if (ok) commit(&v_empty[s]);
+                }
             }
+        }
+        if (__any_sync(0xffffffffu, !ok || *failed)) {   // no product is left under way
+            commit(&drain_bar[role]);
+            warp_wait(&drain_bar[role], 0);
         }
     } else {
         // ---- a thread a row ---------------------------------------------------------------------------------------------
@@ -555,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+    if (warp == kScoreWarp) tmem_dealloc(tmem, 512);
 }
 
 // Puts the parts of a cut pair together, in the order of the line: blockIdx.x the pair, blockIdx.y eight of its dimensions, a
@@ -621,7 +603,7 @@ int sm_count() {
 template <int HD>
 void launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkArgs& a, int blocks, int least_run, cudaStream_t stream) {
     constexpr int NS = stages_of(HD);
-    const size_t smem = 1024 + (size_t)(2 + 2 * NS) * (HD / 64) * kBlockBytes + (12 + 4 * NS) * sizeof(uint64_t) + 8 +
+    const size_t smem = 1024 + (size_t)(2 + 2 * NS) * (HD / 64) * kBlockBytes + (13 + 4 * NS) * sizeof(uint64_t) + 8 +
                         (size_t)(4 * a.seqs + blocks + 2) * sizeof(int);
     auto kernel = attention_chunk_kernel<HD>;
     static bool prepared[kDevices] = {};
