@@ -5,11 +5,21 @@
 // 128 / group tokens, keys are read once for all of them, and few rows lie beyond a tile's causal border. A CTA has two
 // such tiles, A and B, under way: while the threads of one turn scores into weights, the tensor cores work for the other.
 //   S_X = Q_X K^T    tcgen05.mma 128 x 128 x head_dim, both operands in shared memory, S (float) in tensor memory;
-//   P_X = 2^(S * scale - reference) as bfloat16, back into tensor memory over the scores (a thread per row);
+//   P_X = 2^(S * scale - reference) as bfloat16, back into tensor memory (a thread per row);
 //   O_X += P_X V     tcgen05.mma 128 x head_dim x 128, P_X from tensor memory, V as it lies in memory (MN-major).
-// In order on the tensor cores: S_A S_B | P_A: PV_A, next S_A | P_B: PV_B, next S_B | ... A row's reference is lazy: it moves
-// when a tile's maximum exceeds it by more than 2^8, and only then is the accumulator rescaled; the scores of a tile come
-// after the PV of the tile before, so whoever has waited for them may touch the accumulator.
+// A row's reference is lazy: it moves when a tile's maximum exceeds it by more than 2^8, and only then is the accumulator
+// rescaled.
+//
+// Tensor memory holds S (128 columns), P_A, P_B (64 each), O_A, O_B (128 each): the tiles take turns with one place for scores,
+// free as soon as they are in the threads' registers, so S_B is computed while A's threads turn theirs into weights and the
+// next S_A while B's do; the sums of values are issued by a warp of their own whenever weights are there. What was measured at
+// 1,024 tokens of 28 heads of 128 onto 16,000 (249 GFLOP of products), in the order it was built: weights in the place of their
+// scores, one thread issuing everything 278 us; the issuing warp's lanes together, one of them issuing 263; weights beside
+// the scores 249; scores and sums issued by a warp each 241. The products alone, with the same waits, take 177, and 223 with no
+// exponentials: what is left is the way of a tile through its threads (read 64 KB of scores, largest, exponentials at 16 a cycle,
+// write) and the turns with the one place. Two threads a row 247, a place for each tile's scores with heads of 64 115 against
+// 107 (the tiles' threads then want the exponential unit at the same time), halves of 64 keys 414, part of the exponentials
+// as polynomials and tiles issued by a warp each were slower too.
 //
 // Work is shared out as a line: the tiles of 128 keys of all pairs (two query tiles of one kv head), one after the other; each
 // CTA of a grid of one an SM takes an equal run. What a run cuts is left as float accumulators, references and sums in a
