@@ -431,15 +431,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
         constexpr float kLazy = 8.0f;
         int tiles = 0;                       // of keys, of all parts
         bool ok = true;
-        for (int u = u_lo; u < u_hi && ok;) {
+        for (int u = u_lo; u < u_hi;) {
             const Part p = part_at(a, line, blocks, u, u_hi);
+            // (a warp that gave up still says of the pairs that begin here that there is nothing to join)
             if (threadIdx.x == 0 && p.pair_at >= u_lo)
-                a.cuts[p.number] = ChunkCut{p.first_token, p.kvh, p.end == p.pair_at + p.tiles ? 0 : p.tokens, (int)blockIdx.x, (p.pair_at + p.tiles - 1) / run, {0, 0, 0}};
+                a.cuts[p.number] = ChunkCut{p.first_token, p.kvh, p.end == p.pair_at + p.tiles || !ok ? 0 : p.tokens, (int)blockIdx.x, (p.pair_at + p.tiles - 1) / run, {0, 0, 0}};
             const bool whole = u == p.pair_at && p.end == p.pair_at + p.tiles;
             const int cut_slot = p.pair_at < u_lo ? 0 : 1;
             u = p.end;
             const int x_tokens = min(a.tile_tokens, p.tokens - x * a.tile_tokens);               // tokens of this tile of rows
-            if (x_tokens <= 0) continue;
+            if (x_tokens <= 0 || !ok) continue;
             const int first_pos = p.first_pos + x * a.tile_tokens, last_pos = first_pos + x_tokens - 1;
             const int token = row / group, pos = first_pos + min(token, x_tokens - 1);
             float m = -CUDART_INF_F, l = 0.f;
@@ -513,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             }
             if (ok && !warp_wait(&pv_done[x], (uint32_t)(tiles - 1) & 1u)) { fail(48); ok = false; }
             tc_fence_after();
-            if (!__all_sync(0xffffffffu, ok && !*failed)) { ok = false; break; }
+            if (!__all_sync(0xffffffffu, ok && !*failed)) { ok = false; continue; }
             const bool live = token < x_tokens;
             const float inv = 1.0f / l;
             __nv_bfloat16* dst = a.out + ((size_t)(p.first_token + x * a.tile_tokens + token) * a.heads + (size_t)p.kvh * group + (row - token * group)) * HD;
@@ -648,6 +649,7 @@ void attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int
         throw std::invalid_argument("attention_chunk: " + std::to_string(heads) + " heads on " + std::to_string(kv_heads) + " of size " +
                                     std::to_string(head_dim) + " (64 or 128, at most 64 heads a kv head), " + std::to_string(n_seqs) + " sequences, " +
                                     std::to_string(blocks) + " blocks of queries");
+    if (!(scale > 0.f) || !(scale < INFINITY)) throw std::invalid_argument("attention_chunk: a scale of " + std::to_string(scale));
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15)
         throw std::invalid_argument("attention_chunk: operands must be 16-byte aligned");
     if (workspace_floats < attention_chunk_workspace(head_dim, kv_heads, blocks)) throw std::invalid_argument("attention_chunk: the workspace is too small");

@@ -723,21 +723,29 @@ __global__ void __launch_bounds__(line_warps(NHT) * 32, 1) attention_quant_line_
         const int pair_at = table.tiles_before[i] + pair * s.tiles, part_end = min(u_hi, pair_at + s.tiles);
         const int tokens = min(a.block_tokens, s.n - token0), rows = tokens * group;
         const int first_token = a.cu[i] + token0;
+        const bool begins = pair_at >= u_lo, whole = begins && part_end == pair_at + s.tiles;
+        // (a warp that gave up still says of the pairs it begins that there is nothing to join)
+        if (begins && lane == 0)
+            a.cuts[table.pairs_before[i] + pair] =
+                Cut{first_token, kvh, whole || !ok ? 0 : rows, number, (pair_at + s.tiles - 1) / run, {0, 0, 0}};
+        if (!ok) {
+            u = part_end;
+            continue;
+        }
         R_ state;
         state.begin(a, (size_t)first_token * a.heads + (size_t)kvh * group, s.start + token0, tokens);
-        for (; u < part_end && ok; ++u) {
+        for (; u < part_end; ++u) {
             if (!(ok = ring.wait(a))) break;
             state.tile(a, (s.first_tile + (u - pair_at)) * KT, ring.codes_at(ring.stage), ring.scales_at(ring.stage));
             __syncwarp();        // every lane has read the slot
             if (u - u_lo + S < ring.tiles) request(u - u_lo + S, ring.stage);
             ring.next();
         }
-        if (!ok) break;          // (the pair's rows are not valid: the error word says so)
+        if (!ok) {               // (the pair's rows are not valid: the error word says so)
+            u = part_end;
+            continue;
+        }
         const float unit = state.end();
-        const bool begins = pair_at >= u_lo, whole = begins && part_end == pair_at + s.tiles;
-        if (begins && lane == 0)
-            a.cuts[table.pairs_before[i] + pair] =
-                Cut{first_token, kvh, whole ? 0 : rows, number, (pair_at + s.tiles - 1) / run, {0, 0, 0}};
         float* part = a.parts + ((size_t)number * 2 + (begins ? 1 : 0)) * R * LD;
 #pragma unroll
         for (int nh = 0; nh < NHT; ++nh)
@@ -910,6 +918,7 @@ void attention_quant(const QuantPools& p, const void* q, void* out, int n_seqs, 
     if (!attention_quant_supports(heads, kv_heads, head_dim, p.pages))
         throw std::invalid_argument("attention_quant: " + std::to_string(heads) + " heads on " + std::to_string(kv_heads) + " of size " +
                                     std::to_string(head_dim) + " (multiples of 16 up to 128, at most 16 heads a kv head), or a pool of 2^31 rows");
+    if (!(scale > 0.f) || !(scale < INFINITY)) throw std::invalid_argument("attention_quant: a scale of " + std::to_string(scale));
     if (cluster < 0 || cluster > kMaxCluster) throw std::invalid_argument("attention_quant: clusters of " + std::to_string(cluster) + " CTAs");
     if ((long long)pairs * std::max(cluster, 1) > 0x7fffffffll) throw std::invalid_argument("attention_quant: too many pairs for one launch");
     const int group = heads / kv_heads;

@@ -140,8 +140,10 @@ class QuantLayer:
 
     def made_of(self, cache) -> bool:
         k, v, ks, vs, table = self.tensors
+        r = self.record
         return (cache.k_pool is k and cache.v_pool is v and cache.k_scale is ks and cache.v_scale is vs and cache.page_table is table
-                and not cache.ring and cache.kind == "kv")
+                and not cache.ring and cache.kind == "kv" and k.data_ptr() == r.k_codes and v.data_ptr() == r.v_codes
+                and ks.data_ptr() == r.k_scale and vs.data_ptr() == r.v_scale and table.data_ptr() == r.page_table)
 
 
 class PhaseTimes:
@@ -728,6 +730,8 @@ class Ops:
         window = int(window or 0)
         if window < 0:
             raise KernelError(f"a window of {window} positions")
+        if not 0 < scale < float("inf"):
+            raise KernelError(f"a scale of {scale}: positive and finite expected")
         slot_ids, seq_ends, cu = step.slot_ids, step.seq_ends, step.cu_seqlens
         _here(q, slot_ids, seq_ends, cu)
         heads, n_seqs = shape[1], step.n_seqs
@@ -797,6 +801,8 @@ class Ops:
         tokens = 8 * row_tiles // group
         pairs = kv_heads * sum(-(-n // tokens) for n in few)
         longest = max_len if not window else min(max_len, window + max(few))
+        if len(lens) > 4096 or pairs * (-(-longest // 32) + 1) >= 1 << 31:
+            return None                   # (more sequences, or tiles of the line, than the kernel counts)
         cluster = self._quant_cluster(pairs, longest, head_dim)
         floats = 0 if cluster else int(self.lib.sm_attention_quant_workspace(head_dim, row_tiles, pairs, 0))
         return limit, row_tiles, pairs, cluster, longest, floats, blocks, chunk_floats
