@@ -107,7 +107,7 @@ class QuantPools(ctypes.Structure):
 class QuantLayer:
     """The pools of an 8-bit layer cache, checked once, with the record that the kernels take."""
 
-    __slots__ = ("tensors", "record", "address", "pages", "kv_heads", "head_dim", "slots", "table_stride", "device")
+    __slots__ = ("tensors", "pointers", "record", "address", "pages", "kv_heads", "head_dim", "slots", "table_stride", "device")
 
     def __init__(self, cache):
         k, v, ks, vs, table = cache.k_pool, cache.v_pool, cache.k_scale, cache.v_scale, cache.page_table
@@ -133,17 +133,16 @@ class QuantLayer:
             raise KernelError("the pools, exponents and page table of an 8-bit cache must lie on one device")
         self.pages, self.kv_heads, _, self.head_dim = shape
         self.slots, self.table_stride = table.shape
-        self.record = QuantPools(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(), self.pages, fmt, self.kv_heads,
-                                 self.head_dim, self.slots, self.table_stride)
+        self.pointers = (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr())
+        self.record = QuantPools(*self.pointers, self.pages, fmt, self.kv_heads, self.head_dim, self.slots, self.table_stride)
         self.address = ctypes.addressof(self.record)
         self.tensors = (k, v, ks, vs, table)
 
     def made_of(self, cache) -> bool:
         k, v, ks, vs, table = self.tensors
-        r = self.record
         return (cache.k_pool is k and cache.v_pool is v and cache.k_scale is ks and cache.v_scale is vs and cache.page_table is table
-                and not cache.ring and cache.kind == "kv" and k.data_ptr() == r.k_codes and v.data_ptr() == r.v_codes
-                and ks.data_ptr() == r.k_scale and vs.data_ptr() == r.v_scale and table.data_ptr() == r.page_table)
+                and not cache.ring and cache.kind == "kv"
+                and (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr()) == self.pointers)
 
 
 class PhaseTimes:
