@@ -643,7 +643,7 @@ long long attention_chunk_workspace(int head_dim, int kv_heads, int blocks) {
 
 void attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window, const void* k_pages,
                      const void* v_pages, int pages, const int32_t* seq_ends, const int32_t* cu_seqlens, int skip_new, int blocks, float* workspace,
-                     long long workspace_floats, cudaStream_t stream) {
+                     long long workspace_floats, int* error, cudaStream_t stream) {
     if (n_seqs <= 0 || blocks <= 0 || T <= 0) return;
     if (!attention_chunk_supports(heads, kv_heads, head_dim, (long long)n_seqs * pages, n_seqs, blocks))
         throw std::invalid_argument("attention_chunk: " + std::to_string(heads) + " heads on " + std::to_string(kv_heads) + " of size " +
@@ -670,7 +670,7 @@ void attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int
                                         kPageSize, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
     ChunkCut* cuts = (ChunkCut*)workspace;
     ChunkArgs a{(__nv_bfloat16*)out, seq_ends, cu_seqlens, n_seqs, heads, kv_heads, window, skip_new, pages, tile_tokens, blocks, scale * 1.4426950408889634f, cuts,
-                workspace + (long long)blocks * kv_heads * (long long)(sizeof(ChunkCut) / sizeof(float)), error_word()};
+                workspace + (long long)blocks * kv_heads * (long long)(sizeof(ChunkCut) / sizeof(float)), error};
     // a run is at least this many tiles: a part costs about as much as one to leave and join
     const int least_run = 2;
     if (head_dim == 64) launch<64>(mq, mk, mv, a, blocks, least_run, stream);

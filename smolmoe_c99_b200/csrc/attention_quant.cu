@@ -912,7 +912,7 @@ long long attention_quant_workspace(int head_dim, int row_tiles, int pairs, int 
 
 void attention_quant(const QuantPools& p, const void* q, void* out, int n_seqs, int heads, float scale, int window, const int32_t* slot_ids,
                      const int32_t* seq_ends, const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles, int pairs, int cluster,
-                     float* workspace, long long workspace_floats, cudaStream_t stream) {
+                     float* workspace, long long workspace_floats, int* error, cudaStream_t stream) {
     if (n_seqs <= 0 || pairs <= 0) return;
     const int kv_heads = p.kv_heads, head_dim = p.head_dim;
     if (!attention_quant_supports(heads, kv_heads, head_dim, p.pages))
@@ -932,7 +932,7 @@ void attention_quant(const QuantPools& p, const void* q, void* out, int n_seqs, 
                (const uint8_t*)p.v_scale, {p.page_table, p.slots, p.table_stride, p.pages}, slot_ids, seq_ends, cu_seqlens, n_seqs, heads,
                kv_heads, head_dim, window, most_new, 8 * row_tiles / group, pairs, cluster, 0,
                cluster ? kClusterTile : line_tile(row_tiles), scale * 1.4426950408889634f, (Cut*)workspace,
-               workspace + (cluster ? 0 : (long long)pairs * (long long)(sizeof(Cut) / sizeof(float))), error_word()};
+               workspace + (cluster ? 0 : (long long)pairs * (long long)(sizeof(Cut) / sizeof(float))), error};
     CUtensorMap mk{}, mv{};
     if (head_dim == 64 || head_dim == 128) {
         // the pools as rows of codes; a box is a tile of positions of one kv head

@@ -134,18 +134,18 @@ SM_API int sm_kv_store(const void* k_packed, const void* v_packed, int dt, int T
 SM_API int sm_quant_pools_bytes() { return (int)sizeof(sm::QuantPools); }
 
 SM_API int sm_kv_quant_store(const sm::QuantPools* pools, const void* k_packed, const void* v_packed, int dt, int T, void* k_rows, void* v_rows,
-                             const int32_t* positions, const int32_t* token_slot, void* stream) {
+                             const int32_t* positions, const int32_t* token_slot, int* error, void* stream) {
     return guarded([&] {
-        sm::kv_quant_store(*pools, k_packed, v_packed, (sm::DType)dt, T, k_rows, v_rows, positions, token_slot, (cudaStream_t)stream);
+        sm::kv_quant_store(*pools, k_packed, v_packed, (sm::DType)dt, T, k_rows, v_rows, positions, token_slot, error, (cudaStream_t)stream);
     });
 }
 
 SM_API int sm_kv_quant_load(const sm::QuantPools* pools, int dt, int n_seqs, const int32_t* slot_ids, const int32_t* seq_ends, void* k_out,
                             void* v_out, int32_t* out_table, int pages, int whole, const int32_t* cu_seqlens, int skip_new, int attend,
-                            int window, void* stream) {
+                            int window, int* error, void* stream) {
     return guarded([&] {
         sm::kv_quant_load(*pools, (sm::DType)dt, n_seqs, slot_ids, seq_ends, k_out, v_out, out_table, pages, whole != 0, cu_seqlens, skip_new,
-                          attend != 0, window, (cudaStream_t)stream);
+                          attend != 0, window, error, (cudaStream_t)stream);
     });
 }
 
@@ -263,10 +263,10 @@ SM_API long long sm_attention_quant_workspace(int head_dim, int row_tiles, int p
 
 SM_API int sm_attention_quant(const sm::QuantPools* pools, const void* q, void* out, int n_seqs, int heads, float scale, int window,
                               const int32_t* slot_ids, const int32_t* seq_ends, const int32_t* cu_seqlens, int max_len, int most_new,
-                              int row_tiles, int pairs, int cluster, float* workspace, long long workspace_floats, void* stream) {
+                              int row_tiles, int pairs, int cluster, float* workspace, long long workspace_floats, int* error, void* stream) {
     return guarded([&] {
         sm::attention_quant(*pools, q, out, n_seqs, heads, scale, window, slot_ids, seq_ends, cu_seqlens, max_len, most_new, row_tiles, pairs,
-                            cluster, workspace, workspace_floats, (cudaStream_t)stream);
+                            cluster, workspace, workspace_floats, error, (cudaStream_t)stream);
     });
 }
 
@@ -280,10 +280,10 @@ SM_API long long sm_attention_chunk_workspace(int head_dim, int kv_heads, int bl
 
 SM_API int sm_attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window,
                               const void* k_pages, const void* v_pages, int pages, const int32_t* seq_ends, const int32_t* cu_seqlens,
-                              int skip_new, int blocks, float* workspace, long long workspace_floats, void* stream) {
+                              int skip_new, int blocks, float* workspace, long long workspace_floats, int* error, void* stream) {
     return guarded([&] {
         sm::attention_chunk(q, out, T, n_seqs, heads, kv_heads, head_dim, scale, window, k_pages, v_pages, pages, seq_ends, cu_seqlens,
-                            skip_new, blocks, workspace, workspace_floats, (cudaStream_t)stream);
+                            skip_new, blocks, workspace, workspace_floats, error, (cudaStream_t)stream);
     });
 }
 

@@ -95,10 +95,10 @@ struct QuantPools {
 // without a scale is read as zeros and its key as NaN instead (a token that sees it is NaN either way), and pages of 128
 // positions that no token of the step sees in `window` are left alone.
 void kv_quant_store(const QuantPools& pools, const void* k_packed, const void* v_packed, DType dt, int T, void* k_rows, void* v_rows,
-                    const int32_t* positions, const int32_t* token_slot, cudaStream_t stream);
+                    const int32_t* positions, const int32_t* token_slot, int* error, cudaStream_t stream);
 void kv_quant_load(const QuantPools& pools, DType dt, int n_seqs, const int32_t* slot_ids, const int32_t* seq_ends, void* k_out, void* v_out,
                    int32_t* out_table, int pages, bool whole, const int32_t* cu_seqlens, int skip_new, bool attend, int window,
-                   cudaStream_t stream);
+                   int* error, cudaStream_t stream);
 
 // ---- gemm_simt.cu ---------------------------------------------------------------------
 // out[t, n] (+)= sum_k x[t, k] * w[n, k] + bias[n]; float FMA in ascending k for every
@@ -279,7 +279,7 @@ bool attention_quant_supports(int heads, int kv_heads, int head_dim, long long p
 long long attention_quant_workspace(int head_dim, int row_tiles, int pairs, int cluster);   // floats
 void attention_quant(const QuantPools& pools, const void* q, void* out, int n_seqs, int heads, float scale, int window, const int32_t* slot_ids,
                      const int32_t* seq_ends, const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles, int pairs, int cluster,
-                     float* workspace, long long workspace_floats, cudaStream_t stream);
+                     float* workspace, long long workspace_floats, int* error, cudaStream_t stream);
 
 // ---- attention_chunk_tc.cu ------------------------------------------------------------
 // The same attention for sequences that bring more than `skip_new` tokens, over their pages as bfloat16 values as
@@ -289,7 +289,7 @@ bool attention_chunk_supports(int heads, int kv_heads, int head_dim, long long p
 long long attention_chunk_workspace(int head_dim, int kv_heads, int blocks);   // floats
 void attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window, const void* k_pages,
                      const void* v_pages, int pages, const int32_t* seq_ends, const int32_t* cu_seqlens, int skip_new, int blocks, float* workspace,
-                     long long workspace_floats, cudaStream_t stream);
+                     long long workspace_floats, int* error, cudaStream_t stream);
 
 // ---- decode_fused.cu ------------------------------------------------------------------
 // One decode step (every sequence goes on by one token) of a stack of standard layers -- RMSNorm, attention with

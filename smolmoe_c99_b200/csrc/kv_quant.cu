@@ -223,7 +223,7 @@ void check_pools(const char* who, const QuantPools& p) {
 }  // namespace
 
 void kv_quant_store(const QuantPools& p, const void* k_packed, const void* v_packed, DType dt, int T, void* k_rows, void* v_rows,
-                    const int32_t* positions, const int32_t* token_slot, cudaStream_t stream) {
+                    const int32_t* positions, const int32_t* token_slot, int* error, cudaStream_t stream) {
     if (T <= 0) return;
     check_pools("kv_quant_store", p);
     if (((uintptr_t)k_packed | (uintptr_t)v_packed | (uintptr_t)k_rows | (uintptr_t)v_rows) & 15)
@@ -232,7 +232,7 @@ void kv_quant_store(const QuantPools& p, const void* k_packed, const void* v_pac
     int lanes = 1;
     while (lanes * 8 < p.head_dim) lanes *= 2;
     StoreArgs a{{k_packed, v_packed}, {k_rows, v_rows}, {(uint8_t*)p.k_codes, (uint8_t*)p.v_codes}, {(uint8_t*)p.k_scale, (uint8_t*)p.v_scale},
-                positions, token_slot, {p.page_table, p.slots, p.table_stride, p.pages}, p.kv_heads, p.head_dim, (unsigned)(T * p.kv_heads), error_word()};
+                positions, token_slot, {p.page_table, p.slots, p.table_stride, p.pages}, p.kv_heads, p.head_dim, (unsigned)(T * p.kv_heads), error};
     const unsigned per_block = kThreads / lanes * kStoreRows;
     const dim3 grid((a.rows_of_each + per_block - 1) / per_block, 2);
     note_launch();
@@ -243,14 +243,14 @@ void kv_quant_store(const QuantPools& p, const void* k_packed, const void* v_pac
 
 void kv_quant_load(const QuantPools& p, DType dt, int n_seqs, const int32_t* slot_ids, const int32_t* seq_ends, void* k_out, void* v_out,
                    int32_t* out_table, int pages, bool whole, const int32_t* cu_seqlens, int skip_new, bool attend, int window,
-                   cudaStream_t stream) {
+                   int* error, cudaStream_t stream) {
     if (n_seqs <= 0 || pages <= 0) return;
     check_pools("kv_quant_load", p);
     if (n_seqs > 65535) throw std::invalid_argument("kv_quant_load: more than 65535 sequences");
     if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) throw std::invalid_argument("kv_quant_load: outputs must be 16-byte aligned");
     LoadArgs a{{(const uint8_t*)p.k_codes, (const uint8_t*)p.v_codes}, {(const uint8_t*)p.k_scale, (const uint8_t*)p.v_scale}, {k_out, v_out}, out_table,
                slot_ids, seq_ends, {p.page_table, p.slots, p.table_stride, p.pages}, p.kv_heads, p.head_dim, pages, whole ? 1 : 0, cu_seqlens, skip_new,
-               attend ? 1 : 0, attend ? window : 0, error_word()};
+               attend ? 1 : 0, attend ? window : 0, error};
     note_launch();
     auto kernel = dt == F32 ? (p.fmt == QUANT_FP8 ? kv_quant_load_kernel<float, QUANT_FP8> : kv_quant_load_kernel<float, QUANT_INT8>)
                             : (p.fmt == QUANT_FP8 ? kv_quant_load_kernel<__nv_bfloat16, QUANT_FP8> : kv_quant_load_kernel<__nv_bfloat16, QUANT_INT8>);

@@ -187,14 +187,14 @@ class Ops:
             raise KernelError("the record of an 8-bit cache's pools is laid out differently in the library")
         # (with the argument types known, a call takes plain numbers as addresses)
         addr, num, big, real = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
-        self.lib.sm_kv_quant_store.argtypes = [addr] * 3 + [num] * 2 + [addr] * 5
-        self.lib.sm_kv_quant_load.argtypes = [addr, num, num] + [addr] * 5 + [num, num, addr, num, num, num, addr]
-        self.lib.sm_attention_quant.argtypes = [addr] * 3 + [num, num, real, num] + [addr] * 3 + [num] * 5 + [addr, big, addr]
+        self.lib.sm_kv_quant_store.argtypes = [addr] * 3 + [num] * 2 + [addr] * 6
+        self.lib.sm_kv_quant_load.argtypes = [addr, num, num] + [addr] * 5 + [num, num, addr, num, num, num, addr, addr]
+        self.lib.sm_attention_quant.argtypes = [addr] * 3 + [num, num, real, num] + [addr] * 3 + [num] * 5 + [addr, big, addr, addr]
         self.lib.sm_attention_quant_supports.argtypes = [num, num, num, big]
         self.lib.sm_attention_quant_workspace.argtypes, self.lib.sm_attention_quant_workspace.restype = [num] * 4, big
         self.lib.sm_attention_chunk_supports.argtypes = [num, num, num, big, num, num]
         self.lib.sm_attention_chunk_workspace.argtypes, self.lib.sm_attention_chunk_workspace.restype = [num] * 3, big
-        self.lib.sm_attention_chunk.argtypes = [addr, addr] + [num] * 5 + [real, num, addr, addr, num, addr, addr, num, num, addr, big, addr]
+        self.lib.sm_attention_chunk.argtypes = [addr, addr] + [num] * 5 + [real, num, addr, addr, num, addr, addr, num, num, addr, big, addr, addr]
         self._quant_plans: dict = {}      # by sizes alone
         fast = kernels == "fast"
         self.kernels = kernels
@@ -225,6 +225,7 @@ class Ops:
         self.quant_cluster: Optional[int] = None
         self.skinny_single_round_above_8 = True
         self.error_flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+        self._error_address = self.error_flag.data_ptr()
         self.lib.sm_set_error_word.restype = None
         self.lib.sm_set_error_word(_ptr(self.error_flag))
         # scratch of the greedy choice: one word per row, all ones when idle, and arrival counters
@@ -686,7 +687,7 @@ class Ops:
         rows = (torch.empty_like(k_packed), torch.empty_like(v_packed)) if want_rows else None
         self._check(self.lib.sm_kv_quant_store(
             layer.address, k_packed.data_ptr(), v_packed.data_ptr(), _dt(k_packed), step.n_tokens, rows[0].data_ptr() if rows else None,
-            rows[1].data_ptr() if rows else None, positions.data_ptr(), token_slot.data_ptr(), _raw_stream()))
+            rows[1].data_ptr() if rows else None, positions.data_ptr(), token_slot.data_ptr(), self._error_address, _raw_stream()))
         return rows
 
     def kv_quant_load(self, step, cache, dtype: torch.dtype):
@@ -711,7 +712,8 @@ class Ops:
         table = cache.page_table.new_empty((layer.slots, pages))
         self._check(self.lib.sm_kv_quant_load(
             layer.address, F32 if dtype is torch.float32 else BF16, step.n_seqs, slot_ids.data_ptr(), seq_ends.data_ptr(), k.data_ptr(),
-            v.data_ptr(), table.data_ptr(), pages, whole, cu.data_ptr(), skip_new, attend, window, _raw_stream()))
+            v.data_ptr(), table.data_ptr(), pages, whole, cu.data_ptr(), skip_new, attend, window, self._error_address,
+            _raw_stream()))
         return k, v, table
 
     def attention_quant(self, q, step, scale, window, cache):
@@ -747,14 +749,15 @@ class Ops:
             workspace = q.new_empty((floats,), dtype=torch.float32) if floats else None
             self._check(self.lib.sm_attention_quant(
                 layer.address, q.data_ptr(), out.data_ptr(), n_seqs, heads, scale, window, slot_ids.data_ptr(), seq_ends.data_ptr(), cu.data_ptr(),
-                longest, limit, row_tiles, pairs, cluster, workspace.data_ptr() if floats else None, floats, _raw_stream()))
+                longest, limit, row_tiles, pairs, cluster, workspace.data_ptr() if floats else None, floats, self._error_address, _raw_stream()))
         if blocks:
             # many tokens: the pages are read back as bfloat16 once (exactly), and the tcgen05 kernel reads those
             k, v, table = self._quant_load(step, layer, cache, dtype, False, limit, True, window)
             workspace = q.new_empty((chunk_floats,), dtype=torch.float32)
             self._check(self.lib.sm_attention_chunk(
                 q.data_ptr(), out.data_ptr(), step.n_tokens, n_seqs, heads, kv_heads, head_dim, scale, window, k.data_ptr(), v.data_ptr(),
-                table.shape[1], seq_ends.data_ptr(), cu.data_ptr(), limit, blocks, workspace.data_ptr(), chunk_floats, _raw_stream()))
+                table.shape[1], seq_ends.data_ptr(), cu.data_ptr(), limit, blocks, workspace.data_ptr(), chunk_floats, self._error_address,
+                _raw_stream()))
         return out
 
     def _quant_plan(self, lens, max_len, heads, layer, dtype, window):

@@ -1,5 +1,7 @@
 """The calls on the 8-bit cache that are easy to get wrong: every way of sharing the work out, many sequences, pools past
 2^32 bytes, queries that are not numbers, graphs and streams side by side, and places that do not exist."""
+import ctypes
+
 import pytest
 import torch
 
@@ -219,3 +221,22 @@ def test_scales_that_are_refused(ops):
     for scale in (0.0, -0.125, float("nan"), float("inf")):
         with pytest.raises(KernelError, match="a scale of"):
             ops.attention_quant(q, step, scale, 0, layer)
+
+
+def test_what_went_wrong_is_told_to_the_instance_that_was_called(ops):
+    """Another instance of the kernel library, made later, does not receive what this one's calls have to say."""
+    from smolmoe_c99_b200.kernels import KernelError, Ops
+    later = Ops("plain")
+    layer = make_layer("fp8", 2, 64, [200], [0])
+    fill(ops, layer, [0], [200], 78)
+    q, k = _randn((1, 14, 64), 79).bfloat16(), _randn((1, 2, 64), 80).bfloat16()
+    step = pack_step([0], [199], [[0]], torch.device("cuda"))
+    layer.page_table[0, 3] = -1
+    for call, name in ((lambda: ops.kv_quant_store(k, k, step, layer), "kv_quant_store"),
+                       (lambda: ops.kv_quant_load(step, layer, torch.bfloat16), "kv_quant_load"),
+                       (lambda: ops.attention_quant(q, step, 0.125, 0, layer), "attention_quant")):
+        call()
+        later.check_error_flag()
+        with pytest.raises(KernelError, match=f"{name} met"):
+            ops.check_error_flag()
+    ops.lib.sm_set_error_word(ctypes.c_void_p(ops._error_address))       # (as it was before `later`)
