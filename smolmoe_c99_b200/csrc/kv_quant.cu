@@ -17,19 +17,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-}
 __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
     *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
     *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
@@ -57,38 +44,74 @@ struct StoreArgs {
     int* error;
 };
 
-// One row per group of `lanes` threads (a power of two, at least head_dim / 8); blockIdx.y: keys or values. A thread does
-// kStoreRows rows, so that as many loads are under way together.
+// One row per group of threads (a power of two of them), V values each; blockIdx.y: keys or values. A thread does kStoreRows
+// rows, so that as many loads are under way together. What a row costs whatever its length (its token, its page, its
+// place) weighs as much as 16 values do, so a thread takes 16 of bfloat16 where the head size allows (prompts of 22,000 tokens of 4
+// heads of 128 written, and 61,000 positions read back: 48 us, with 8 values a thread 55), and 8 of float (prompts of up to 2,000
+// tokens: 8.4 us, with 16 9.0).
 constexpr int kStoreRows = 2;
 
-template <typename T, int FMT>
-__global__ void __launch_bounds__(kThreads) kv_quant_store_kernel(StoreArgs a, int lanes) {
+// V values of a row as they were loaded: 16-byte pieces of a type.
+template <typename T, int V>
+struct Piece {
+    static constexpr int N = V * sizeof(T) / 16;
+    uint4 raw[N];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) raw[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ uint32_t word(int i) const {
+        const uint4& r = raw[i / 4];
+        return i % 4 == 0 ? r.x : i % 4 == 1 ? r.y : i % 4 == 2 ? r.z : r.w;
+    }
+    __device__ __forceinline__ float value(int i) const {
+        if (sizeof(T) == 4) return __uint_as_float(word(i));
+        return i % 2 == 0 ? __uint_as_float(word(i / 2) << 16) : __uint_as_float(word(i / 2) & 0xffff0000u);
+    }
+    // Magnitudes as whole numbers, whose order is theirs: of float one a word, of bfloat16 two.
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return sizeof(T) == 4 ? max(a, b) : __vmaxu2(a, b); }
+    __device__ __forceinline__ uint32_t largest() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < N * 4; ++i) m = larger(m, word(i) & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu));
+        return m;
+    }
+    static __device__ __forceinline__ uint32_t as_float_bits(uint32_t m) { return sizeof(T) == 4 ? m : max(m & 0xffff0000u, m << 16); }
+};
+
+template <typename T, int FMT, int V>
+__global__ void __launch_bounds__(kThreads) kv_quant_store_kernel(StoreArgs a, int log_lanes, unsigned per_kv_head) {
     pdl_wait();                  // the rows come from the kernel before
     pdl_launch_dependents();
-    const int per_block = kThreads / lanes;
-    const unsigned row0 = blockIdx.x * (per_block * kStoreRows) + threadIdx.x / lanes;
-    const int part = threadIdx.x % lanes;
+    const int lanes = 1 << log_lanes, per_block = kThreads >> log_lanes;
+    const unsigned row0 = blockIdx.x * (per_block * kStoreRows) + (threadIdx.x >> log_lanes);
+    const int part = threadIdx.x & (lanes - 1);
     // (chosen, not indexed: an index that is not a constant would put the arguments into local memory)
     const bool keys = blockIdx.y == 0;
     const T* packed = (const T*)(keys ? a.packed[0] : a.packed[1]);
     T* rows = (T*)(keys ? a.rows[0] : a.rows[1]);
     uint8_t* codes = keys ? a.codes[0] : a.codes[1];
     uint8_t* scales = keys ? a.scales[0] : a.scales[1];
-    float x[kStoreRows][8];
+    Piece<T, V> x[kStoreRows];
     int at_token[kStoreRows], at_slot[kStoreRows], kv_head[kStoreRows];
     bool mine[kStoreRows];
 #pragma unroll
     for (int u = 0; u < kStoreRows; ++u) {
         const unsigned row = row0 + u * per_block;
         const bool live = row < a.rows_of_each;
-        mine[u] = live && part * 8 < a.head_dim;
-        const unsigned t = live ? row / (unsigned)a.kv_heads : 0;
-        kv_head[u] = (int)(row - t * (unsigned)a.kv_heads);
+        mine[u] = live && part * V < a.head_dim;
+        x[u].clear();
+        if (mine[u]) x[u].load(packed + (size_t)row * a.head_dim + part * V);
+        // row / kv_heads, by the floor of 2^32 / kv_heads (2^32 - 1 for one head): at most one too few
+        unsigned t = live ? __umulhi(row, per_kv_head) : 0, h = live ? row - t * (unsigned)a.kv_heads : 0;
+        if (h >= (unsigned)a.kv_heads) { ++t; h -= (unsigned)a.kv_heads; }
+        kv_head[u] = (int)h;
         at_token[u] = a.positions[t];
         at_slot[u] = a.token_slot[t];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
-        if (mine[u]) load8(packed + (size_t)row * a.head_dim + part * 8, x[u]);
     }
     int page[kStoreRows];
 #pragma unroll
@@ -96,36 +119,37 @@ __global__ void __launch_bounds__(kThreads) kv_quant_store_kernel(StoreArgs a, i
 #pragma unroll
     for (int u = 0; u < kStoreRows; ++u) {
         const unsigned row = row0 + u * per_block;
-        uint32_t amax = 0;
+        uint32_t m = x[u].largest();
+        for (int o = lanes >> 1; o > 0; o >>= 1) m = Piece<T, V>::larger(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (!mine[u]) continue;
+        const int byte = scale_byte<FMT>(Piece<T, V>::as_float_bits(m));
+        uint32_t code[V / 4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(x[u][i]) & 0x7fffffffu);
+        for (int i = 0; i < V / 4; ++i) code[i] = 0;
+        if (byte != kNoScale) {
+            const float up = power_of_two(127 - byte);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const uint32_t other = __shfl_xor_sync(0xffffffffu, amax, o);
-            if (o < lanes) amax = max(amax, other);
+            for (int i = 0; i < V / 4; ++i)
+                code[i] = encode4<FMT>(x[u].value(4 * i) * up, x[u].value(4 * i + 1) * up, x[u].value(4 * i + 2) * up, x[u].value(4 * i + 3) * up);
         }
-        if (mine[u]) {
-            const int byte = scale_byte<FMT>(amax);
-            uint32_t lo = 0, hi = 0;
-            if (byte != kNoScale) {
-                const float up = power_of_two(127 - byte);
-                lo = encode4<FMT>(x[u][0] * up, x[u][1] * up, x[u][2] * up, x[u][3] * up);
-                hi = encode4<FMT>(x[u][4] * up, x[u][5] * up, x[u][6] * up, x[u][7] * up);
-            }
-            if (page[u] >= 0) {
-                const size_t cell = ((size_t)page[u] * a.kv_heads + kv_head[u]) * kPageSize + at_token[u] % kPageSize;
-                *reinterpret_cast<uint2*>(codes + cell * a.head_dim + part * 8) = make_uint2(lo, hi);
-                if (part == 0) scales[cell] = (uint8_t)byte;
-            } else if (a.error) {
-                atomicExch(a.error, kBadPlaceInStore);
-            }
-            if (rows != nullptr) {
-                const float scale = scale_of(byte);
+        if (page[u] >= 0) {
+            const size_t cell = ((size_t)page[u] * a.kv_heads + kv_head[u]) * kPageSize + at_token[u] % kPageSize;
+            uint8_t* dst = codes + cell * a.head_dim + part * V;
+            if (V == 16) *reinterpret_cast<uint4*>(dst) = make_uint4(code[0], code[1], code[V / 4 - 2], code[V / 4 - 1]);
+            else *reinterpret_cast<uint2*>(dst) = make_uint2(code[0], code[1]);
+            if (part == 0) scales[cell] = (uint8_t)byte;
+        } else if (a.error) {
+            atomicExch(a.error, kBadPlaceInStore);
+        }
+        if (rows != nullptr) {
+            const float scale = scale_of(byte);
+#pragma unroll
+            for (int i = 0; i < V / 8; ++i) {
                 float v[4], w[4];
-                decode4<FMT>(lo, v);
-                decode4<FMT>(hi, w);
+                decode4<FMT>(code[2 * i], v);
+                decode4<FMT>(code[2 * i + 1], w);
                 const float y[8] = {v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale, w[0] * scale, w[1] * scale, w[2] * scale, w[3] * scale};
-                store8(rows + (size_t)row * a.head_dim + part * 8, y);
+                store8(rows + (size_t)row * a.head_dim + part * V + 8 * i, y);
             }
         }
     }
@@ -229,16 +253,22 @@ void kv_quant_store(const QuantPools& p, const void* k_packed, const void* v_pac
     if (((uintptr_t)k_packed | (uintptr_t)v_packed | (uintptr_t)k_rows | (uintptr_t)v_rows) & 15)
         throw std::invalid_argument("kv_quant_store: rows must be 16-byte aligned");
     if ((long long)T * p.kv_heads > 0x7fffffffll) throw std::invalid_argument("kv_quant_store: more than 2^31 rows in one call");
-    int lanes = 1;
-    while (lanes * 8 < p.head_dim) lanes *= 2;
+    const int each = dt == F32 || p.head_dim % 16 || ((uintptr_t)p.k_codes | (uintptr_t)p.v_codes) & 15 ? 8 : 16;      // values a thread
+    int log_lanes = 0;
+    while ((each << log_lanes) < p.head_dim) ++log_lanes;
     StoreArgs a{{k_packed, v_packed}, {k_rows, v_rows}, {(uint8_t*)p.k_codes, (uint8_t*)p.v_codes}, {(uint8_t*)p.k_scale, (uint8_t*)p.v_scale},
                 positions, token_slot, {p.page_table, p.slots, p.table_stride, p.pages}, p.kv_heads, p.head_dim, (unsigned)(T * p.kv_heads), error};
-    const unsigned per_block = kThreads / lanes * kStoreRows;
+    const unsigned per_block = (kThreads >> log_lanes) * kStoreRows;
     const dim3 grid((a.rows_of_each + per_block - 1) / per_block, 2);
+    const unsigned per_kv_head = p.kv_heads == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / (unsigned)p.kv_heads);
     note_launch();
-    auto kernel = dt == F32 ? (p.fmt == QUANT_FP8 ? kv_quant_store_kernel<float, QUANT_FP8> : kv_quant_store_kernel<float, QUANT_INT8>)
-                            : (p.fmt == QUANT_FP8 ? kv_quant_store_kernel<__nv_bfloat16, QUANT_FP8> : kv_quant_store_kernel<__nv_bfloat16, QUANT_INT8>);
-    launch_kernel("kv_quant_store", kernel, grid, dim3(kThreads), 0, stream, 1, dependent_launch_enabled(), a, lanes);
+    auto launch = [&](auto kernel) {
+        launch_kernel("kv_quant_store", kernel, grid, dim3(kThreads), 0, stream, 1, dependent_launch_enabled(), a, log_lanes, per_kv_head);
+    };
+    auto of_type = [&](auto fp8, auto int8) { p.fmt == QUANT_FP8 ? launch(fp8) : launch(int8); };
+    if (dt == F32) of_type(kv_quant_store_kernel<float, QUANT_FP8, 8>, kv_quant_store_kernel<float, QUANT_INT8, 8>);
+    else if (each == 16) of_type(kv_quant_store_kernel<__nv_bfloat16, QUANT_FP8, 16>, kv_quant_store_kernel<__nv_bfloat16, QUANT_INT8, 16>);
+    else of_type(kv_quant_store_kernel<__nv_bfloat16, QUANT_FP8, 8>, kv_quant_store_kernel<__nv_bfloat16, QUANT_INT8, 8>);
 }
 
 void kv_quant_load(const QuantPools& p, DType dt, int n_seqs, const int32_t* slot_ids, const int32_t* seq_ends, void* k_out, void* v_out,
