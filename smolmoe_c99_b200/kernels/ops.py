@@ -780,12 +780,16 @@ class Ops:
             return None
         group, limit, blocks, chunk_floats = heads // kv_heads, max(lens), 0, 0
         # Sequences that bring up to this many tokens attend straight from the codes, the others through pages read back and
-        # the tcgen05 kernel. Measured on a B200, us a call, codes against pages: 14 heads on 2 of 64, 32 tokens onto 8,000
-        # 29 / 36, 64 onto 8,000 22 / 36, 64 onto 32,000 62 / 60; 28 heads on 4 of 128, 32 onto 8,000 33 / 45, 64 onto 8,000
-        # 52 / 48, 32 onto 32,000 89 / 85, 64 onto 32,000 165 / 90.
+        # the tcgen05 kernel. Measured on a B200, us a call, codes against pages: 14 heads on 2 of 64, 64 tokens onto 1,000
+        # 10 / 18, 32 onto 8,000 22 / 21, 32 onto 32,000 52 / 31; 28 heads on 4 of 128, 32 onto 1,000 12 / 26, 16 onto 8,000
+        # 22 / 28, 32 onto 8,000 36 / 33, 16 onto 32,000 58 / 52, 32 onto 32,000 95 / 58. So: rows of queries (tokens times
+        # heads of a group) against the positions they see, and a few rows whatever those are (reading pages back costs the
+        # more the longer the sequence is).
         few_tokens = self.quant_rows_tokens
         if few_tokens is None:
-            few_tokens = max(1, (448 if head_dim <= 64 else 256) // group)
+            most, rows_by_positions = (448, 2_240_000) if head_dim <= 64 else (256, 1_600_000)
+            seen = max_len if not window else min(max_len, window + most // group)
+            few_tokens = max(1, min(most, max(96, rows_by_positions // seen)) // group)
         if limit > few_tokens and self.use_tcgen05_attention:
             many = 2 * (128 // group)     # tokens of a block of the tcgen05 kernel
             blocks = sum(-(-n // many) for n in lens if n > few_tokens)
