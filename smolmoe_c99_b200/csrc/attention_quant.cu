@@ -22,10 +22,12 @@
 //   V: ldmatrix of 8-bit 16 x 16 blocks, transposed: four neighbouring rows (positions) of one dimension.
 // The rows that a matrix names are permuted by row_position() so that both kinds of read are free of bank conflicts and P
 // needs no exchange beyond movmatrix.
-// Scales: the exponent of a key's row multiplies its scores; that of a value's row goes into the weight. Weights are half
-// precision: P * 2^(e - E + 15) with E the largest exponent so far, so the largest weight is 2^15 and what is lost lies 2^40
-// below it. The rows of queries are scaled by powers of two to half precision, which holds all 8 bits of a bfloat16.
-// Sums, maxima and accumulators are float.
+// Scales: the exponent of a key's row multiplies its scores; that of a value's row goes into the weight, P * 2^e. Weights are
+// half precision, so each row of queries puts its own by a power of two that brings the largest of those it has added up to
+// between 2^8 and 2^15: steps of half precision end at 2^-24, so what a weight may lose lies 2^33 below the row's own largest. What a
+// row does not see, and value rows that have no weight in it, do not count. The rows of queries are scaled by powers of two to
+// half precision, which holds all 8 bits of a bfloat16. Sums, maxima and accumulators are float. A row's reference for P is its
+// largest score rounded up to a whole power of two, so that nothing is rounded when it moves.
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -195,6 +197,11 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 // 2, 3, 10, 11, and the other eight).
 __device__ __forceinline__ int row_position(int r) { return r < 8 ? r : 8 + ((r - 8) ^ 4); }
 
+// Weights go to half precision as at most 2^15 (its largest number lies just below 2^16); where one would be larger, they are
+// put anew with the largest below 2^(15 - kSlack), so that the weights of the tiles to come rarely need that again. A weight of 1
+// with the least scale that a row can have needs 2^kMostShift to get there: none needs more.
+constexpr int kSlack = 6, kMostShift = 15 - kLeastExponent;
+
 // What a warp knows of the pair it works on, and what it has added up. NB: blocks of 64 of the head dimension; NHT: tiles
 // of 8 rows of queries; BOX: head_dim is 64 * NB. A thread holds, of each tile of rows, rows 2 q4 and 2 q4 + 1 (q4 = lane % 4)
 // and, of each 16 positions or dimensions, two (of positions: row_position(g) and row_position(g + 8), g = lane / 4).
@@ -205,7 +212,8 @@ struct Rows {
     float q_scale[NHT][2];               // undoes the power of two, times scale * log2(e)
     float ot[CH][NHT][4];
     float run_m[NHT][2], run_l[NHT][2];
-    int top_exponent;                    // E, as a byte; 0: none yet
+    int shift[NHT][2];                   // 2^shift takes weights to half precision; what has been added up has that factor too
+    int most_byte;                       // no weight passes 2^15 where the value row's byte is at most this, whatever its score
     int first_pos, tokens, lowest;       // position of the first row's token, tokens, the lowest position that any sees
     uint32_t k_lane, v_lane;             // offsets in a tile of what this lane names in an ldmatrix of keys, of values
 
@@ -216,7 +224,6 @@ struct Rows {
         first_pos = first;
         tokens = n_tokens;
         lowest = a.window > 0 ? max(0, first - a.window + 1) : 0;
-        top_exponent = 0;
         // the row this lane names of 16 keys, and of a 16 x 16 block of values; lanes from 16 on name the next piece
         const int which = lane >> 4, at = lane & 15;
         const int k_row = row_position((lane & 7) + ((lane >> 3) & 1) * 8), v_row = row_position(2 * (at >> 2) + (at & 1) + ((at >> 1) & 1) * 8);
@@ -252,8 +259,10 @@ struct Rows {
                 q_scale[nh][e] = __shfl_sync(0xffffffffu, down, (2 * q4 + e) * 4);
                 run_m[nh][e] = -CUDART_INF_F;
                 run_l[nh][e] = 0.f;
+                shift[nh][e] = kMostShift;
             }
         }
+        most_byte = 15 + 127 - kMostShift;
     }
 
     // Shared-memory offset of a piece of 16 bytes of a row of a tile.
@@ -347,8 +356,8 @@ struct Rows {
                     }
                 }
         }
-        // whether any score exceeds its row's maximum so far
-        bool moved = top > top_exponent;
+        // whether any score exceeds its row's reference, or any weight may pass half precision
+        bool moved = top > most_byte;
 #pragma unroll
         for (int nh = 0; nh < NHT; ++nh)
 #pragma unroll
@@ -358,45 +367,43 @@ struct Rows {
                 for (int mt = 1; mt < MT; ++mt) x = fmax3(x, st[mt][nh][e], st[mt][nh][e + 2]);
                 moved |= x > run_m[nh][e];
             }
-        if (__any_sync(0xffffffffu, moved)) {
-            // a larger maximum or exponent: what has been added up is put on the new footing (most tiles of a long
-            // sequence bring neither, and then no maximum is looked for among the threads)
-            top = max((int)__reduce_max_sync(0xffffffffu, (unsigned)top), top_exponent);
-            const float less = top_exponent == 0 ? 0.f : power_of_two(-min(top - top_exponent, 126));
-            top_exponent = top;
+        // (most tiles of a long sequence bring neither, and then no maximum is looked for among the threads)
+        moved = __any_sync(0xffffffffu, moved);
+        int over[NHT][2];        // what has been added up is to be put smaller by 2^over
+        if (moved) {
+            // A larger reference: what has been added up stays as it is, weights to come are put larger by as much as the
+            // reference has grown, up to kMostShift.
+            bool scaled = false;
+            int largest = kLeastExponent;
 #pragma unroll
-            for (int nh = 0; nh < NHT; ++nh) {
-                float f[2];
+            for (int nh = 0; nh < NHT; ++nh)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float x = run_m[nh][e];
+                    float x = st[0][nh][e];
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) x = fmax3(x, st[mt][nh][e], st[mt][nh][e + 2]);
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    const float by = x == -CUDART_INF_F ? 1.f : ex2_approx(run_m[nh][e] - x);
+                    x = fmaxf(run_m[nh][e], ceilf(max_of_row(x)));
+                    const int grown = (int)fminf(x - run_m[nh][e], 1000.f);      // (the first reference: 1000)
                     run_m[nh][e] = x;
-                    run_l[nh][e] *= by;
-                    f[e] = by * less;
+                    run_l[nh][e] *= power_of_two_or_zero(-grown);
+                    over[nh][e] = max(shift[nh][e] + grown - kMostShift, 0);
+                    shift[nh][e] += grown - over[nh][e];
+                    scaled |= over[nh][e] > 0;
+                    largest = max(largest, shift[nh][e]);
                 }
-#pragma unroll
-                for (int c = 0; c < CH; ++c) { ot[c][nh][0] *= f[0]; ot[c][nh][1] *= f[1]; ot[c][nh][2] *= f[0]; ot[c][nh][3] *= f[1]; }
-            }
+            most_byte = 15 + 127 - __reduce_max_sync(0xffffffffu, largest);
+            moved = __any_sync(0xffffffffu, scaled || top > most_byte);
         }
-        // P = 2^(score - maximum), summed up
+        // P = 2^(score - reference), summed up, and P * 2^e
         float ref[NHT][2];
 #pragma unroll
         for (int nh = 0; nh < NHT; ++nh)
 #pragma unroll
             for (int e = 0; e < 2; ++e) ref[nh][e] = run_m[nh][e] == -CUDART_INF_F ? 0.f : run_m[nh][e];
-        const int shift = 142 - top_exponent;        // 127 + 15 - E
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            // the weights P * 2^(e - E + 15)
             const int b0 = lds_u8(ks_lo + KT + mt * 16), b1 = lds_u8(ks_hi + KT + mt * 16);
-            const float w0 = b0 == kNoScale ? CUDART_NAN_F : __int_as_float(max(b0 + shift, 0) << 23);
-            const float w1 = b1 == kNoScale ? CUDART_NAN_F : __int_as_float(max(b1 + shift, 0) << 23);
+            const float w0 = b0 == kNoScale ? CUDART_NAN_F : scale_of(b0), w1 = b1 == kNoScale ? CUDART_NAN_F : scale_of(b1);
 #pragma unroll
             for (int nh = 0; nh < NHT; ++nh)
 #pragma unroll
@@ -407,14 +414,42 @@ struct Rows {
                     st[mt][nh][e] = masked && st[mt][nh][e] == -CUDART_INF_F ? 0.f : v * ((e & 2) ? w1 : w0);
                 }
         }
+        if (moved) {
+            // the largest weights of the tile, exactly (a maximum passes over NaN); where one passes 2^15 the row's are put anew
+            int largest = kLeastExponent;
+#pragma unroll
+            for (int nh = 0; nh < NHT; ++nh) {
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) x = fmax3(x, st[mt][nh][e], st[mt][nh][e + 2]);
+                    x = max_of_row(x);
+                    const int power = (int)((__float_as_uint(x) + 0x7fffffu) >> 23) - 127;      // x is at most 2^power
+                    const int less = power + shift[nh][e] > 15 ? power + shift[nh][e] - (15 - kSlack) : 0;
+                    shift[nh][e] -= less;
+                    f[e] = power_of_two_or_zero(-(less + over[nh][e]));
+                    largest = max(largest, shift[nh][e]);
+                }
+#pragma unroll
+                for (int c = 0; c < CH; ++c) { ot[c][nh][0] *= f[0]; ot[c][nh][1] *= f[1]; ot[c][nh][2] *= f[0]; ot[c][nh][3] *= f[1]; }
+            }
+            most_byte = 15 + 127 - __reduce_max_sync(0xffffffffu, largest);
+        }
+        float to_half[NHT][2];
+#pragma unroll
+        for (int nh = 0; nh < NHT; ++nh)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) to_half[nh][e] = power_of_two(shift[nh][e]);
         // ... as the B operand
         uint32_t pb[MT][NHT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int nh = 0; nh < NHT; ++nh) {
-                pb[mt][nh][0] = movmatrix_trans(pack_half2(st[mt][nh][0], st[mt][nh][1]));
-                pb[mt][nh][1] = movmatrix_trans(pack_half2(st[mt][nh][2], st[mt][nh][3]));
+                pb[mt][nh][0] = movmatrix_trans(pack_half2(st[mt][nh][0] * to_half[nh][0], st[mt][nh][1] * to_half[nh][1]));
+                pb[mt][nh][1] = movmatrix_trans(pack_half2(st[mt][nh][2] * to_half[nh][0], st[mt][nh][3] * to_half[nh][1]));
             }
         // O^T += V^T P^T
 #pragma unroll
@@ -436,8 +471,17 @@ struct Rows {
             }
     }
 
-    // The end: sums over the threads that share a row; what takes values out of units of 2^(E - 15).
-    __device__ __forceinline__ float end() {
+    // The largest among the threads that share a row.
+    static __device__ __forceinline__ float max_of_row(float x) {
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+    }
+    // 2^e for e <= 0, and 0 below float's least normal number
+    static __device__ __forceinline__ float power_of_two_or_zero(int e) { return __int_as_float(max(e + 127, 0) << 23); }
+
+    // The end: sums over the threads that share a row.
+    __device__ __forceinline__ void end() {
 #pragma unroll
         for (int nh = 0; nh < NHT; ++nh)
 #pragma unroll
@@ -448,7 +492,6 @@ struct Rows {
                 l += __shfl_xor_sync(0xffffffffu, l, 16);
                 run_l[nh][e] = l;
             }
-        return power_of_two(max(top_exponent - 127 - 15, -126));     // (no exponent yet: nothing was added up)
     }
 };
 
@@ -596,13 +639,14 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_cluster_kernel(co
 
     // ---- the warps' results put together, then the CTAs' --------------------------------------------------------------
     {
-        const float unit = state.end();
+        state.end();
         float* o = wo + (size_t)warp * R * LD;
 #pragma unroll
         for (int nh = 0; nh < NHT; ++nh)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int r = nh * 8 + 2 * q4 + e;
+                const float unit = power_of_two(-state.shift[nh][e]);
                 if (g == 0) { wm[warp * R + r] = state.run_m[nh][e]; wl[warp * R + r] = state.run_l[nh][e]; }
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
@@ -745,7 +789,7 @@ __global__ void __launch_bounds__(line_warps(NHT) * 32, 1) attention_quant_line_
             u = part_end;
             continue;
         }
-        const float unit = state.end();
+        state.end();
         float* part = a.parts + ((size_t)number * 2 + (begins ? 1 : 0)) * R * LD;
 #pragma unroll
         for (int nh = 0; nh < NHT; ++nh)
@@ -753,6 +797,7 @@ __global__ void __launch_bounds__(line_warps(NHT) * 32, 1) attention_quant_line_
             for (int e = 0; e < 2; ++e) {
                 const int r = nh * 8 + 2 * q4 + e;
                 if (r >= rows) continue;
+                const float unit = power_of_two(-state.shift[nh][e]);
                 if (whole) {
                     __nv_bfloat16* dst = a.out + ((size_t)(first_token + r / group) * a.heads + (size_t)kvh * group + r % group) * hd;
                     const float by = unit / state.run_l[nh][e];

@@ -1,0 +1,101 @@
+"""Calls on the 8-bit cache at the ends of what they take: values of very unequal size, long chunks, many sequences, lengths and
+windows at the borders of their types."""
+import pytest
+import torch
+
+from smolmoe_c99_b200.engine.batch import pack_step
+from test_gpu_kv_quant import _randn, fill, held, make_layer, ops  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def row_by_row(layer, q, slots, starts, news, scale, window):
+    """The output in 64 bits and how far a kernel may be off, each row from what it sees alone. Half a step of the output (2^-8
+    for bfloat16); half a step of a bfloat16 weight (2^-8; half precision has 2^-11); what float sums of head-size products move
+    a score by, twice (numerator and denominator); 2^-18 for float sums of up to 2^5 parts of the weighted values. A half-precision
+    weight is P 2^e put between 2^8 and 2^15 for the row's largest (e the exponent of the value row's scale) and ends in steps
+    of 2^-24, so each of the n weights may be off by 2^-25 / 2^8 = 2^-33 of the largest P 2^e, and a value is a code of at most
+    448 (127) times 2^e, at most twice the largest magnitude of a row of that scale: 2^-32 of the largest P amax."""
+    heads, kv_heads = q.shape[1], layer.k_pool.shape[1]
+    hd = q.shape[2]
+    out, room = torch.empty(q.shape, dtype=torch.float64), torch.empty(q.shape, dtype=torch.float64)
+    qd, first = q.double().cpu(), 0
+    for slot, s, n in zip(slots, starts, news):
+        k, v = held(layer, "k", slot, s + n), held(layer, "v", slot, s + n)
+        for i in range(n):
+            lo = max(0, s + i - window + 1) if window else 0
+            for h in range(heads):
+                kh, vh, x = (t[lo:s + i + 1, h // (heads // kv_heads)] for t in (k, v, k))
+                x = qd[first + i, h]
+                p = torch.softmax(kh @ x * scale, 0)
+                moved = (hd + 8) * 2.0 ** -24 * float((kh.abs() @ x.abs()).max()) * scale
+                spread = p @ vh.abs()
+                lost = 2.0 ** -32 * len(p) * float((p * vh.abs().amax(-1)).max())
+                out[first + i, h] = p @ vh
+                room[first + i, h] = 2.0 ** -8 * out[first + i, h].abs() + (2.0 ** -8 + 2 * moved + 2.0 ** -18) * spread + lost
+        first += n
+    return out, room
+
+
+def check_rows(ops, layer, q, slots, starts, news, scale, window):
+    step = pack_step(slots, starts, [[0] * n for n in news], torch.device("cuda"))
+    got = ops.attention_quant(q, step, scale, window, layer).double().cpu()
+    ops.check_error_flag()
+    want, room = row_by_row(layer, q, slots, starts, news, scale, window)
+    off = (got - want).abs() / room
+    assert float(off.max()) <= 1.0, f"{float(off.max()):.3g} of what rounding can move"
+
+
+# ---- value rows of very unequal size ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("power", [30, 45, 90])
+@pytest.mark.parametrize("cluster,rows_tokens", [(None, 64), (0, 64), (4, 64), (None, 1)])
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(14, 2, 64), (8, 1, 128)])
+def test_large_values_that_a_row_does_not_see(ops, heads, kv_heads, hd, fmt, cluster, rows_tokens, power, monkeypatch):
+    """The last token of each chunk, and the position that leaves the window with the second, have values 2^power times the
+    others'."""
+    monkeypatch.setattr(ops, "quant_cluster", cluster)
+    monkeypatch.setattr(ops, "quant_rows_tokens", rows_tokens)
+    starts, news, slots, window = [70, 200], [4, 9], [1, 0], 50
+    ends = [s + n for s, n in zip(starts, news)]
+    layer = make_layer(fmt, kv_heads, hd, ends, slots)
+
+    def enlarge(v):
+        for base, s, n in ((0, starts[0], news[0]), (ends[0], starts[1], news[1])):
+            v[base + s + n - 1] *= 2.0 ** power
+            v[base + s - window + 1] *= 2.0 ** power
+        return v
+    fill(ops, layer, slots, ends, 90, v_of=enlarge)
+    q = _randn((sum(news), heads, hd), 91).bfloat16()
+    check_rows(ops, layer, q, slots, starts, news, hd ** -0.5, window)
+    check_rows(ops, layer, q, slots, starts, news, hd ** -0.5, 0)
+
+
+@pytest.mark.parametrize("power", [30, 45, 90])
+@pytest.mark.parametrize("cluster", [None, 0, 4])
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+def test_large_values_without_weight(ops, fmt, cluster, power, monkeypatch):
+    """Positions whose values are 2^power times the others' and whose scores lie 2^-140 and less below the largest, met before,
+    among and after the others; then scores that rise from position to position, with values that fall."""
+    monkeypatch.setattr(ops, "quant_cluster", cluster)
+    n, hd = 500, 64
+    layer = make_layer(fmt, 2, hd, [n], [0])
+    q = (_randn((1, 2, hd), 92).abs() + 0.5).bfloat16()
+
+    def keys(k):
+        k *= 0.25
+        for p in (0, 40, 255, 499):
+            k[p] = -8.0
+        return k
+
+    def values(v):
+        for p in (0, 40, 255, 499):
+            v[p] *= 2.0 ** power
+        return v
+    fill(ops, layer, [0], [n], 93, keys, values)
+    check_rows(ops, layer, q, [0], [n - 1], [1], 0.25, 0)
+    rise = torch.linspace(-10, 10, n, device="cuda").view(-1, 1, 1)
+    fall = torch.exp2(torch.linspace(power, -power, n, device="cuda")).view(-1, 1, 1)
+    fill(ops, layer, [0], [n], 94, lambda k: k * 0.1 + rise, lambda v: v * fall)
+    check_rows(ops, layer, q, [0], [n - 1], [1], 0.25, 0)
