@@ -731,6 +731,8 @@ class Ops:
         window = int(window or 0)
         if window < 0:
             raise KernelError(f"a window of {window} positions")
+        if window >= layer.table_stride * PAGE_SIZE:
+            window = 0      # (as wide as any sequence: everything is seen, and the kernels' 32-bit numbers need not hold it)
         if not 0 < scale < float("inf"):
             raise KernelError(f"a scale of {scale}: positive and finite expected")
         slot_ids, seq_ends, cu = step.slot_ids, step.seq_ends, step.cu_seqlens

@@ -99,3 +99,21 @@ def test_large_values_without_weight(ops, fmt, cluster, power, monkeypatch):
     fall = torch.exp2(torch.linspace(power, -power, n, device="cuda")).view(-1, 1, 1)
     fill(ops, layer, [0], [n], 94, lambda k: k * 0.1 + rise, lambda v: v * fall)
     check_rows(ops, layer, q, [0], [n - 1], [1], 0.25, 0)
+
+
+# ---- windows ------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows_tokens", [64, 1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_windows_wider_than_any_sequence_see_all(ops, dtype, rows_tokens, monkeypatch):
+    monkeypatch.setattr(ops, "quant_rows_tokens", rows_tokens)
+    starts, news, slots = [300, 128, 0], [1, 40, 3], [2, 0, 1]
+    ends = [s + n for s, n in zip(starts, news)]
+    layer = make_layer("fp8", 2, 64, ends, slots)
+    fill(ops, layer, slots, ends, 95)
+    q = _randn((sum(news), 4, 64), 96).to(dtype)
+    step = pack_step(slots, starts, [[0] * n for n in news], torch.device("cuda"))
+    want = ops.attention_quant(q, step, 0.125, 0, layer)
+    for window in (10_000, 2 ** 31 - 1, 2 ** 31 + 5, 2 ** 32 + 5, 2 ** 40):
+        assert torch.equal(ops.attention_quant(q, step, 0.125, window, layer), want), window
+    ops.check_error_flag()
