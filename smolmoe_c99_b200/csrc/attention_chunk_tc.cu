@@ -270,9 +270,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
         line.first[i] = first;
         line.start[i] = end - n;
         line.n[i] = n;
-        return n > a.skip_new && n <= end ? (n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens) : 0;
+        return n > a.skip_new && n <= end && end <= a.pages * kPageSize ? (n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens) : 0;
     });
-    // (lengths on the device that are not those on the host: nothing is done)
+    // (lengths on the device that are not those on the host, or pass the pages that were read back: nothing is done)
     const int blocks = line.blocks_before[a.seqs] == a.blocks ? a.blocks : 0;
     if (blocks == 0 && blockIdx.x == 0) {
         if (threadIdx.x == 0 && a.error) atomicExch(a.error, kBadPlaceInAttention);

@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(kThreads) kv_quant_load_kernel(LoadArgs a) {
         return;
     }
     if (which == 0 && threadIdx.x == 0) a.out_table[(size_t)slot * a.pages + page] = seq * a.pages + page;
+    if (end > a.pages * kPageSize && a.error && threadIdx.x == 0) atomicExch(a.error, kBadPlaceInLoad);       // (what does not fit is left out)
     const int live = min(end - page * kPageSize, kPageSize);      // positions of the page that the sequence holds
     if (live <= 0 && !a.whole) return;
     if (a.window > 0) {

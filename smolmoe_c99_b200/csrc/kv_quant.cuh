@@ -28,7 +28,8 @@ constexpr int kLeastExponent = -100;   // rows whose largest value is below abou
 constexpr int kNoScale = 255;
 
 // Codes in the library's error word for a slot, position or page that lies outside the page table or the pools: the access
-// is left out (rows are not written, or read as zeros). Attention also reports lengths that are not those of the host.
+// is left out (rows are not written, or read as zeros). Reading back also reports a sequence that is longer than the pages it reads,
+// attention lengths that are not those of the host.
 constexpr int kBadPlaceInStore = 31, kBadPlaceInLoad = 32, kBadPlaceInAttention = 33;
 
 // The page of a sequence's positions 64 * index .. 64 * index + 63, or -1 where there is none.

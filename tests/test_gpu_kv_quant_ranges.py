@@ -117,3 +117,30 @@ def test_windows_wider_than_any_sequence_see_all(ops, dtype, rows_tokens, monkey
     for window in (10_000, 2 ** 31 - 1, 2 ** 31 + 5, 2 ** 32 + 5, 2 ** 40):
         assert torch.equal(ops.attention_quant(q, step, 0.125, window, layer), want), window
     ops.check_error_flag()
+
+
+# ---- lengths ------------------------------------------------------------------------------------------------------------
+
+def test_lengths_on_the_device_past_the_hosts_bound_are_reported(ops, monkeypatch):
+    """Each sequence brings as many tokens as the host planned for, but is longer on the device than the longest that the host
+    knows of: the pages that were read back do not hold it."""
+    from smolmoe_c99_b200.kernels import KernelError
+    monkeypatch.setattr(ops, "quant_rows_tokens", 1)
+    news, starts, slots = [60, 70], [66, 200], [0, 1]
+    layer = make_layer("fp8", 2, 64, [600, 600], slots)
+    fill(ops, layer, slots, [600, 600], 97)
+    step = pack_step(slots, starts, [[0] * n for n in news], torch.device("cuda"))
+    q = _randn((sum(news), 14, 64), 98).bfloat16()
+    want = ops.attention_quant(q, step, 0.125, 0, layer)
+    ops.check_error_flag()
+    ends = step.seq_ends.clone()
+    step.seq_ends += 256
+    ops.attention_quant(q, step, 0.125, 0, layer)
+    with pytest.raises(KernelError, match="attention_quant met|kv_quant_load met"):
+        ops.check_error_flag()
+    ops.kv_quant_load(step, layer, torch.bfloat16)
+    with pytest.raises(KernelError, match="kv_quant_load met"):
+        ops.check_error_flag()
+    step.seq_ends.copy_(ends)
+    assert torch.equal(ops.attention_quant(q, step, 0.125, 0, layer), want)
+    ops.check_error_flag()
