@@ -901,31 +901,48 @@ struct LaunchSizes {
 };
 constexpr size_t kRoom = 226 * 1024;     // shared memory of an SM, less what the system and the static part take
 
+// Shared memory of a CTA: what it takes however many tiles are in flight (the step's sequences among it), and for one tile in
+// flight a warp (codes, exponents, a barrier).
+struct Smem {
+    size_t fixed, a_tile;
+    bool fits() const { return fixed + a_tile <= kRoom; }
+};
+Smem smem_of(int head_dim, int row_tiles, int seqs, int cluster) {
+    const bool box = head_dim == 64 || head_dim == 128;
+    const size_t R = 8 * row_tiles, LD = (head_dim <= 64 ? 64 : 128) + 4, warps = cluster ? kWarps : line_warps(row_tiles);
+    const size_t tile = cluster ? kClusterTile : line_tile(row_tiles);
+    return {(box ? 1024 : 0) + seq_table_bytes(seqs) + (cluster ? (kWarps * R * (LD + 2) + cluster * R * LD) * sizeof(float) : 0),
+            warps * (2 * tile * (head_dim + 1) + sizeof(uint64_t))};
+}
+
 template <int NB, int NHT, int FMT, bool BOX>
 void launch(AttnArgs a, const CUtensorMap& mk, const CUtensorMap& mv, const LaunchSizes& sizes, cudaStream_t stream) {
-    constexpr int HDP = NB * 64, R = 8 * NHT, LD = HDP + 4;
-    const size_t slot = (size_t)2 * a.tile * (a.head_dim + 1) + sizeof(uint64_t);      // codes, exponents, a barrier
-    const size_t table = (BOX ? 1024 : 0) + seq_table_bytes(a.seqs);
+    constexpr int HDP = NB * 64, R = 8 * NHT;
+    const Smem smem = smem_of(a.head_dim, NHT, a.seqs, a.cluster);
+    if (!smem.fits())
+        throw std::invalid_argument("attention_quant: " + std::to_string(a.seqs) + " sequences, head size " + std::to_string(a.head_dim) + ", " +
+                                    std::to_string(NHT) + " tiles of rows and clusters of " + std::to_string(a.cluster) +
+                                    " do not fit shared memory (attention_quant_fits)");
+    const int room_for = (int)((kRoom - smem.fixed) / smem.a_tile);                    // tiles in flight
     if (a.cluster) {
-        const size_t fixed = table + ((size_t)kWarps * R * (LD + 2) + (size_t)a.cluster * R * LD) * sizeof(float);
         // as many tiles in flight as a warp gets, at most what is left
         const int tiles = ((sizes.max_len + a.tile - 1) / a.tile + 1 + a.cluster - 1) / a.cluster;
-        a.stages = std::max(1, std::min({(tiles + kWarps - 1) / kWarps, kMaxStages, (int)((kRoom - fixed) / (kWarps * slot))}));
+        a.stages = std::max(1, std::min({(tiles + kWarps - 1) / kWarps, kMaxStages, room_for}));
         static bool prepared[kDevices] = {};
         auto kernel = attention_quant_cluster_kernel<NB, NHT, FMT, BOX>;
         allow_smem((const void*)kernel, prepared, kRoom);
         note_launch();
-        launch_kernel("attention_quant", kernel, dim3((unsigned)(sizes.pairs * a.cluster)), dim3(kWarps * 32), fixed + kWarps * a.stages * slot,
+        launch_kernel("attention_quant", kernel, dim3((unsigned)(sizes.pairs * a.cluster)), dim3(kWarps * 32), smem.fixed + a.stages * smem.a_tile,
                       stream, a.cluster, dependent_launch_enabled(), mk, mv, a);
         return;
     }
     constexpr int W = line_warps(NHT);
-    a.stages = std::max(1, std::min(kMaxStages, (int)((kRoom - table) / (W * slot))));
+    a.stages = std::min(kMaxStages, room_for);
     static bool prepared[kDevices] = {};
     auto kernel = attention_quant_line_kernel<NB, NHT, FMT, BOX>;
     allow_smem((const void*)kernel, prepared, kRoom);
     note_launch(2);
-    launch_kernel("attention_quant", kernel, dim3((unsigned)sm_count()), dim3(W * 32), table + W * a.stages * slot, stream, 1,
+    launch_kernel("attention_quant", kernel, dim3((unsigned)sm_count()), dim3(W * 32), smem.fixed + a.stages * smem.a_tile, stream, 1,
                   dependent_launch_enabled(), mk, mv, a);
     auto join = [&](auto kernel, int P) {
         const int rows_of_cta = join_warps(P) / P;
@@ -960,6 +977,11 @@ void launch_fmt(const AttnArgs& a, int row_tiles, const CUtensorMap& mk, const C
 bool attention_quant_supports(int heads, int kv_heads, int head_dim, long long pool_pages) {
     return head_dim % 16 == 0 && head_dim >= 16 && head_dim <= 128 && kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= 16 &&
            pool_pages > 0 && pool_pages * kv_heads * kPageSize < (1ll << 31);
+}
+
+// Whether that many sequences' numbers fit beside the tiles.
+bool attention_quant_fits(int head_dim, int row_tiles, int n_seqs, int cluster) {
+    return n_seqs <= kMaxSeqs && smem_of(head_dim, row_tiles, n_seqs, cluster).fits();
 }
 
 // Floats of workspace that a launch needs: the line's cuts and parts.

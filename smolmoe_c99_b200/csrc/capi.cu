@@ -257,6 +257,10 @@ SM_API int sm_attention_quant_supports(int heads, int kv_heads, int head_dim, lo
     return sm::attention_quant_supports(heads, kv_heads, head_dim, pool_pages) ? 1 : 0;
 }
 
+SM_API int sm_attention_quant_fits(int head_dim, int row_tiles, int n_seqs, int cluster) {
+    return sm::attention_quant_fits(head_dim, row_tiles, n_seqs, cluster) ? 1 : 0;
+}
+
 SM_API long long sm_attention_quant_workspace(int head_dim, int row_tiles, int pairs, int cluster) {
     return sm::attention_quant_workspace(head_dim, row_tiles, pairs, cluster);
 }

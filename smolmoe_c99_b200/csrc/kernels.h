@@ -274,8 +274,10 @@ void attention_decode(const void* q, void* out, int B, int heads, int kv_heads, 
 // host: max_len, a bound of the lengths; row_tiles (1, 2, or 4 for head sizes up to 64): tiles of 8 rows of queries (token,
 // head of a group) that are worked on together; pairs = kv_heads * blocks of such rows over the sequences; cluster: 1 to 8
 // CTAs work on a pair, or 0: one CTA an SM, whose warps share the tiles of all pairs out evenly, with a second kernel that
-// joins what they cut (workspace, attention_quant.cu). head_dim: multiples of 16 up to 128; at most 16 heads a kv head.
+// joins what they cut (workspace, attention_quant.cu). head_dim: multiples of 16 up to 128; at most 16 heads a kv head. The
+// sequences' numbers lie in shared memory: attention_quant_fits says whether there is room for them beside one tile a warp.
 bool attention_quant_supports(int heads, int kv_heads, int head_dim, long long pool_pages);
+bool attention_quant_fits(int head_dim, int row_tiles, int n_seqs, int cluster);
 long long attention_quant_workspace(int head_dim, int row_tiles, int pairs, int cluster);   // floats
 void attention_quant(const QuantPools& pools, const void* q, void* out, int n_seqs, int heads, float scale, int window, const int32_t* slot_ids,
                      const int32_t* seq_ends, const int32_t* cu_seqlens, int max_len, int most_new, int row_tiles, int pairs, int cluster,

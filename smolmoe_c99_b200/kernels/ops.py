@@ -191,6 +191,7 @@ class Ops:
         self.lib.sm_kv_quant_load.argtypes = [addr, num, num] + [addr] * 5 + [num, num, addr, num, num, num, addr, addr]
         self.lib.sm_attention_quant.argtypes = [addr] * 3 + [num, num, real, num] + [addr] * 3 + [num] * 5 + [addr, big, addr, addr]
         self.lib.sm_attention_quant_supports.argtypes = [num, num, num, big]
+        self.lib.sm_attention_quant_fits.argtypes = [num] * 4
         self.lib.sm_attention_quant_workspace.argtypes, self.lib.sm_attention_quant_workspace.restype = [num] * 4, big
         self.lib.sm_attention_chunk_supports.argtypes = [num, num, num, big, num, num]
         self.lib.sm_attention_chunk_workspace.argtypes, self.lib.sm_attention_chunk_workspace.restype = [num] * 3, big
@@ -806,12 +807,23 @@ class Ops:
         row_tiles = 1
         while 8 * row_tiles < min(max(few) * group, 32 if head_dim <= 64 else 16) or 8 * row_tiles < group:
             row_tiles *= 2
-        tokens = 8 * row_tiles // group
-        pairs = kv_heads * sum(-(-n // tokens) for n in few)
+        pairs_with = lambda row_tiles: kv_heads * sum(-(-n // (8 * row_tiles // group)) for n in few)
+        fits = lambda row_tiles, cluster: self.lib.sm_attention_quant_fits(head_dim, row_tiles, len(lens), cluster)
+        pairs = pairs_with(row_tiles)
         longest = max_len if not window else min(max_len, window + max(few))
-        if len(lens) > 4096 or pairs * (-(-longest // 32) + 1) >= 1 << 31:
-            return None                   # (more sequences, or tiles of the line, than the kernel counts)
+        if pairs * (-(-longest // 32) + 1) >= 1 << 31:
+            return None                   # (more tiles of the line than the kernel counts)
         cluster = self._quant_cluster(pairs, longest, head_dim)
+        # Thousands of sequences leave no room for their numbers beside the tiles: fewer CTAs a cluster, then the line; of that,
+        # two tiles of rows, which has 8 warps with tiles of 32 positions in place of 12 with 64 (2,000 sequences of 200 to 1,000
+        # on 4 kv heads of 128: 347 us, in clusters of one CTA 814).
+        while cluster and not fits(row_tiles, cluster):
+            cluster //= 2
+        if not fits(row_tiles, cluster) and row_tiles == 1:
+            row_tiles = 2
+            pairs = pairs_with(row_tiles)
+        if not fits(row_tiles, cluster):
+            return None
         floats = 0 if cluster else int(self.lib.sm_attention_quant_workspace(head_dim, row_tiles, pairs, 0))
         return limit, row_tiles, pairs, cluster, longest, floats, blocks, chunk_floats
 

@@ -144,3 +144,27 @@ def test_lengths_on_the_device_past_the_hosts_bound_are_reported(ops, monkeypatc
     step.seq_ends.copy_(ends)
     assert torch.equal(ops.attention_quant(q, step, 0.125, 0, layer), want)
     ops.check_error_flag()
+
+
+# ---- many sequences -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("heads,kv_heads,hd", [(2, 1, 128), (3, 1, 112), (9, 1, 128), (10, 1, 64)])
+@pytest.mark.parametrize("n,cluster", [(1607, 0), (1608, 0), (1608, None), (2888, 0), (4096, None), (4096, 0), (4096, 8)])
+def test_as_many_sequences_as_are_promised(ops, heads, kv_heads, hd, n, cluster, monkeypatch):
+    """Single tokens, each sequence's numbers beside the tiles in shared memory."""
+    monkeypatch.setattr(ops, "quant_cluster", cluster)
+    ends = [1 + (37 * i) % 90 for i in range(n)]
+    slots = [n - 1 - i for i in range(n)]
+    layer = make_layer("fp8", kv_heads, hd, ends, slots)
+    fill(ops, layer, slots, ends, 99)
+    q = _randn((n, heads, hd), 100).bfloat16()
+    step = pack_step(slots, [e - 1 for e in ends], [[0]] * n, torch.device("cuda"))
+    got = ops.attention_quant(q, step, hd ** -0.5, 0, layer)
+    ops.check_error_flag()
+    picked = [0, 1, 31, 32, 255, 256, 1023, 1024, n - 2, n - 1]
+    want, room = row_by_row(layer, q[picked], [slots[i] for i in picked], [ends[i] - 1 for i in picked], [1] * len(picked), hd ** -0.5, 0)
+    assert ((got[picked].double().cpu() - want).abs() <= room).all()
+    # (the others against the plain kernel: both are rounded to bfloat16 once, and the weights of one of them)
+    monkeypatch.setattr(ops, "use_fast_attention", False)
+    plain = ops.attention_quant(q, step, hd ** -0.5, 0, layer).double()
+    assert float((got.double() - plain).abs().max()) <= 2.0 ** -6 * float(plain.abs().max())
