@@ -48,6 +48,7 @@ class LayerCache:
     state: Optional[torch.Tensor] = None  # [slots, *shape]
     k_scale: Optional[torch.Tensor] = None  # an 8-bit cache: uint8 [pages, kv_heads, PAGE_SIZE]
     v_scale: Optional[torch.Tensor] = None
+    exclusive: bool = False               # no page is in the tables of two sequences (bounds what is read back of an 8-bit cache)
 
     def quant_layer(self) -> QuantLayer:
         """The pools of an 8-bit cache as the kernels take them, checked when first asked for (and again where a tensor of
@@ -221,7 +222,8 @@ class SequenceCache:
         if kind == "kv":
             g = self.groups[index]
             k_scale, v_scale = (None, None) if g.k_scale is None else (g.k_scale[layer], g.v_scale[layer])
-            return LayerCache("kv", g.k[layer], g.v[layer], g.table, g.ring, g.need.window, k_scale=k_scale, v_scale=v_scale)
+            return LayerCache("kv", g.k[layer], g.v[layer], g.table, g.ring, g.need.window, k_scale=k_scale, v_scale=v_scale,
+                              exclusive=True)
         if kind == "state":
             return LayerCache("state", state=self.states[index])
         return LayerCache("none")

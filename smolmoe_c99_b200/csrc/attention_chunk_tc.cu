@@ -67,7 +67,8 @@ struct ChunkArgs {
     __nv_bfloat16* out;                  // [T, heads, HD]
     const int32_t* seq_ends;             // [seqs] lengths after the step
     const int32_t* cu;                   // [seqs + 1]
-    int seqs, heads, kv_heads, window, skip_new, pages;    // pages: of each sequence in the pools
+    int seqs, heads, kv_heads, window, skip_new, pages;    // pages: of the longest sequence, at most
+    int room;                            // pages that were read back, at most
     int tile_tokens;                     // tokens of a tile of rows
     int blocks;                          // what the host says there are
     float scale_log2;
@@ -172,19 +173,20 @@ __device__ void prefix_sums(int* before, int n, F value) {
 struct Line {
     int *blocks_before, *tiles_before;   // [seqs + 1] blocks before a sequence, [blocks + 1] tiles of the line before a block
     int *first, *start, *n;              // [seqs] first new token among the step's, its position, new tokens
+    int* pages_before;                   // [seqs + 1] pages read back before those of a sequence
 };
 // One part of one pair: what a run holds of it.
 struct Part {
-    int seq, kvh, number, pair_at, tiles;      // the pair's number, its place on the line, its tiles of keys
+    int kvh, number, pair_at, tiles;      // the pair's number, its place on the line, its tiles of keys
     int kt0, n_kt;                             // the part's tiles of keys
-    int first_token, tokens, first_pos, last_page;
+    int first_token, tokens, first_pos;
+    int page0, last_page;                      // where page 0 of the sequence would lie; its last page
     int end;                                   // where the part ends on the line
 };
 __device__ __forceinline__ Part part_at(const ChunkArgs& a, const Line& line, int blocks, int u, int u_hi) {
     const int block_number = find_last(line.tiles_before, blocks, u), seq = find_last(line.blocks_before, a.seqs, block_number);
     const Block b = block_of(a, line.start[seq], line.n[seq], block_number - line.blocks_before[seq]);
     Part p;
-    p.seq = seq;
     p.kvh = (u - line.tiles_before[block_number]) / b.tiles;
     p.number = block_number * a.kv_heads + p.kvh;
     p.pair_at = line.tiles_before[block_number] + p.kvh * b.tiles;
@@ -195,6 +197,7 @@ __device__ __forceinline__ Part part_at(const ChunkArgs& a, const Line& line, in
     p.first_token = line.first[seq] + b.token0;
     p.tokens = b.tokens;
     p.first_pos = b.start + b.token0;
+    p.page0 = line.pages_before[seq] - pages_read(b.start, b.start + line.n[seq], a.window, a.pages).first;
     p.last_page = (b.start + line.n[seq] - 1) / kPageSize;
     return p;
 }
@@ -232,7 +235,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
     line.first = line.blocks_before + a.seqs + 1;
     line.start = line.first + a.seqs;
     line.n = line.start + a.seqs;
-    line.tiles_before = line.n + a.seqs;
+    line.pages_before = line.n + a.seqs;
+    line.tiles_before = line.pages_before + a.seqs + 1;
 
     const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads, tile_rows = a.tile_tokens * group;
     if (threadIdx.x == 0) {
@@ -272,8 +276,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
         line.n[i] = n;
         return n > a.skip_new && n <= end && end <= a.pages * kPageSize ? (n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens) : 0;
     });
+    prefix_sums(line.pages_before, a.seqs, [&](int i) {
+        return line.n[i] > a.skip_new ? pages_read(line.start[i], line.start[i] + line.n[i], a.window, a.pages).count : 0;
+    });
     // (lengths on the device that are not those on the host, or pass the pages that were read back: nothing is done)
-    const int blocks = line.blocks_before[a.seqs] == a.blocks ? a.blocks : 0;
+    const int blocks = line.blocks_before[a.seqs] == a.blocks && line.pages_before[a.seqs] <= a.room ? a.blocks : 0;
     if (blocks == 0 && blockIdx.x == 0) {
         if (threadIdx.x == 0 && a.error) atomicExch(a.error, kBadPlaceInAttention);
         for (int i = threadIdx.x; i < a.blocks * a.kv_heads; i += kThreads) a.cuts[i].tokens = 0;
@@ -309,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         // (a page the sequence does not hold is replaced by its last one: its rows are masked, but must be numbers)
-                        const int row = ((p.seq * a.pages + min(2 * (p.kt0 + t) + half, p.last_page)) * a.kv_heads + p.kvh) * kPageSize;
+                        const int row = ((p.page0 + min(2 * (p.kt0 + t) + half, p.last_page)) * a.kv_heads + p.kvh) * kPageSize;
 #pragma unroll
                         for (int d = 0; d < DB; ++d) tma_load_2d(dst + d * kBlockBytes + half * (kBlockBytes / 2), map, d * 64, row, bar);
                     }
@@ -641,7 +648,7 @@ template <int HD>
 void launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkArgs& a, int blocks, int least_run, cudaStream_t stream) {
     constexpr int NS = stages_of(HD);
     const size_t smem = 1024 + (size_t)(2 + 2 * NS) * (HD / 64) * kBlockBytes + (13 + 4 * NS) * sizeof(uint64_t) + 8 +
-                        (size_t)(4 * a.seqs + blocks + 2) * sizeof(int);
+                        (size_t)(5 * a.seqs + blocks + 3) * sizeof(int);
     auto kernel = attention_chunk_kernel<HD>;
     static bool prepared[kDevices] = {};
     const int dev = this_device();
@@ -673,10 +680,10 @@ long long attention_chunk_workspace(int head_dim, int kv_heads, int blocks) {
 }
 
 void attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window, const void* k_pages,
-                     const void* v_pages, int pages, const int32_t* seq_ends, const int32_t* cu_seqlens, int skip_new, int blocks, float* workspace,
+                     const void* v_pages, int pages, long long room, const int32_t* seq_ends, const int32_t* cu_seqlens, int skip_new, int blocks, float* workspace,
                      long long workspace_floats, int* error, cudaStream_t stream) {
     if (n_seqs <= 0 || blocks <= 0 || T <= 0) return;
-    if (!attention_chunk_supports(heads, kv_heads, head_dim, (long long)n_seqs * pages, n_seqs, blocks))
+    if (!attention_chunk_supports(heads, kv_heads, head_dim, room, n_seqs, blocks))
         throw std::invalid_argument("attention_chunk: " + std::to_string(heads) + " heads on " + std::to_string(kv_heads) + " of size " +
                                     std::to_string(head_dim) + " (64 or 128, at most 64 heads a kv head), " + std::to_string(n_seqs) + " sequences, " +
                                     std::to_string(blocks) + " blocks of queries");
@@ -693,14 +700,14 @@ void attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int
     const CUresult r = tensor_map_encoder()(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) throw std::runtime_error("attention_chunk: cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
-    // pages [n_seqs * pages, kv heads, 64 positions, head_dim] as rows of head_dim: a box is 64 columns of a page of one kv head
-    const uint64_t rows = (uint64_t)n_seqs * pages * kv_heads * kPageSize;
+    // pages [room, kv heads, 64 positions, head_dim] as rows of head_dim: a box is 64 columns of a page of one kv head
+    const uint64_t rows = (uint64_t)room * kv_heads * kPageSize;
     const CUtensorMap mk = tiled_map_2d("attention_chunk", CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, k_pages, (uint64_t)head_dim, rows, (uint64_t)head_dim * 2, 64,
                                         kPageSize, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
     const CUtensorMap mv = tiled_map_2d("attention_chunk", CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, v_pages, (uint64_t)head_dim, rows, (uint64_t)head_dim * 2, 64,
                                         kPageSize, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
     ChunkCut* cuts = (ChunkCut*)workspace;
-    ChunkArgs a{(__nv_bfloat16*)out, seq_ends, cu_seqlens, n_seqs, heads, kv_heads, window, skip_new, pages, tile_tokens, blocks, scale * 1.4426950408889634f, cuts,
+    ChunkArgs a{(__nv_bfloat16*)out, seq_ends, cu_seqlens, n_seqs, heads, kv_heads, window, skip_new, pages, (int)room, tile_tokens, blocks, scale * 1.4426950408889634f, cuts,
                 workspace + (long long)blocks * kv_heads * (long long)(sizeof(ChunkCut) / sizeof(float)), error};
     // a run is at least this many tiles: a part costs about as much as one to leave and join
     const int least_run = 2;

@@ -141,11 +141,11 @@ SM_API int sm_kv_quant_store(const sm::QuantPools* pools, const void* k_packed, 
 }
 
 SM_API int sm_kv_quant_load(const sm::QuantPools* pools, int dt, int n_seqs, const int32_t* slot_ids, const int32_t* seq_ends, void* k_out,
-                            void* v_out, int32_t* out_table, int pages, int whole, const int32_t* cu_seqlens, int skip_new, int attend,
-                            int window, int* error, void* stream) {
+                            void* v_out, int32_t* out_table, int pages, int whole, long long room, int read_seqs, int read_pages,
+                            const int32_t* cu_seqlens, int skip_new, int attend, int window, int* error, void* stream) {
     return guarded([&] {
-        sm::kv_quant_load(*pools, (sm::DType)dt, n_seqs, slot_ids, seq_ends, k_out, v_out, out_table, pages, whole != 0, cu_seqlens, skip_new,
-                          attend != 0, window, error, (cudaStream_t)stream);
+        sm::kv_quant_load(*pools, (sm::DType)dt, n_seqs, slot_ids, seq_ends, k_out, v_out, out_table, pages, whole != 0, room, read_seqs,
+                          read_pages, cu_seqlens, skip_new, attend != 0, window, error, (cudaStream_t)stream);
     });
 }
 
@@ -283,11 +283,11 @@ SM_API long long sm_attention_chunk_workspace(int head_dim, int kv_heads, int bl
 }
 
 SM_API int sm_attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window,
-                              const void* k_pages, const void* v_pages, int pages, const int32_t* seq_ends, const int32_t* cu_seqlens,
+                              const void* k_pages, const void* v_pages, int pages, long long room, const int32_t* seq_ends, const int32_t* cu_seqlens,
                               int skip_new, int blocks, float* workspace, long long workspace_floats, int* error, void* stream) {
     return guarded([&] {
-        sm::attention_chunk(q, out, T, n_seqs, heads, kv_heads, head_dim, scale, window, k_pages, v_pages, pages, seq_ends, cu_seqlens,
-                            skip_new, blocks, workspace, workspace_floats, error, (cudaStream_t)stream);
+        sm::attention_chunk(q, out, T, n_seqs, heads, kv_heads, head_dim, scale, window, k_pages, v_pages, pages, room, seq_ends,
+                            cu_seqlens, skip_new, blocks, workspace, workspace_floats, error, (cudaStream_t)stream);
     });
 }
 

@@ -87,18 +87,20 @@ struct QuantPools {
     int slots, table_stride;
 };
 // kv_quant_store: a step's packed keys and values [T, kv_heads, head_dim] (F32 or BF16) as codes and exponents into the pages
-// of their positions; k_rows, v_rows (nullable) receive what the cache then stands for, in dt. kv_quant_load: the pages of
-// n_seqs sequences as values of dt, [n_seqs, pages, kv_heads, 64, head_dim], positions at and past seq_ends[i] as zeros (pages
-// wholly past it only if `whole`, else they are left alone), and out_table [slots, pages] to find them by slot. A place outside
-// the page table or the pools is left out and recorded in the error word. Sequences that bring at most `skip_new` tokens by
-// cu_seqlens [n_seqs + 1] are left out. `attend`: for a kernel that multiplies masked values by zero weights: a value row
-// without a scale is read as zeros and its key as NaN instead (a token that sees it is NaN either way), and pages of 128
-// positions that no token of the step sees in `window` are left alone.
+// of their positions; k_rows, v_rows (nullable) receive what the cache then stands for, in dt. kv_quant_load: pages of the step's
+// sequences as values of dt, [room, kv_heads, 64, head_dim], positions at and past seq_ends[i] as zeros, and out_table [slots,
+// pages] (nullable) to find them by slot. `whole`: sequence i has the pages from i * pages on, those wholly past its end as zeros
+// (room = n_seqs * pages). Otherwise the sequences that bring more than `skip_new` tokens by cu_seqlens [n_seqs + 1] lie one
+// behind the other, each with the pages it holds: read_seqs of them with at most read_pages pages each, as the host knows. A
+// sequence longer than `pages` pages, one that `room` does not take, and a place outside the page table or the pools, are left
+// out and recorded in the error word. `attend`: for a kernel that multiplies masked values by zero weights: a value row without a
+// scale is read as zeros and its key as NaN instead (a token that sees it is NaN either way), and of each sequence only the
+// pages of pages_read (kv_quant.cuh) are taken, those that a token of the step sees in `window`.
 void kv_quant_store(const QuantPools& pools, const void* k_packed, const void* v_packed, DType dt, int T, void* k_rows, void* v_rows,
                     const int32_t* positions, const int32_t* token_slot, int* error, cudaStream_t stream);
 void kv_quant_load(const QuantPools& pools, DType dt, int n_seqs, const int32_t* slot_ids, const int32_t* seq_ends, void* k_out, void* v_out,
-                   int32_t* out_table, int pages, bool whole, const int32_t* cu_seqlens, int skip_new, bool attend, int window,
-                   int* error, cudaStream_t stream);
+                   int32_t* out_table, int pages, bool whole, long long room, int read_seqs, int read_pages, const int32_t* cu_seqlens,
+                   int skip_new, bool attend, int window, int* error, cudaStream_t stream);
 
 // ---- gemm_simt.cu ---------------------------------------------------------------------
 // out[t, n] (+)= sum_k x[t, k] * w[n, k] + bias[n]; float FMA in ascending k for every
@@ -285,12 +287,12 @@ void attention_quant(const QuantPools& pools, const void* q, void* out, int n_se
 
 // ---- attention_chunk_tc.cu ------------------------------------------------------------
 // The same attention for sequences that bring more than `skip_new` tokens, over their pages as bfloat16 values as
-// kv_quant_load (attend) leaves them: [n_seqs, pages, kv_heads, 64, head_dim], sequence by sequence. Head sizes 64 and 128.
+// kv_quant_load (attend) leaves them, in `room` pages; `pages`: what the longest sequence has at most. Head sizes 64 and 128.
 // `blocks`: blocks of 2 * (128 / group) new tokens over those sequences (group: heads a kv head).
 bool attention_chunk_supports(int heads, int kv_heads, int head_dim, long long pool_pages, int n_seqs, int blocks);
 long long attention_chunk_workspace(int head_dim, int kv_heads, int blocks);   // floats
 void attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int kv_heads, int head_dim, float scale, int window, const void* k_pages,
-                     const void* v_pages, int pages, const int32_t* seq_ends, const int32_t* cu_seqlens, int skip_new, int blocks, float* workspace,
+                     const void* v_pages, int pages, long long room, const int32_t* seq_ends, const int32_t* cu_seqlens, int skip_new, int blocks, float* workspace,
                      long long workspace_floats, int* error, cudaStream_t stream);
 
 // ---- decode_fused.cu ------------------------------------------------------------------

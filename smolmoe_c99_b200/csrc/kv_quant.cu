@@ -158,50 +158,76 @@ __global__ void __launch_bounds__(kThreads) kv_quant_store_kernel(StoreArgs a, i
 struct LoadArgs {
     const uint8_t* codes[2];
     const uint8_t* scales[2];
-    void* out[2];                // [sequences, pages, kv_heads, kPageSize, head_dim]
-    int32_t* out_table;          // [slots, pages]: where a slot's pages lie in `out`
+    void* out[2];                // [room, kv_heads, kPageSize, head_dim]
+    int32_t* out_table;          // [slots, pages]: where a slot's pages lie in `out` (nullable)
     const int32_t* slot_ids;     // [sequences]
     const int32_t* seq_ends;     // [sequences]
     QuantPages table;
-    int kv_heads, head_dim, pages, whole;
-    const int32_t* cu;           // [sequences + 1] (read only where skip_new or a window asks for it)
+    int kv_heads, head_dim, seqs, pages, whole;
+    long long room;              // pages of `out`
+    const int32_t* cu;           // [sequences + 1] (not read where all is read back whole)
     int skip_new;                // sequences that bring at most this many tokens are left out
     int attend, window;          // see kv_quant_load in kernels.h
     int* error;
 };
 
-// A CTA reads one page (blockIdx.x) of one sequence (blockIdx.y), keys or values (blockIdx.z): a page's kv heads lie one
-// behind the other in the pools and in the output, so this is one run of bytes and one of values, 8 of them a thread and
-// kLoadSteps such pieces under way together. Positions at and past the sequence's end read as zero; pages wholly past it
-// are left alone unless `whole`.
+// The sequence that is number `rank` of those that are read back (-1: there is none), its pages, and how many pages the ones before
+// it take. Each warp goes through the step's sequences by itself, 32 at once.
+struct SequenceRead {
+    int seq;
+    long long before;
+    PagesRead pages;
+};
+__device__ __forceinline__ SequenceRead find_sequence(const LoadArgs& a, int rank) {
+    const int lane = threadIdx.x & 31;
+    int seen = 0;
+    long long before = 0;
+    for (int i0 = 0; i0 < a.seqs; i0 += 32) {
+        const int i = i0 + lane, n = i < a.seqs ? a.cu[i + 1] - a.cu[i] : -1, end = i < a.seqs ? a.seq_ends[i] : 0;
+        const PagesRead p = pages_read(end - n, end, a.window, a.pages);
+        const unsigned read = __ballot_sync(0xffffffffu, n > a.skip_new);
+        const int mine = n > a.skip_new ? seen + __popc(read & ((1u << lane) - 1)) : -1;
+        before += __reduce_add_sync(0xffffffffu, mine >= 0 && mine < rank ? p.count : 0);
+        const unsigned hit = __ballot_sync(0xffffffffu, mine == rank);
+        if (hit) {
+            const int at = __ffs(hit) - 1;
+            return {i0 + at, before, {__shfl_sync(0xffffffffu, p.first, at), __shfl_sync(0xffffffffu, p.count, at)}};
+        }
+        seen += __popc(read);
+    }
+    return {-1, 0, {0, 0}};
+}
+
+// A CTA reads one page (blockIdx.x, from the first that is read back) of one sequence (blockIdx.y, of those that are read back),
+// keys or values (blockIdx.z): a page's kv heads lie one behind the other in the pools and in the output, so this is one run of
+// bytes and one of values, 8 of them a thread and kLoadSteps such pieces under way together. Positions at and past the sequence's
+// end read as zero. `whole`: every sequence has `pages` pages of the output, zeros past its end; otherwise they lie one behind
+// the other, each as many as it holds.
 constexpr int kLoadSteps = 4;
 
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kThreads) kv_quant_load_kernel(LoadArgs a) {
     pdl_wait();                  // the cache may have been written by the kernel before
     pdl_launch_dependents();
-    const int page = blockIdx.x, seq = blockIdx.y, which = blockIdx.z;
-    const int slot = a.slot_ids[seq], end = a.seq_ends[seq];
-    if (a.skip_new > 0 && a.cu[seq + 1] - a.cu[seq] <= a.skip_new) return;
-    if ((unsigned)slot >= (unsigned)a.table.slots) {
+    const int which = blockIdx.z;
+    const SequenceRead r = a.whole ? SequenceRead{(int)blockIdx.y, (long long)blockIdx.y * a.pages, {0, a.pages}} : find_sequence(a, blockIdx.y);
+    if (r.seq < 0) return;
+    const int slot = a.slot_ids[r.seq], end = a.seq_ends[r.seq], page = r.pages.first + blockIdx.x;
+    // (what does not fit is left out)
+    if ((unsigned)slot >= (unsigned)a.table.slots || end > a.pages * kPageSize || r.before + r.pages.count > a.room) {
         if (a.error && threadIdx.x == 0) atomicExch(a.error, kBadPlaceInLoad);
-        return;
+        if ((unsigned)slot >= (unsigned)a.table.slots || r.before + r.pages.count > a.room) return;
     }
-    if (which == 0 && threadIdx.x == 0) a.out_table[(size_t)slot * a.pages + page] = seq * a.pages + page;
-    if (end > a.pages * kPageSize && a.error && threadIdx.x == 0) atomicExch(a.error, kBadPlaceInLoad);       // (what does not fit is left out)
+    if ((int)blockIdx.x >= r.pages.count) return;
+    const long long to = r.before + blockIdx.x;
+    if (which == 0 && threadIdx.x == 0 && a.out_table) a.out_table[(size_t)slot * a.pages + page] = (int)to;
     const int live = min(end - page * kPageSize, kPageSize);      // positions of the page that the sequence holds
-    if (live <= 0 && !a.whole) return;
-    if (a.window > 0) {
-        // pages that no token of the step sees, but for the neighbour that shares a tile of 128 positions with a seen one
-        const int lowest = end - (a.cu[seq + 1] - a.cu[seq]) - a.window + 1;
-        if (lowest > 0 && page < lowest / 128 * (128 / kPageSize)) return;
-    }
     const int held = live > 0 ? a.table.at(slot, page) : -1;
     if (live > 0 && held < 0 && a.error && threadIdx.x == 0) atomicExch(a.error, kBadPlaceInLoad);
     const int parts = a.head_dim / 8, total = a.kv_heads * kPageSize * parts;      // pieces of 8 values: of a row, of the page
     const size_t cell0 = held < 0 ? 0 : (size_t)held * a.kv_heads * kPageSize;
     const uint8_t* codes = a.codes[which] + cell0 * a.head_dim;
-    T* out = (T*)a.out[which] + ((size_t)seq * a.pages + page) * a.kv_heads * kPageSize * a.head_dim;
+    T* out = (T*)a.out[which] + (size_t)to * a.kv_heads * kPageSize * a.head_dim;
     for (int base = threadIdx.x; base < total; base += kThreads * kLoadSteps) {
         uint2 raw[kLoadSteps];
         int byte[kLoadSteps];
@@ -273,19 +299,21 @@ void kv_quant_store(const QuantPools& p, const void* k_packed, const void* v_pac
 }
 
 void kv_quant_load(const QuantPools& p, DType dt, int n_seqs, const int32_t* slot_ids, const int32_t* seq_ends, void* k_out, void* v_out,
-                   int32_t* out_table, int pages, bool whole, const int32_t* cu_seqlens, int skip_new, bool attend, int window,
-                   int* error, cudaStream_t stream) {
-    if (n_seqs <= 0 || pages <= 0) return;
+                   int32_t* out_table, int pages, bool whole, long long room, int read_seqs, int read_pages, const int32_t* cu_seqlens,
+                   int skip_new, bool attend, int window, int* error, cudaStream_t stream) {
+    if (whole) { read_seqs = n_seqs; read_pages = pages; }
+    if (n_seqs <= 0 || pages <= 0 || read_seqs <= 0 || read_pages <= 0) return;
     check_pools("kv_quant_load", p);
-    if (n_seqs > 65535) throw std::invalid_argument("kv_quant_load: more than 65535 sequences");
+    if (read_seqs > 65535) throw std::invalid_argument("kv_quant_load: more than 65535 sequences");
     if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) throw std::invalid_argument("kv_quant_load: outputs must be 16-byte aligned");
+    if (room > 0x7fffffffll) throw std::invalid_argument("kv_quant_load: more than 2^31 pages in one call");
     LoadArgs a{{(const uint8_t*)p.k_codes, (const uint8_t*)p.v_codes}, {(const uint8_t*)p.k_scale, (const uint8_t*)p.v_scale}, {k_out, v_out}, out_table,
-               slot_ids, seq_ends, {p.page_table, p.slots, p.table_stride, p.pages}, p.kv_heads, p.head_dim, pages, whole ? 1 : 0, cu_seqlens, skip_new,
-               attend ? 1 : 0, attend ? window : 0, error};
+               slot_ids, seq_ends, {p.page_table, p.slots, p.table_stride, p.pages}, p.kv_heads, p.head_dim, n_seqs, pages, whole ? 1 : 0, room,
+               cu_seqlens, whole ? 0 : skip_new, attend ? 1 : 0, attend ? window : 0, error};
     note_launch();
     auto kernel = dt == F32 ? (p.fmt == QUANT_FP8 ? kv_quant_load_kernel<float, QUANT_FP8> : kv_quant_load_kernel<float, QUANT_INT8>)
                             : (p.fmt == QUANT_FP8 ? kv_quant_load_kernel<__nv_bfloat16, QUANT_FP8> : kv_quant_load_kernel<__nv_bfloat16, QUANT_INT8>);
-    launch_kernel("kv_quant_load", kernel, dim3((unsigned)pages, (unsigned)n_seqs, 2), dim3(kThreads), 0, stream, 1, dependent_launch_enabled(), a);
+    launch_kernel("kv_quant_load", kernel, dim3((unsigned)read_pages, (unsigned)read_seqs, 2), dim3(kThreads), 0, stream, 1, dependent_launch_enabled(), a);
 }
 
 }  // namespace sm

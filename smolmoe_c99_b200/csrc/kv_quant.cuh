@@ -45,6 +45,16 @@ struct QuantPages {
     }
 };
 
+// What kv_quant_load reads back of a sequence for a kernel that attends over it: `count` pages from `first` on, those that a token
+// of the step sees in `window` (0: all) and the neighbour that shares 128 positions with the first of them; at most page most - 1.
+struct PagesRead {
+    int first, count;
+};
+__device__ __forceinline__ PagesRead pages_read(int start, int end, int window, int most) {
+    const int first = (window > 0 ? max(0, start - window + 1) : 0) / 128 * (128 / kPageSize);
+    return {first, max(min((end + kPageSize - 1) / kPageSize, most) - first, 0)};
+}
+
 // 2^e for -126 <= e <= 127
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 // the factor of a row from its byte (infinity for kNoScale: its codes are 0, so the product is NaN; 0 for a row never written)

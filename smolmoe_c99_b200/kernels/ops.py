@@ -188,14 +188,14 @@ class Ops:
         # (with the argument types known, a call takes plain numbers as addresses)
         addr, num, big, real = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
         self.lib.sm_kv_quant_store.argtypes = [addr] * 3 + [num] * 2 + [addr] * 6
-        self.lib.sm_kv_quant_load.argtypes = [addr, num, num] + [addr] * 5 + [num, num, addr, num, num, num, addr, addr]
+        self.lib.sm_kv_quant_load.argtypes = [addr, num, num] + [addr] * 5 + [num, num, big, num, num, addr, num, num, num, addr, addr]
         self.lib.sm_attention_quant.argtypes = [addr] * 3 + [num, num, real, num] + [addr] * 3 + [num] * 5 + [addr, big, addr, addr]
         self.lib.sm_attention_quant_supports.argtypes = [num, num, num, big]
         self.lib.sm_attention_quant_fits.argtypes = [num] * 4
         self.lib.sm_attention_quant_workspace.argtypes, self.lib.sm_attention_quant_workspace.restype = [num] * 4, big
         self.lib.sm_attention_chunk_supports.argtypes = [num, num, num, big, num, num]
         self.lib.sm_attention_chunk_workspace.argtypes, self.lib.sm_attention_chunk_workspace.restype = [num] * 3, big
-        self.lib.sm_attention_chunk.argtypes = [addr, addr] + [num] * 5 + [real, num, addr, addr, num, addr, addr, num, num, addr, big, addr, addr]
+        self.lib.sm_attention_chunk.argtypes = [addr, addr] + [num] * 5 + [real, num, addr, addr, num, big, addr, addr, num, num, addr, big, addr, addr]
         self._quant_plans: dict = {}      # by sizes alone
         fast = kernels == "fast"
         self.kernels = kernels
@@ -698,24 +698,41 @@ class Ops:
         zeros."""
         if dtype is not torch.float32 and dtype is not torch.bfloat16:
             raise KernelError(f"an 8-bit cache is read back as float32 or bfloat16, not {dtype}")
-        k, v, table = self._quant_load(step, self._quant_cache(cache), cache, dtype, True, 0, False, 0)
+        layer = self._quant_cache(cache)
+        pages = min((step.max_seq_len + PAGE_SIZE - 1) // PAGE_SIZE, layer.table_stride)
+        table = cache.page_table.new_empty((layer.slots, pages))
+        k, v = self._quant_load(step, layer, cache, dtype, table, True, pages, step.n_seqs * pages, step.n_seqs, pages, 0, False, 0)
         return type(cache)("kv", k, v, table, 0, cache.window)
 
-    def _quant_load(self, step, layer, cache, dtype, whole, skip_new, attend, window):
-        """Values of keys, of values, and their page table. ``whole``: pages past a sequence's end are zeroed too; the
-        others: see kv_quant_load in csrc/kernels.h."""
-        # (a captured step's longest sequence is a bound that may pass what the page table can hold)
-        pages = min((step.max_seq_len + PAGE_SIZE - 1) // PAGE_SIZE, layer.table_stride)
+    def _quant_load(self, step, layer, cache, dtype, table, whole, pages, room, read_seqs, read_pages, skip_new, attend, window):
+        """Values of keys and of values, [room, kv heads, 64, head size] each: see kv_quant_load in csrc/kernels.h."""
         slot_ids, seq_ends, cu = step.slot_ids, step.seq_ends, step.cu_seqlens
         _here(slot_ids, seq_ends, cu)
-        k = cache.k_pool.new_empty((step.n_seqs * pages, layer.kv_heads, PAGE_SIZE, layer.head_dim), dtype=dtype)
+        k = cache.k_pool.new_empty((room, layer.kv_heads, PAGE_SIZE, layer.head_dim), dtype=dtype)
         v = torch.empty_like(k)
-        table = cache.page_table.new_empty((layer.slots, pages))
         self._check(self.lib.sm_kv_quant_load(
             layer.address, F32 if dtype is torch.float32 else BF16, step.n_seqs, slot_ids.data_ptr(), seq_ends.data_ptr(), k.data_ptr(),
-            v.data_ptr(), table.data_ptr(), pages, whole, cu.data_ptr(), skip_new, attend, window, self._error_address,
-            _raw_stream()))
-        return k, v, table
+            v.data_ptr(), None if table is None else table.data_ptr(), pages, whole, room, read_seqs, read_pages, cu.data_ptr(), skip_new,
+            attend, window, self._error_address, _raw_stream()))
+        return k, v
+
+    @staticmethod
+    def _pages_read(step, layer, cache, skip_new, window):
+        """For the sequences that bring more than ``skip_new`` tokens: (the most pages that the longest has, pages of all together that
+        attention in ``window`` reads back, sequences, the most pages of one), as ``pages_read`` in csrc/kv_quant.cuh counts them.
+        From the sequences' lengths where the host knows them; in a captured step, which is replayed with others, from the longest
+        that the step is kept for, and all together at most what the pools hold where no two sequences share a page."""
+        most = min((step.max_seq_len + PAGE_SIZE - 1) // PAGE_SIZE, layer.table_stride)
+        per_tile = 128 // PAGE_SIZE
+        if step.seq_starts is not None and not torch.cuda.is_current_stream_capturing():
+            first = lambda s: max(0, s - window + 1) // 128 * per_tile if window else 0
+            counts = [max(min((s + n + PAGE_SIZE - 1) // PAGE_SIZE, most) - first(s), 0) for s, n in zip(step.seq_starts, step.seq_lens) if n > skip_new]
+            room = sum(counts)
+        else:
+            # (the positions seen are n + window - 1, and up to 127 before them share their 128)
+            counts = [min(most, (n + window + 126 + PAGE_SIZE - 1) // PAGE_SIZE) if window else most for n in step.seq_lens if n > skip_new]
+            room = min(sum(counts), layer.pages) if cache.exclusive else sum(counts)
+        return most, room, len(counts), max(counts)
 
     def attention_quant(self, q, step, scale, window, cache):
         """Causal attention of this step's tokens (one or any number per sequence) over an 8-bit cache, which holds their own
@@ -742,7 +759,9 @@ class Ops:
         plan = self._quant_plan(step.seq_lens, step.max_seq_len, heads, layer, dtype, window)
         if plan is None:
             # the plain kernel over pages that have been read back: float queries, other head sizes
-            k, v, table = self._quant_load(step, layer, cache, dtype, False, 0, False, 0)
+            most, room, seqs, pages = self._pages_read(step, layer, cache, 0, 0)
+            table = cache.page_table.new_empty((layer.slots, most))
+            k, v = self._quant_load(step, layer, cache, dtype, table, False, most, room, seqs, pages, 0, False, 0)
             return self.attention_plain(q, step.positions, scale, window, k_pool=k, v_pool=v, page_table=table, token_slot=step.token_slot,
                                         kv_heads=kv_heads)
         limit, row_tiles, pairs, cluster, longest, floats, blocks, chunk_floats = plan
@@ -755,11 +774,12 @@ class Ops:
                 longest, limit, row_tiles, pairs, cluster, workspace.data_ptr() if floats else None, floats, self._error_address, _raw_stream()))
         if blocks:
             # many tokens: the pages are read back as bfloat16 once (exactly), and the tcgen05 kernel reads those
-            k, v, table = self._quant_load(step, layer, cache, dtype, False, limit, True, window)
+            most, room, seqs, pages = self._pages_read(step, layer, cache, limit, window)
+            k, v = self._quant_load(step, layer, cache, dtype, None, False, most, room, seqs, pages, limit, True, window)
             workspace = q.new_empty((chunk_floats,), dtype=torch.float32)
             self._check(self.lib.sm_attention_chunk(
                 q.data_ptr(), out.data_ptr(), step.n_tokens, n_seqs, heads, kv_heads, head_dim, scale, window, k.data_ptr(), v.data_ptr(),
-                table.shape[1], seq_ends.data_ptr(), cu.data_ptr(), limit, blocks, workspace.data_ptr(), chunk_floats, self._error_address,
+                most, room, seq_ends.data_ptr(), cu.data_ptr(), limit, blocks, workspace.data_ptr(), chunk_floats, self._error_address,
                 _raw_stream()))
         return out
 

@@ -168,3 +168,37 @@ def test_as_many_sequences_as_are_promised(ops, heads, kv_heads, hd, n, cluster,
     monkeypatch.setattr(ops, "use_fast_attention", False)
     plain = ops.attention_quant(q, step, hd ** -0.5, 0, layer).double()
     assert float((got.double() - plain).abs().max()) <= 2.0 ** -6 * float(plain.abs().max())
+
+
+# ---- memory -------------------------------------------------------------------------------------------------------------
+
+def _peak(call):
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    call()
+    torch.cuda.synchronize()
+    return torch.cuda.max_memory_allocated() - before
+
+
+@pytest.mark.parametrize("window,dtype", [(0, torch.bfloat16), (500, torch.bfloat16), (0, torch.float32)])
+def test_what_a_mixed_step_reads_back_is_what_its_chunks_see(ops, window, dtype):
+    """Many sequences that decode beside one that brings a portion onto a long one: the pages read back are those of the long
+    one alone (within its window), not as many for each; in the 32-bit path those that each sequence holds."""
+    n, heads, kv_heads, hd = 40, 8, 4, 128
+    starts, news, slots = [9000] + [100 + i for i in range(n)], [300] + [1] * n, list(range(n + 1))
+    ends = [s + k for s, k in zip(starts, news)]
+    layer = make_layer("fp8", kv_heads, hd, ends, slots)
+    fill(ops, layer, slots, ends, 101)
+    q = _randn((sum(news), heads, hd), 102).to(dtype)
+    step = pack_step(slots, starts, [[0] * k for k in news], torch.device("cuda"))
+    page = 2 * kv_heads * 64 * hd * q.element_size()
+    pages = -(-ends[0] // 64) if not window else -(-(window + news[0]) // 64) + 4
+    if dtype == torch.float32:
+        pages += sum(-(-e // 64) for e in ends[1:])
+    room = pages * page + q.numel() * q.element_size() + (1 << 20)
+    if dtype == torch.bfloat16:     # (what the two kernels keep their parts in)
+        room += 4 * (ops.lib.sm_attention_chunk_workspace(hd, kv_heads, 10) + ops.lib.sm_attention_quant_workspace(hd, 2, kv_heads * (n + 1), 0))
+    ops.attention_quant(q, step, hd ** -0.5, window, layer)
+    assert _peak(lambda: ops.attention_quant(q, step, hd ** -0.5, window, layer)) <= room
+    ops.check_error_flag()

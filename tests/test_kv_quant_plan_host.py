@@ -1,0 +1,39 @@
+"""How much of an 8-bit cache a step reads back, counted on the host."""
+import random
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from smolmoe_c99_b200.engine.batch import pack_step
+from smolmoe_c99_b200.kernels import Ops
+
+
+@pytest.mark.parametrize("window", [0, 1, 64, 65, 300])
+def test_pages_that_are_read_back(window, monkeypatch):
+    """Against a count position by position; a captured step's bound holds for every start that its span allows."""
+    rng = random.Random(window)
+    layer, capturing = SimpleNamespace(table_stride=20, pages=60), False
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    for _ in range(60):
+        starts, news = zip(*[(rng.choice([0, 1, 63, 64, 127, 128, 129, rng.randrange(1000)]), rng.choice([1, 2, 65, 200])) for _ in range(rng.randint(1, 6))])
+        step = pack_step(list(range(len(starts))), list(starts), [[0] * n for n in news], torch.device("cpu"))
+        skip = rng.choice([0, 1, 64])
+        reading = [(s, n) for s, n in zip(starts, news) if n > skip]
+        if not reading:
+            continue
+        taken = []
+        for s, n in reading:
+            seen = {p // 128 for t in range(s, s + n) for p in range(max(0, t - window + 1) if window else 0, t + 1)}
+            taken.append(sum(1 for page in range(-(-(s + n) // 64)) if page // 2 >= min(seen)))
+        capturing = False
+        most, room, seqs, pages = Ops._pages_read(step, layer, SimpleNamespace(exclusive=False), skip, window)
+        assert (most, room, seqs, pages) == (-(-max(s + n for s, n in zip(starts, news)) // 64), sum(taken), len(taken), max(taken))
+        capturing = True
+        step.max_seq_len = 1280
+        for exclusive in (False, True):
+            most, room, seqs, pages = Ops._pages_read(step, layer, SimpleNamespace(exclusive=exclusive), skip, window)
+            assert most == 20 and seqs == len(taken) and pages >= max(taken)
+            assert room >= sum(taken) if not exclusive else room == min(60, room)
+        step.seq_starts, capturing = None, False          # (a decode step's graph knows no starts)
+        assert Ops._pages_read(step, layer, SimpleNamespace(exclusive=False), skip, window)[1] >= sum(taken)
