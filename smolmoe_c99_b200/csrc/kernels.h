@@ -89,8 +89,8 @@ struct QuantPools {
 // kv_quant_store: a step's packed keys and values [T, kv_heads, head_dim] (F32 or BF16) as codes and exponents into the pages
 // of their positions; k_rows, v_rows (nullable) receive what the cache then stands for, in dt. kv_quant_load: pages of the step's
 // sequences as values of dt, [room, kv_heads, 64, head_dim], positions at and past seq_ends[i] as zeros, and out_table [slots,
-// pages] (nullable) to find them by slot. `whole`: sequence i has the pages from i * pages on, those wholly past its end as zeros
-// (room = n_seqs * pages). Otherwise the sequences that bring more than `skip_new` tokens by cu_seqlens [n_seqs + 1] lie one
+// pages] (nullable) to find them by slot. `whole`: sequence i has the pages from i * pages on, those wholly past its end as zeros,
+// and slots that are not the step's have page 0 throughout (room = n_seqs * pages; out_table is needed). Otherwise the sequences that bring more than `skip_new` tokens by cu_seqlens [n_seqs + 1] lie one
 // behind the other, each with the pages it holds: read_seqs of them with at most read_pages pages each, as the host knows. A
 // sequence longer than `pages` pages, one that `room` does not take, and a place outside the page table or the pools, are left
 // out and recorded in the error word. `attend`: for a kernel that multiplies masked values by zero weights: a value row without a

@@ -210,6 +210,12 @@ __global__ void __launch_bounds__(kThreads) kv_quant_load_kernel(LoadArgs a) {
     pdl_wait();                  // the cache may have been written by the kernel before
     pdl_launch_dependents();
     const int which = blockIdx.z;
+    if (a.whole && which == 1 && blockIdx.y == 0)       // slots that are not the step's are given a page that exists
+        for (int slot = threadIdx.x; slot < a.table.slots; slot += kThreads) {
+            bool named = false;
+            for (int i = 0; i < a.seqs; ++i) named |= a.slot_ids[i] == slot;
+            if (!named) a.out_table[(size_t)slot * a.pages + blockIdx.x] = 0;
+        }
     const SequenceRead r = a.whole ? SequenceRead{(int)blockIdx.y, (long long)blockIdx.y * a.pages, {0, a.pages}} : find_sequence(a, blockIdx.y);
     if (r.seq < 0) return;
     const int slot = a.slot_ids[r.seq], end = a.seq_ends[r.seq], page = r.pages.first + blockIdx.x;
@@ -306,6 +312,7 @@ void kv_quant_load(const QuantPools& p, DType dt, int n_seqs, const int32_t* slo
     check_pools("kv_quant_load", p);
     if (read_seqs > 65535) throw std::invalid_argument("kv_quant_load: more than 65535 sequences");
     if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) throw std::invalid_argument("kv_quant_load: outputs must be 16-byte aligned");
+    if (whole && !out_table) throw std::invalid_argument("kv_quant_load: the pages of whole sequences need a page table");
     if (room > 0x7fffffffll) throw std::invalid_argument("kv_quant_load: more than 2^31 pages in one call");
     LoadArgs a{{(const uint8_t*)p.k_codes, (const uint8_t*)p.v_codes}, {(const uint8_t*)p.k_scale, (const uint8_t*)p.v_scale}, {k_out, v_out}, out_table,
                slot_ids, seq_ends, {p.page_table, p.slots, p.table_stride, p.pages}, p.kv_heads, p.head_dim, n_seqs, pages, whole ? 1 : 0, room,

@@ -695,7 +695,7 @@ class Ops:
         """What an 8-bit cache holds of the step's sequences (their lengths after the step), as values: a ``LayerCache`` of
         ``dtype`` whose page table has the same slots. Sequence ``i`` of the step has its pages from ``i * P`` on, ``P``
         the pages of ``step.max_seq_len`` positions (at most the page table's width); positions past its end read as
-        zeros."""
+        zeros. Slots that are not the step's are given page 0."""
         if dtype is not torch.float32 and dtype is not torch.bfloat16:
             raise KernelError(f"an 8-bit cache is read back as float32 or bfloat16, not {dtype}")
         layer = self._quant_cache(cache)

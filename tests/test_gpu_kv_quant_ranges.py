@@ -202,3 +202,20 @@ def test_what_a_mixed_step_reads_back_is_what_its_chunks_see(ops, window, dtype)
     ops.attention_quant(q, step, hd ** -0.5, window, layer)
     assert _peak(lambda: ops.attention_quant(q, step, hd ** -0.5, window, layer)) <= room
     ops.check_error_flag()
+
+
+# ---- pages read back ----------------------------------------------------------------------------------------------------
+
+def test_slots_that_are_not_of_the_step_have_a_page_that_exists(ops):
+    """kv_quant_load's page table has every slot of the cache's: those that the step does not name must not lead out of the pages
+    that were read back."""
+    layer = make_layer("int8", 2, 64, [100, 200, 70], [7, 2, 33])
+    fill(ops, layer, [7, 2, 33], [100, 200, 70], 103)
+    step = pack_step([33, 7], [69, 99], [[0], [0]], torch.device("cuda"))
+    poison = torch.full((layer.page_table.shape[0], 2), 1 << 30, dtype=torch.int32, device="cuda")
+    del poison                                   # (its memory is what the table is likely to get)
+    back = ops.kv_quant_load(step, layer, torch.bfloat16)
+    table = back.page_table.cpu()
+    assert tuple(table.shape) == (35, 2) and int(table.min()) >= 0 and int(table.max()) < back.k_pool.shape[0]
+    assert table[33].tolist() == [0, 1] and table[7].tolist() == [2, 3]
+    ops.check_error_flag()
