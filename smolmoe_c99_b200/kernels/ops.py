@@ -717,6 +717,16 @@ class Ops:
         return k, v
 
     @staticmethod
+    def _check_places(step, layer):
+        """Refuses a step whose slots or positions, as far as the host knows them, lie outside the page table."""
+        if step.slots and not 0 <= min(step.slots) <= max(step.slots) < layer.slots:
+            raise KernelError(f"a step of slots {min(step.slots)} to {max(step.slots)}: the page table has {layer.slots}")
+        if step.seq_starts is not None:
+            longest = max(s + n for s, n in zip(step.seq_starts, step.seq_lens))
+            if longest > layer.table_stride * PAGE_SIZE:
+                raise KernelError(f"a sequence of {longest} positions: the page table holds {layer.table_stride * PAGE_SIZE}")
+
+    @staticmethod
     def _pages_read(step, layer, cache, skip_new, window):
         """For the sequences that bring more than ``skip_new`` tokens: (the most pages that the longest has, pages of all together that
         attention in ``window`` reads back, sequences, the most pages of one), as ``pages_read`` in csrc/kv_quant.cuh counts them.
@@ -759,8 +769,10 @@ class Ops:
         plan = self._quant_plan(step.seq_lens, step.max_seq_len, heads, layer, dtype, window)
         if plan is None:
             # the plain kernel over pages that have been read back: float queries, other head sizes
+            # (it checks no slot, position or page: those that the host knows are looked at here, and what is not read back has page 0)
+            self._check_places(step, layer)
             most, room, seqs, pages = self._pages_read(step, layer, cache, 0, 0)
-            table = cache.page_table.new_empty((layer.slots, most))
+            table = cache.page_table.new_zeros((layer.slots, most))
             k, v = self._quant_load(step, layer, cache, dtype, table, False, most, room, seqs, pages, 0, False, 0)
             return self.attention_plain(q, step.positions, scale, window, k_pool=k, v_pool=v, page_table=table, token_slot=step.token_slot,
                                         kv_heads=kv_heads)

@@ -219,3 +219,19 @@ def test_slots_that_are_not_of_the_step_have_a_page_that_exists(ops):
     assert tuple(table.shape) == (35, 2) and int(table.min()) >= 0 and int(table.max()) < back.k_pool.shape[0]
     assert table[33].tolist() == [0, 1] and table[7].tolist() == [2, 3]
     ops.check_error_flag()
+
+
+# ---- places, where the plain kernel attends ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 64), (torch.bfloat16, 24)])
+def test_places_outside_the_page_table_are_refused_by_the_plain_form(ops, dtype, hd):
+    """Float queries and head sizes of no kernel of their own are attended by one that checks no place."""
+    from smolmoe_c99_b200.kernels import KernelError
+    layer = make_layer("fp8", 2, hd, [100, 128], [0, 1])
+    fill(ops, layer, [0, 1], [100, 128], 104)
+    q = _randn((2, 4, hd), 105).to(dtype)
+    for slots, starts in (([0, layer.page_table.shape[0]], [99, 0]), ([0, 1], [99, 64 * layer.page_table.shape[1]])):
+        with pytest.raises(KernelError, match="the page table"):
+            ops.attention_quant(q, pack_step(slots, starts, [[0], [0]], torch.device("cuda")), 0.125, 0, layer)
+    ops.attention_quant(q, pack_step([1, 0], [127, 99], [[0], [0]], torch.device("cuda")), 0.125, 0, layer)
+    ops.check_error_flag()

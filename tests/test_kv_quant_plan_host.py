@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from smolmoe_c99_b200.engine.batch import pack_step
-from smolmoe_c99_b200.kernels import Ops
+from smolmoe_c99_b200.kernels import KernelError, Ops
 
 
 @pytest.mark.parametrize("window", [0, 1, 64, 65, 300])
@@ -37,3 +37,17 @@ def test_pages_that_are_read_back(window, monkeypatch):
             assert room >= sum(taken) if not exclusive else room == min(60, room)
         step.seq_starts, capturing = None, False          # (a decode step's graph knows no starts)
         assert Ops._pages_read(step, layer, SimpleNamespace(exclusive=False), skip, window)[1] >= sum(taken)
+
+
+@pytest.mark.parametrize("slots,starts,message", [([0, 5], [0, 9], "slots 0 to 5: the page table has 5"), ([-1, 2], [0, 9], "slots -1 to 2"),
+                                                  ([0, 4], [3, 126], "129 positions: the page table holds 128")])
+def test_places_outside_the_page_table_are_refused_where_no_kernel_would(slots, starts, message):
+    step = pack_step(slots, starts, [[0, 0], [0, 0, 0]], torch.device("cpu"))
+    with pytest.raises(KernelError, match=message):
+        Ops._check_places(step, SimpleNamespace(slots=5, table_stride=2))
+
+
+def test_places_inside_the_page_table_are_not_refused():
+    layer = SimpleNamespace(slots=5, table_stride=2)
+    Ops._check_places(pack_step([0, 4], [3, 125], [[0, 0], [0, 0, 0]], torch.device("cpu")), layer)
+    Ops._check_places(SimpleNamespace(slots=[], seq_starts=None), layer)
