@@ -78,7 +78,7 @@ struct AttnArgs {
     int most_new;                        // sequences with more new tokens are not this kernel's
     int block_tokens;                    // tokens of a block of rows
     int pairs;                           // what the host says there are
-    int cluster, stages, tile;           // CTAs of a cluster (0: the line); tiles a warp keeps in flight; positions of a tile
+    int cluster, stages, tile_log;       // CTAs of a cluster (0: the line); tiles a warp keeps in flight; positions of a tile: 2^tile_log
     float scale_log2;
     Cut* cuts;                           // the line: [pairs]
     float* parts;                        // the line: [warps][2][rows][padded head size + 4]: values, then maximum and sum
@@ -94,16 +94,25 @@ struct SeqTable {
 };
 constexpr size_t seq_table_bytes(int seqs) { return ((size_t)5 * seqs + 2) * sizeof(int); }
 
+// A sequence: every pair of it has as many tiles (a closed form keeps the line's arithmetic short): all from the first new token's
+// window to the last new token, or, in a window, as many as a block's positions can touch, ending with the block's last one
+// (but none before the sequence's first: of a block near it some lie behind the block and are masked away). Without a window
+// the blocks of a long chunk are given its last tiles too, up to twice what they see; chunks that long go to the tcgen05 kernel
+// where it takes their head size.
 struct Seq {
-    int start, n, blocks, first_tile, tiles;   // tiles of one pair
+    int start, n, blocks, first_tile, tiles;   // the sequence's first tile; tiles of one pair
+    __device__ __forceinline__ int first_of(const AttnArgs& a, int token0) const {      // the first tile of the block of that token
+        return max(first_tile, ((start + min(token0 + a.block_tokens, n) - 1) >> a.tile_log) - tiles + 1);
+    }
 };
 __device__ __forceinline__ Seq seq_from(const AttnArgs& a, int start, int n) {
     Seq s;
     s.n = n;
     s.start = start;
     s.blocks = n <= 0 || n > a.most_new || start < 0 ? 0 : (n + a.block_tokens - 1) / a.block_tokens;
-    s.first_tile = (a.window > 0 ? max(0, start - a.window + 1) : 0) / a.tile;
-    s.tiles = (start + n - 1) / a.tile - s.first_tile + 1;
+    s.first_tile = (a.window > 0 ? max(0, start - a.window + 1) : 0) >> a.tile_log;
+    s.tiles = ((start + n - 1) >> a.tile_log) - s.first_tile + 1;
+    if (a.window > 0 && a.window < start + n) s.tiles = min(s.tiles, ((a.window + a.block_tokens - 3) >> a.tile_log) + 2);
     return s;
 }
 
@@ -552,7 +561,7 @@ struct Ring {
 };
 // The row of the pools of tile t (from the sequence's first) of sequence i and kv head kvh.
 __device__ __forceinline__ int place_of(const AttnArgs& a, const SeqTable& table, int i, int tile, int kvh) {
-    const int key = tile * a.tile;
+    const int key = tile << a.tile_log;
     int page = a.pages.at(table.slot[i], key / kPageSize);
     if (page < 0) {
         if (a.error) atomicExch(a.error, kBadPlaceInAttention);
@@ -614,7 +623,8 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_cluster_kernel(co
     const int tokens = min(a.block_tokens, s.n - token0), rows = tokens * group;
     const size_t row0 = (size_t)(a.cu[i] + token0) * a.heads + (size_t)kvh * group;
     // this CTA's tiles, and of those the warp's: warp, warp + 8, ...
-    const int per = (s.tiles + C - 1) / C, t_lo = s.first_tile + rank * per, t_hi = min(t_lo + per, s.first_tile + s.tiles);
+    const int per = (s.tiles + C - 1) / C, t_first = s.first_of(a, token0), t_lo = t_first + rank * per,
+              t_hi = min(t_lo + per, t_first + s.tiles);
     ring.tiles = t_hi - t_lo > warp ? (t_hi - t_lo - warp + kWarps - 1) / kWarps : 0;
     // places are looked up 32 at once, a lane each
     auto look_up = [&](int first) { return first + lane < ring.tiles ? place_of(a, table, i, t_lo + warp + kWarps * (first + lane), kvh) : 0; };
@@ -749,7 +759,8 @@ __global__ void __launch_bounds__(line_warps(NHT) * 32, 1) attention_quant_line_
         const int u = u_lo + first + lane, i = find_seq(table.tiles_before, a.seqs, u);
         const Seq s = seq_from(a, table.start[i], table.n[i]);
         const int pair = (u - table.tiles_before[i]) / s.tiles, t = u - table.tiles_before[i] - pair * s.tiles;
-        return place_of(a, table, i, s.first_tile + t, pair / s.blocks);
+        const int kvh = pair / s.blocks;
+        return place_of(a, table, i, s.first_of(a, (pair - kvh * s.blocks) * a.block_tokens) + t, kvh);
     };
     int places = look_up(0), looked = 0;
     auto request = [&](int k, int into) {
@@ -766,7 +777,7 @@ __global__ void __launch_bounds__(line_warps(NHT) * 32, 1) attention_quant_line_
         const int pair = (u - table.tiles_before[i]) / s.tiles, kvh = pair / s.blocks, token0 = (pair - kvh * s.blocks) * a.block_tokens;
         const int pair_at = table.tiles_before[i] + pair * s.tiles, part_end = min(u_hi, pair_at + s.tiles);
         const int tokens = min(a.block_tokens, s.n - token0), rows = tokens * group;
-        const int first_token = a.cu[i] + token0;
+        const int first_token = a.cu[i] + token0, first_tile = s.first_of(a, token0);
         const bool begins = pair_at >= u_lo, whole = begins && part_end == pair_at + s.tiles;
         // (a warp that gave up still says of the pairs it begins that there is nothing to join)
         if (begins && lane == 0)
@@ -780,7 +791,7 @@ __global__ void __launch_bounds__(line_warps(NHT) * 32, 1) attention_quant_line_
         state.begin(a, (size_t)first_token * a.heads + (size_t)kvh * group, s.start + token0, tokens);
         for (; u < part_end; ++u) {
             if (!(ok = ring.wait(a))) break;
-            state.tile(a, (s.first_tile + (u - pair_at)) * KT, ring.codes_at(ring.stage), ring.scales_at(ring.stage));
+            state.tile(a, (first_tile + (u - pair_at)) * KT, ring.codes_at(ring.stage), ring.scales_at(ring.stage));
             __syncwarp();        // every lane has read the slot
             if (u - u_lo + S < ring.tiles) request(u - u_lo + S, ring.stage);
             ring.next();
@@ -926,7 +937,7 @@ void launch(AttnArgs a, const CUtensorMap& mk, const CUtensorMap& mv, const Laun
     const int room_for = (int)((kRoom - smem.fixed) / smem.a_tile);                    // tiles in flight
     if (a.cluster) {
         // as many tiles in flight as a warp gets, at most what is left
-        const int tiles = ((sizes.max_len + a.tile - 1) / a.tile + 1 + a.cluster - 1) / a.cluster;
+        const int tiles = ((sizes.max_len + kClusterTile - 1) / kClusterTile + 1 + a.cluster - 1) / a.cluster;
         a.stages = std::max(1, std::min({(tiles + kWarps - 1) / kWarps, kMaxStages, room_for}));
         static bool prepared[kDevices] = {};
         auto kernel = attention_quant_cluster_kernel<NB, NHT, FMT, BOX>;
@@ -1009,10 +1020,11 @@ void attention_quant(const QuantPools& p, const void* q, void* out, int n_seqs, 
     if (((uintptr_t)q | (uintptr_t)out) & 15 || ((uintptr_t)p.k_codes | (uintptr_t)p.v_codes | (uintptr_t)p.k_scale | (uintptr_t)p.v_scale) & 15)
         throw std::invalid_argument("attention_quant: operands must be 16-byte aligned");
     if (workspace_floats < attention_quant_workspace(head_dim, row_tiles, pairs, cluster)) throw std::invalid_argument("attention_quant: the workspace is too small");
+    const int log_tile = (cluster ? kClusterTile : line_tile(row_tiles)) == 64 ? 6 : 5;
     AttnArgs a{(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)p.k_codes, (const uint8_t*)p.v_codes, (const uint8_t*)p.k_scale,
                (const uint8_t*)p.v_scale, {p.page_table, p.slots, p.table_stride, p.pages}, slot_ids, seq_ends, cu_seqlens, n_seqs, heads,
                kv_heads, head_dim, window, most_new, 8 * row_tiles / group, pairs, cluster, 0,
-               cluster ? kClusterTile : line_tile(row_tiles), scale * 1.4426950408889634f, (Cut*)workspace,
+               log_tile, scale * 1.4426950408889634f, (Cut*)workspace,
                workspace + (cluster ? 0 : (long long)pairs * (long long)(sizeof(Cut) / sizeof(float))), error};
     CUtensorMap mk{}, mv{};
     if (head_dim == 64 || head_dim == 128) {
@@ -1020,9 +1032,9 @@ void attention_quant(const QuantPools& p, const void* q, void* out, int n_seqs, 
         const CUtensorMapSwizzle swizzle = head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
         const uint64_t rows = (uint64_t)p.pages * kv_heads * kPageSize;
         mk = tiled_map_2d("attention_quant", CU_TENSOR_MAP_DATA_TYPE_UINT8, p.k_codes, (uint64_t)head_dim, rows, (uint64_t)head_dim, (uint32_t)head_dim,
-                          (uint32_t)a.tile, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+                          1u << log_tile, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
         mv = tiled_map_2d("attention_quant", CU_TENSOR_MAP_DATA_TYPE_UINT8, p.v_codes, (uint64_t)head_dim, rows, (uint64_t)head_dim, (uint32_t)head_dim,
-                          (uint32_t)a.tile, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+                          1u << log_tile, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
     }
     const LaunchSizes sizes{pairs, a.block_tokens * group, max_len};
     if (p.fmt == QUANT_FP8) launch_fmt<QUANT_FP8>(a, row_tiles, mk, mv, sizes, stream);

@@ -842,7 +842,7 @@ class Ops:
         pairs_with = lambda row_tiles: kv_heads * sum(-(-n // (8 * row_tiles // group)) for n in few)
         fits = lambda row_tiles, cluster: self.lib.sm_attention_quant_fits(head_dim, row_tiles, len(lens), cluster)
         pairs = pairs_with(row_tiles)
-        longest = max_len if not window else min(max_len, window + max(few))
+        longest = max_len if not window else min(max_len, window + min(max(few), 8 * row_tiles // group))
         if pairs * (-(-longest // 32) + 1) >= 1 << 31:
             return None                   # (more tiles of the line than the kernel counts)
         cluster = self._quant_cluster(pairs, longest, head_dim)

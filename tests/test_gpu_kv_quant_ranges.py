@@ -235,3 +235,41 @@ def test_places_outside_the_page_table_are_refused_by_the_plain_form(ops, dtype,
             ops.attention_quant(q, pack_step(slots, starts, [[0], [0]], torch.device("cuda")), 0.125, 0, layer)
     ops.attention_quant(q, pack_step([1, 0], [127, 99], [[0], [0]], torch.device("cuda")), 0.125, 0, layer)
     ops.check_error_flag()
+
+
+# ---- long chunks in a window --------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cluster", [None, 0, 1, 4])
+@pytest.mark.parametrize("window", [1, 2, 31, 33, 64, 129, 400])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(3, 1, 32), (5, 5, 48), (9, 1, 96), (14, 2, 64)])
+def test_long_chunks_in_a_window_straight_from_the_codes(ops, heads, kv_heads, hd, window, cluster, monkeypatch):
+    """Each block of tokens attends over tiles of its own, at the sequence's start and around the tiles' edges."""
+    monkeypatch.setattr(ops, "quant_cluster", cluster)
+    monkeypatch.setattr(ops, "quant_rows_tokens", 1 << 20)
+    starts, news, slots = [0, 61, 300], [150, 97, 40], [2, 0, 1]
+    ends = [s + n for s, n in zip(starts, news)]
+    layer = make_layer("int8", kv_heads, hd, ends, slots)
+    fill(ops, layer, slots, ends, 106)
+    q = _randn((sum(news), heads, hd), 107).bfloat16()
+    check_rows(ops, layer, q, slots, starts, news, hd ** -0.5, window)
+
+
+def test_the_work_of_a_long_chunk_in_a_window_grows_with_its_tokens(ops):
+    """Head size 48 has no tcgen05 kernel. Four times the tokens take about four times as long, not sixteen times (on a GPU that
+    both fill)."""
+    def microseconds(n):
+        layer = make_layer("fp8", 4, 48, [n], [0])
+        fill(ops, layer, [0], [n], 108)
+        q = _randn((n, 16, 48), 109).bfloat16()
+        step = pack_step([0], [0], [[0] * n], torch.device("cuda"))
+        best = float("inf")
+        for _ in range(7):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            ops.attention_quant(q, step, 48 ** -0.5, 64, layer)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b) * 1e3)
+        return best
+    short, long = microseconds(8192), microseconds(32768)
+    assert long < 8 * short, f"{short:.0f} and {long:.0f} us"
