@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             int f = 0, parts = 0, v_asked = 0;       // fills of K (as many of V, or one fewer), parts
             for (int u = u_lo; u < u_hi && ok;) {
                 const Part p = part_at(a, line, blocks, u, u_hi);
-                if (parts > 0 && !(ok = mbar_wait(q_empty, (uint32_t)(parts - 1) & 1u))) { fail(49); break; }
+                if (parts > 0 && !(ok = mbar_wait(q_empty, (uint32_t)(parts - 1) & 1u))) { fail(43); break; }
                 const int both = p.tokens > a.tile_tokens ? 2 : 1;
                 mbar_expect_tx(q_full, (uint32_t)(both * DB * tile_rows * 128));
                 for (int x = 0; x < both; ++x)

@@ -51,3 +51,13 @@ def test_places_inside_the_page_table_are_not_refused():
     layer = SimpleNamespace(slots=5, table_stride=2)
     Ops._check_places(pack_step([0, 4], [3, 125], [[0, 0], [0, 0, 0]], torch.device("cpu")), layer)
     Ops._check_places(SimpleNamespace(slots=[], seq_starts=None), layer)
+
+
+def test_each_bounded_wait_of_the_chunk_kernel_has_a_code_of_its_own():
+    import os
+    import re
+
+    import smolmoe_c99_b200
+    with open(os.path.join(os.path.dirname(smolmoe_c99_b200.__file__), "csrc", "attention_chunk_tc.cu")) as f:
+        codes = [int(c) for c in re.findall(r"fail\((\d+)\)", f.read())]
+    assert len(codes) >= 10 and len(set(codes)) == len(codes) and all(41 <= c <= 52 for c in codes), sorted(codes)
