@@ -671,7 +671,7 @@ void launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
 }  // namespace
 
 bool attention_chunk_supports(int heads, int kv_heads, int head_dim, long long pool_pages, int n_seqs, int blocks) {
-    return (head_dim == 64 || head_dim == 128) && kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= 64 && pool_pages > 0 &&
+    return (head_dim == 64 || head_dim == 128) && kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= 16 && pool_pages > 0 &&
            pool_pages * kv_heads * kPageSize < (1ll << 31) && n_seqs <= kMaxSeqs && blocks <= kMaxBlocks;
 }
 
@@ -685,7 +685,7 @@ void attention_chunk(const void* q, void* out, int T, int n_seqs, int heads, int
     if (n_seqs <= 0 || blocks <= 0 || T <= 0) return;
     if (!attention_chunk_supports(heads, kv_heads, head_dim, room, n_seqs, blocks))
         throw std::invalid_argument("attention_chunk: " + std::to_string(heads) + " heads on " + std::to_string(kv_heads) + " of size " +
-                                    std::to_string(head_dim) + " (64 or 128, at most 64 heads a kv head), " + std::to_string(n_seqs) + " sequences, " +
+                                    std::to_string(head_dim) + " (64 or 128, at most 16 heads a kv head), " + std::to_string(n_seqs) + " sequences, " +
                                     std::to_string(blocks) + " blocks of queries");
     if (!(scale > 0.f) || !(scale < INFINITY)) throw std::invalid_argument("attention_chunk: a scale of " + std::to_string(scale));
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15)

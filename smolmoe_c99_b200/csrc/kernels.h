@@ -287,7 +287,8 @@ void attention_quant(const QuantPools& pools, const void* q, void* out, int n_se
 
 // ---- attention_chunk_tc.cu ------------------------------------------------------------
 // The same attention for sequences that bring more than `skip_new` tokens, over their pages as bfloat16 values as
-// kv_quant_load (attend) leaves them, in `room` pages; `pages`: what the longest sequence has at most. Head sizes 64 and 128.
+// kv_quant_load (attend) leaves them, in `room` pages; `pages`: what the longest sequence has at most. Head sizes 64 and 128,
+// at most 16 heads a kv head (as attention_quant, which takes the step's other sequences).
 // `blocks`: blocks of 2 * (128 / group) new tokens over those sequences (group: heads a kv head).
 bool attention_chunk_supports(int heads, int kv_heads, int head_dim, long long pool_pages, int n_seqs, int blocks);
 long long attention_chunk_workspace(int head_dim, int kv_heads, int blocks);   // floats
