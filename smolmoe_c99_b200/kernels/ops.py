@@ -698,6 +698,7 @@ class Ops:
         zeros. Slots that are not the step's are given page 0."""
         if dtype is not torch.float32 and dtype is not torch.bfloat16:
             raise KernelError(f"an 8-bit cache is read back as float32 or bfloat16, not {dtype}")
+        self._check_slots_once(step)
         layer = self._quant_cache(cache)
         pages = min((step.max_seq_len + PAGE_SIZE - 1) // PAGE_SIZE, layer.table_stride)
         table = cache.page_table.new_empty((layer.slots, pages))
@@ -715,6 +716,12 @@ class Ops:
             v.data_ptr(), None if table is None else table.data_ptr(), pages, whole, room, read_seqs, read_pages, cu.data_ptr(), skip_new,
             attend, window, self._error_address, _raw_stream()))
         return k, v
+
+    @staticmethod
+    def _check_slots_once(step):
+        """Refuses a step with two sequences of one slot: the pages read back are found by slot."""
+        if len(set(step.slots)) != len(step.slots):
+            raise KernelError("a slot appears twice in the step")
 
     @staticmethod
     def _check_places(step, layer):
@@ -770,6 +777,7 @@ class Ops:
         if plan is None:
             # the plain kernel over pages that have been read back: float queries, other head sizes
             # (it checks no slot, position or page: those that the host knows are looked at here, and what is not read back has page 0)
+            self._check_slots_once(step)
             self._check_places(step, layer)
             most, room, seqs, pages = self._pages_read(step, layer, cache, 0, 0)
             table = cache.page_table.new_zeros((layer.slots, most))

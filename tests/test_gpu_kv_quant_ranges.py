@@ -273,3 +273,27 @@ def test_the_work_of_a_long_chunk_in_a_window_grows_with_its_tokens(ops):
         return best
     short, long = microseconds(8192), microseconds(32768)
     assert long < 8 * short, f"{short:.0f} and {long:.0f} us"
+
+
+# ---- the same slot twice ------------------------------------------------------------------------------------------------
+
+def test_a_slot_twice_in_a_step(ops):
+    """Two sequences of one slot that end at different positions. From the codes and through pages each is what it is alone; a page
+    table by slot cannot tell them apart, so reading back and the plain form refuse."""
+    from smolmoe_c99_b200.kernels import KernelError
+    layer = make_layer("fp8", 2, 64, [300, 50], [1, 0])
+    fill(ops, layer, [1, 0], [300, 50], 110)
+    slots, starts = [1, 0, 1], [99, 49, 297]
+    for news in ([1, 1, 1], [1, 1, 3]):
+        step = pack_step(slots, starts, [[0] * n for n in news], torch.device("cuda"))
+        q = _randn((sum(news), 4, 64), 111)
+        for rows_tokens in (64, 1):
+            ops.quant_rows_tokens = rows_tokens
+            try:
+                check_rows(ops, layer, q.bfloat16(), slots, starts, news, 0.125, 0)
+            finally:
+                ops.quant_rows_tokens = None
+        with pytest.raises(KernelError, match="slot appears twice"):
+            ops.attention_quant(q, step, 0.125, 0, layer)
+        with pytest.raises(KernelError, match="slot appears twice"):
+            ops.kv_quant_load(step, layer, torch.float32)

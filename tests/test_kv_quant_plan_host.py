@@ -61,3 +61,9 @@ def test_each_bounded_wait_of_the_chunk_kernel_has_a_code_of_its_own():
     with open(os.path.join(os.path.dirname(smolmoe_c99_b200.__file__), "csrc", "attention_chunk_tc.cu")) as f:
         codes = [int(c) for c in re.findall(r"fail\((\d+)\)", f.read())]
     assert len(codes) >= 10 and len(set(codes)) == len(codes) and all(41 <= c <= 52 for c in codes), sorted(codes)
+
+
+def test_a_slot_twice_is_refused_where_pages_are_found_by_slot():
+    with pytest.raises(KernelError, match="slot appears twice"):
+        Ops._check_slots_once(pack_step([1, 0, 1], [3, 0, 9], [[0], [0], [0]], torch.device("cpu")))
+    Ops._check_slots_once(pack_step([1, 0, 2], [3, 0, 9], [[0], [0], [0]], torch.device("cpu")))
