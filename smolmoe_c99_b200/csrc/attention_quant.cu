@@ -7,7 +7,7 @@
 //    together through shared memory, the CTAs through the leader's (distributed shared memory). One launch, no workspace.
 //  - the line (much work): the tiles of all pairs are put in one line, and every warp of a grid that fills the GPU once takes
 //    an equal run of it, whatever the sequences' lengths are. Warps meet nobody. A run that begins or ends inside a pair
-//    leaves the running maximum, the sum and the weighted values of its part in a workspace, and a second kernel puts the
+//    leaves its rows' references, sums and weighted values of its part in a workspace, and a second kernel puts the
 //    parts of each cut pair together in the order of the line.
 // All that this needs of the step (lengths, slots, pages) is read on the device, so a captured launch follows a growing
 // sequence, and results depend on no order of arrival.
@@ -23,11 +23,11 @@
 // The rows that a matrix names are permuted by row_position() so that both kinds of read are free of bank conflicts and P
 // needs no exchange beyond movmatrix.
 // Scales: the exponent of a key's row multiplies its scores; that of a value's row goes into the weight, P * 2^e. Weights are
-// half precision, so each row of queries puts its own by a power of two that brings the largest of those it has added up to
-// between 2^8 and 2^15: steps of half precision end at 2^-24, so what a weight may lose lies 2^33 below the row's own largest. What a
-// row does not see, and value rows that have no weight in it, do not count. The rows of queries are scaled by powers of two to
-// half precision, which holds all 8 bits of a bfloat16. Sums, maxima and accumulators are float. A row's reference for P is its
-// largest score rounded up to a whole power of two, so that nothing is rounded when it moves.
+// half precision, so what a row of queries puts its own against is the largest it has met of score + e, not of the score: its
+// largest weight lies between 2^8 and 2^15, steps of half precision end at 2^-24, and what a weight may lose lies 2^33 below the
+// row's own largest. What a row does not see, and value rows that have no weight in it, do not count. P itself, which is summed
+// up in float, goes by the same reference (see below why float's range does). The rows of queries are scaled by powers of two to
+// half precision, which holds all 8 bits of a bfloat16. Sums, maxima and accumulators are float.
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -81,7 +81,7 @@ struct AttnArgs {
     int cluster, stages, tile_log;       // CTAs of a cluster (0: the line); tiles a warp keeps in flight; positions of a tile: 2^tile_log
     float scale_log2;
     Cut* cuts;                           // the line: [pairs]
-    float* parts;                        // the line: [warps][2][rows][padded head size + 4]: values, then maximum and sum
+    float* parts;                        // the line: [warps][2][rows][padded head size + 4]: values, then reference and sum
     int* error;
 };
 
@@ -206,10 +206,13 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 // 2, 3, 10, 11, and the other eight).
 __device__ __forceinline__ int row_position(int r) { return r < 8 ? r : 8 + ((r - 8) ^ 4); }
 
-// Weights go to half precision as at most 2^15 (its largest number lies just below 2^16); where one would be larger, they are
-// put anew with the largest below 2^(15 - kSlack), so that the weights of the tiles to come rarely need that again. A weight of 1
-// with the least scale that a row can have needs 2^kMostShift to get there: none needs more.
-constexpr int kSlack = 6, kMostShift = 15 - kLeastExponent;
+// With R a row's reference, the largest score + e so far rounded up, what is summed up is 2^(score - R + kSumShift), and the weight
+// is that times 2^(e - kSumShift + 15 - kSlack). The reference moves where a score + e exceeds R + kSlack, so it seldom does, and
+// weights are at most 2^15. e lies between -100 and 120 (kv_quant.cuh), and counts as at least kLeastCounted in R: so s, the largest
+// score, has s - R between -121 and 86, and its 2^(s - R + kSumShift) lies between 2^-101, where a sum still has 2^-25 of it, and
+// 2^106, of which a sum holds a million. Where all e are -100 the largest weight is at least 2^-12, a normal number of half precision.
+constexpr int kSlack = 6, kSumShift = 20, kLeastCounted = -80;
+constexpr float kUnit = 1 << (kSumShift - 15 + kSlack);          // what has been added up, over the sum, in these units is the output
 
 // What a warp knows of the pair it works on, and what it has added up. NB: blocks of 64 of the head dimension; NHT: tiles
 // of 8 rows of queries; BOX: head_dim is 64 * NB. A thread holds, of each tile of rows, rows 2 q4 and 2 q4 + 1 (q4 = lane % 4)
@@ -220,9 +223,7 @@ struct Rows {
     uint32_t qf[CH][NHT][2];             // queries as half precision, scaled by a power of two to at most 2^11
     float q_scale[NHT][2];               // undoes the power of two, times scale * log2(e)
     float ot[CH][NHT][4];
-    float run_m[NHT][2], run_l[NHT][2];
-    int shift[NHT][2];                   // 2^shift takes weights to half precision; what has been added up has that factor too
-    int most_byte;                       // no weight passes 2^15 where the value row's byte is at most this, whatever its score
+    float limit[NHT][2], run_l[NHT][2];  // R + kSlack; the sum
     int first_pos, tokens, lowest;       // position of the first row's token, tokens, the lowest position that any sees
     uint32_t k_lane, v_lane;             // offsets in a tile of what this lane names in an ldmatrix of keys, of values
 
@@ -266,12 +267,10 @@ struct Rows {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 q_scale[nh][e] = __shfl_sync(0xffffffffu, down, (2 * q4 + e) * 4);
-                run_m[nh][e] = -CUDART_INF_F;
+                limit[nh][e] = -CUDART_INF_F;
                 run_l[nh][e] = 0.f;
-                shift[nh][e] = kMostShift;
             }
         }
-        most_byte = 15 + 127 - kMostShift;
     }
 
     // Shared-memory offset of a piece of 16 bytes of a row of a tile.
@@ -297,11 +296,8 @@ struct Rows {
         };
         // every row sees every position of the tile, or a mask is needed
         const bool masked = key0 + KT - 1 > first_pos || (a.window > 0 && key0 <= last_pos - a.window);
-        int top = lds_u8(exponents + KT + lane), top2 = KT == 64 ? lds_u8(exponents + KT + 32 + lane) : 0;
         if (masked) {
             const int from = max(lowest - key0, 0), to = last_pos + 1 - key0;    // positions some row sees: [from, to)
-            if (lane < from || lane >= to) top = 0;
-            if (lane + 32 < from || lane + 32 >= to) top2 = 0;
             if (from > 0 || to < KT) {
                 // value rows that no row sees may hold bytes that were never written: zeros (times zero weights)
                 for (int idx = lane; idx < KT * pieces; idx += 32) {
@@ -312,7 +308,6 @@ struct Rows {
                 __syncwarp();
             }
         }
-        top = max(top == kNoScale ? 0 : top, top2 == kNoScale ? 0 : top2);
         // S^T = K Q^T
         float st[MT][NHT][4];
 #pragma unroll
@@ -365,54 +360,58 @@ struct Rows {
                     }
                 }
         }
-        // whether any score exceeds its row's reference, or any weight may pass half precision
-        bool moved = top > most_byte;
+        // whether any score + e exceeds its row's limit
+        float e0[MT], e1[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            e0[mt] = (float)(max(lds_u8(ks_lo + KT + mt * 16) - 127, kLeastCounted));
+            e1[mt] = (float)(max(lds_u8(ks_hi + KT + mt * 16) - 127, kLeastCounted));
+        }
+        bool moved = false;
 #pragma unroll
         for (int nh = 0; nh < NHT; ++nh)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float x = fmaxf(st[0][nh][e], st[0][nh][e + 2]);
+                float x = fmaxf(st[0][nh][e] + e0[0], st[0][nh][e + 2] + e1[0]);
 #pragma unroll
-                for (int mt = 1; mt < MT; ++mt) x = fmax3(x, st[mt][nh][e], st[mt][nh][e + 2]);
-                moved |= x > run_m[nh][e];
+                for (int mt = 1; mt < MT; ++mt) x = fmax3(x, st[mt][nh][e] + e0[mt], st[mt][nh][e + 2] + e1[mt]);
+                moved |= x > limit[nh][e];
             }
-        // (most tiles of a long sequence bring neither, and then no maximum is looked for among the threads)
-        moved = __any_sync(0xffffffffu, moved);
-        int over[NHT][2];        // what has been added up is to be put smaller by 2^over
-        if (moved) {
-            // A larger reference: what has been added up stays as it is, weights to come are put larger by as much as the
-            // reference has grown, up to kMostShift.
-            bool scaled = false;
-            int largest = kLeastExponent;
+        if (__any_sync(0xffffffffu, moved)) {
+            // a larger reference: what has been added up is put on the new footing (most tiles bring none, and then no maximum is
+            // looked for among the threads)
 #pragma unroll
-            for (int nh = 0; nh < NHT; ++nh)
+            for (int nh = 0; nh < NHT; ++nh) {
+                float f[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float x = st[0][nh][e];
+                    float x = st[0][nh][e] + e0[0];
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) x = fmax3(x, st[mt][nh][e], st[mt][nh][e + 2]);
-                    x = fmaxf(run_m[nh][e], ceilf(max_of_row(x)));
-                    const int grown = (int)fminf(x - run_m[nh][e], 1000.f);      // (the first reference: 1000)
-                    run_m[nh][e] = x;
-                    run_l[nh][e] *= power_of_two_or_zero(-grown);
-                    over[nh][e] = max(shift[nh][e] + grown - kMostShift, 0);
-                    shift[nh][e] += grown - over[nh][e];
-                    scaled |= over[nh][e] > 0;
-                    largest = max(largest, shift[nh][e]);
+                    for (int mt = 0; mt < MT; ++mt) x = fmax3(x, st[mt][nh][e] + e0[mt], st[mt][nh][e + 2] + e1[mt]);
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    x = x > limit[nh][e] ? ceilf(x) + kSlack : limit[nh][e];
+                    const float root = x == limit[nh][e] ? 1.f : ex2_approx(0.5f * (limit[nh][e] - x));
+                    limit[nh][e] = x;
+                    run_l[nh][e] = run_l[nh][e] * root * root;      // (a sum may have to go down by more than float has a factor for)
+                    f[e] = root * root;
                 }
-            most_byte = 15 + 127 - __reduce_max_sync(0xffffffffu, largest);
-            moved = __any_sync(0xffffffffu, scaled || top > most_byte);
+#pragma unroll
+                for (int c = 0; c < CH; ++c) { ot[c][nh][0] *= f[0]; ot[c][nh][1] *= f[1]; ot[c][nh][2] *= f[0]; ot[c][nh][3] *= f[1]; }
+            }
         }
-        // P = 2^(score - reference), summed up, and P * 2^e
+        // P, summed up, and the weights
         float ref[NHT][2];
 #pragma unroll
         for (int nh = 0; nh < NHT; ++nh)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) ref[nh][e] = run_m[nh][e] == -CUDART_INF_F ? 0.f : run_m[nh][e];
+            for (int e = 0; e < 2; ++e) ref[nh][e] = limit[nh][e] == -CUDART_INF_F ? 0.f : limit[nh][e] - (kSlack + kSumShift);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const int b0 = lds_u8(ks_lo + KT + mt * 16), b1 = lds_u8(ks_hi + KT + mt * 16);
-            const float w0 = b0 == kNoScale ? CUDART_NAN_F : scale_of(b0), w1 = b1 == kNoScale ? CUDART_NAN_F : scale_of(b1);
+            const float w0 = b0 == kNoScale ? CUDART_NAN_F : __int_as_float(max(b0 - (kSumShift - 15 + kSlack), 0) << 23);
+            const float w1 = b1 == kNoScale ? CUDART_NAN_F : __int_as_float(max(b1 - (kSumShift - 15 + kSlack), 0) << 23);
 #pragma unroll
             for (int nh = 0; nh < NHT; ++nh)
 #pragma unroll
@@ -423,42 +422,14 @@ struct Rows {
                     st[mt][nh][e] = masked && st[mt][nh][e] == -CUDART_INF_F ? 0.f : v * ((e & 2) ? w1 : w0);
                 }
         }
-        if (moved) {
-            // the largest weights of the tile, exactly (a maximum passes over NaN); where one passes 2^15 the row's are put anew
-            int largest = kLeastExponent;
-#pragma unroll
-            for (int nh = 0; nh < NHT; ++nh) {
-                float f[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float x = 0.f;
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) x = fmax3(x, st[mt][nh][e], st[mt][nh][e + 2]);
-                    x = max_of_row(x);
-                    const int power = (int)((__float_as_uint(x) + 0x7fffffu) >> 23) - 127;      // x is at most 2^power
-                    const int less = power + shift[nh][e] > 15 ? power + shift[nh][e] - (15 - kSlack) : 0;
-                    shift[nh][e] -= less;
-                    f[e] = power_of_two_or_zero(-(less + over[nh][e]));
-                    largest = max(largest, shift[nh][e]);
-                }
-#pragma unroll
-                for (int c = 0; c < CH; ++c) { ot[c][nh][0] *= f[0]; ot[c][nh][1] *= f[1]; ot[c][nh][2] *= f[0]; ot[c][nh][3] *= f[1]; }
-            }
-            most_byte = 15 + 127 - __reduce_max_sync(0xffffffffu, largest);
-        }
-        float to_half[NHT][2];
-#pragma unroll
-        for (int nh = 0; nh < NHT; ++nh)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) to_half[nh][e] = power_of_two(shift[nh][e]);
         // ... as the B operand
         uint32_t pb[MT][NHT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int nh = 0; nh < NHT; ++nh) {
-                pb[mt][nh][0] = movmatrix_trans(pack_half2(st[mt][nh][0] * to_half[nh][0], st[mt][nh][1] * to_half[nh][1]));
-                pb[mt][nh][1] = movmatrix_trans(pack_half2(st[mt][nh][2] * to_half[nh][0], st[mt][nh][3] * to_half[nh][1]));
+                pb[mt][nh][0] = movmatrix_trans(pack_half2(st[mt][nh][0], st[mt][nh][1]));
+                pb[mt][nh][1] = movmatrix_trans(pack_half2(st[mt][nh][2], st[mt][nh][3]));
             }
         // O^T += V^T P^T
 #pragma unroll
@@ -479,15 +450,6 @@ struct Rows {
                 }
             }
     }
-
-    // The largest among the threads that share a row.
-    static __device__ __forceinline__ float max_of_row(float x) {
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-        return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-    }
-    // 2^e for e <= 0, and 0 below float's least normal number
-    static __device__ __forceinline__ float power_of_two_or_zero(int e) { return __int_as_float(max(e + 127, 0) << 23); }
 
     // The end: sums over the threads that share a row.
     __device__ __forceinline__ void end() {
@@ -574,10 +536,11 @@ __device__ __forceinline__ void store_row4(__nv_bfloat16* dst, float4 v, float b
     const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x * by, v.y * by), hi = __floats2bfloat162_rn(v.z * by, v.w * by);
     *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
-// How a part with maximum m and sum l counts against the maximum `top` of all parts. (Without positions: 0; without a
-// maximum, because every score it saw is NaN: 1, and its sum is NaN.)
-__device__ __forceinline__ float part_factor(float m, float l, float top) {
-    return m == -CUDART_INF_F ? (l == 0.f ? 0.f : 1.f) : ex2_approx(m - top);
+// How a part with reference (limit) m and sum l counts against the largest one, `top`: the root of the factor, to be applied twice,
+// since a sum may have to go down by more than float has a factor for. (Without positions: 0; without a reference, because every
+// score it saw is NaN: 1, and its sum is NaN.)
+__device__ __forceinline__ float part_root(float m, float l, float top) {
+    return m == -CUDART_INF_F ? (l == 0.f ? 0.f : 1.f) : ex2_approx(0.5f * (m - top));
 }
 
 // ---- clusters: blockIdx.x / cluster is the pair ---------------------------------------------------------------------------
@@ -593,9 +556,9 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_cluster_kernel(co
     const size_t ring_bytes = (size_t)kWarps * S * 2 * kClusterTile * hd;
     unsigned char* ring0 = BOX ? reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023) : smem_raw;
     float* wo = reinterpret_cast<float*>(ring0 + ring_bytes);       // [warp][R][LD] values
-    float* wm = wo + kWarps * R * LD;                               // [warp][R] maxima, then the warps' factors
+    float* wm = wo + kWarps * R * LD;                               // [warp][R] references, then the warps' factors
     float* wl = wm + kWarps * R;                                    // [warp][R] sums
-    float* parts = wl + kWarps * R;                                 // the leader's: [C][R][LD] values, maximum, sum
+    float* parts = wl + kWarps * R;                                 // the leader's: [C][R][LD] values, reference, sum
     float* end_of_parts = parts + (C > 1 ? C : 1) * R * LD;
     unsigned char* scales = reinterpret_cast<unsigned char*>(end_of_parts);
     uint64_t* bars = reinterpret_cast<uint64_t*>(scales + (size_t)kWarps * S * 2 * kClusterTile);
@@ -656,12 +619,11 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_cluster_kernel(co
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int r = nh * 8 + 2 * q4 + e;
-                const float unit = power_of_two(-state.shift[nh][e]);
-                if (g == 0) { wm[warp * R + r] = state.run_m[nh][e]; wl[warp * R + r] = state.run_l[nh][e]; }
+                if (g == 0) { wm[warp * R + r] = state.limit[nh][e]; wl[warp * R + r] = state.run_l[nh][e]; }
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
-                    o[r * LD + c * 16 + g] = state.ot[c][nh][e] * unit;
-                    o[r * LD + c * 16 + 8 + g] = state.ot[c][nh][2 + e] * unit;
+                    o[r * LD + c * 16 + g] = state.ot[c][nh][e];
+                    o[r * LD + c * 16 + 8 + g] = state.ot[c][nh][2 + e];
                 }
             }
     }
@@ -676,9 +638,9 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_cluster_kernel(co
         for (int w = 0; w < kWarps; ++w) m = fmaxf(m, wm[w * R + r]);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float f = part_factor(wm[w * R + r], wl[w * R + r], m);
-            l += wl[w * R + r] * f;
-            wm[w * R + r] = f;
+            const float root = part_root(wm[w * R + r], wl[w * R + r], m);
+            l += wl[w * R + r] * root * root;
+            wm[w * R + r] = root * root;
         }
         mine[r * LD + HDP] = m;
         mine[r * LD + HDP + 1] = failed ? CUDART_NAN_F : l;
@@ -696,7 +658,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_cluster_kernel(co
             }
         }
         if (C > 1) *reinterpret_cast<float4*>(mine + (size_t)r * LD + d) = sum;
-        else if (BOX || d < hd) store_row4(a.out + (row0 + (size_t)(r / group) * a.heads + r % group) * hd + d, sum, 1.0f / parts[r * LD + HDP + 1]);
+        else if (BOX || d < hd) store_row4(a.out + (row0 + (size_t)(r / group) * a.heads + r % group) * hd + d, sum, kUnit / parts[r * LD + HDP + 1]);
     }
     if (C == 1) return;
     cluster.sync();
@@ -708,13 +670,13 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_cluster_kernel(co
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int c = 0; c < C; ++c) {
             const float* part = parts + ((size_t)c * R + r) * LD;
-            const float f = part_factor(part[HDP], part[HDP + 1], m);
+            const float root = part_root(part[HDP], part[HDP + 1], m), f = root * root;
+            l += part[HDP + 1] * root * root;
             if (f == 0.f) continue;
             const float4 x = *reinterpret_cast<const float4*>(part + d);
-            l += part[HDP + 1] * f;
             sum.x = fmaf(x.x, f, sum.x); sum.y = fmaf(x.y, f, sum.y); sum.z = fmaf(x.z, f, sum.z); sum.w = fmaf(x.w, f, sum.w);
         }
-        if (BOX || d < hd) store_row4(a.out + (row0 + (size_t)(r / group) * a.heads + r % group) * hd + d, sum, 1.0f / l);
+        if (BOX || d < hd) store_row4(a.out + (row0 + (size_t)(r / group) * a.heads + r % group) * hd + d, sum, kUnit / l);
     }
 }
 
@@ -808,10 +770,9 @@ __global__ void __launch_bounds__(line_warps(NHT) * 32, 1) attention_quant_line_
             for (int e = 0; e < 2; ++e) {
                 const int r = nh * 8 + 2 * q4 + e;
                 if (r >= rows) continue;
-                const float unit = power_of_two(-state.shift[nh][e]);
                 if (whole) {
                     __nv_bfloat16* dst = a.out + ((size_t)(first_token + r / group) * a.heads + (size_t)kvh * group + r % group) * hd;
-                    const float by = unit / state.run_l[nh][e];
+                    const float by = kUnit / state.run_l[nh][e];
 #pragma unroll
                     for (int c = 0; c < CH; ++c)
                         if (BOX || c * 16 < hd) {
@@ -819,11 +780,11 @@ __global__ void __launch_bounds__(line_warps(NHT) * 32, 1) attention_quant_line_
                             dst[c * 16 + 8 + g] = __float2bfloat16_rn(state.ot[c][nh][2 + e] * by);
                         }
                 } else {
-                    if (g == 0) { part[r * LD + HDP] = state.run_m[nh][e]; part[r * LD + HDP + 1] = state.run_l[nh][e]; }
+                    if (g == 0) { part[r * LD + HDP] = state.limit[nh][e]; part[r * LD + HDP + 1] = state.run_l[nh][e]; }
 #pragma unroll
                     for (int c = 0; c < CH; ++c) {
-                        part[r * LD + c * 16 + g] = state.ot[c][nh][e] * unit;
-                        part[r * LD + c * 16 + 8 + g] = state.ot[c][nh][2 + e] * unit;
+                        part[r * LD + c * 16 + g] = state.ot[c][nh][e];
+                        part[r * LD + c * 16 + 8 + g] = state.ot[c][nh][2 + e];
                     }
                 }
             }
@@ -857,9 +818,9 @@ __global__ void __launch_bounds__(join_warps(P) * 32) attention_quant_join_kerne
             const float pm = part[HDP], pl = part[HDP + 1];
             const float4 x = lane < Q ? *reinterpret_cast<const float4*>(part + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
             const float top = fmaxf(m, pm);
-            const float f = part_factor(m, l, top), h = part_factor(pm, pl, top);
+            const float fr = part_root(m, l, top), hr = part_root(pm, pl, top), f = fr * fr, h = hr * hr;
             m = top;
-            l = l * f + pl * h;
+            l = l * fr * fr + pl * hr * hr;
             o.x = o.x * f + x.x * h; o.y = o.y * f + x.y * h; o.z = o.z * f + x.z * h; o.w = o.w * f + x.w * h;
         }
     }
@@ -874,15 +835,15 @@ __global__ void __launch_bounds__(join_warps(P) * 32) attention_quant_join_kerne
     o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < P; ++w) {
-        const float f = part_factor(ms[warp + w], ls[warp + w], m);
+        const float root = part_root(ms[warp + w], ls[warp + w], m), f = root * root;
+        l += ls[warp + w] * root * root;
         if (f == 0.f || lane >= Q) continue;
         const float4 x = sums[warp + w][lane];
-        l += ls[warp + w] * f;
         o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
     }
     const int d = lane * 4;
     if (r < cut.rows && lane < Q && d < a.head_dim)
-        store_row4(a.out + ((size_t)(cut.token0 + r / group) * a.heads + (size_t)cut.kv_head * group + r % group) * a.head_dim + d, o, 1.0f / l);
+        store_row4(a.out + ((size_t)(cut.token0 + r / group) * a.heads + (size_t)cut.kv_head * group + r % group) * a.head_dim + d, o, kUnit / l);
 }
 
 constexpr int kDevices = 64;

@@ -101,6 +101,23 @@ def test_large_values_without_weight(ops, fmt, cluster, power, monkeypatch):
     check_rows(ops, layer, q, [0], [n - 1], [1], 0.25, 0)
 
 
+@pytest.mark.parametrize("cluster,rows_tokens", [(None, 64), (0, 64), (4, 64), (1, 64)])
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("rising", [True, False])
+def test_values_over_all_that_a_scale_can_be(ops, fmt, rising, cluster, rows_tokens, monkeypatch):
+    """Equal scores, values from 2^-88 to 2^118 in runs of 40 positions: sums of weights count every position alike, however little its
+    values add. Then the least values alone, and the largest alone."""
+    monkeypatch.setattr(ops, "quant_cluster", cluster)
+    monkeypatch.setattr(ops, "quant_rows_tokens", rows_tokens)
+    n, hd = 1000, 64
+    layer = make_layer(fmt, 2, hd, [n], [0])
+    q = _randn((2, 4, hd), 112).bfloat16()
+    power = torch.linspace(-88, 118, 25).round().repeat_interleave(40)[:n]
+    for powers in (power if rising else power.flip(0), torch.full((n,), -98.0), torch.full((n,), 118.0)):
+        fill(ops, layer, [0], [n], 113, lambda k: k * 0.02, lambda v: v.clamp(-4, 4) * torch.exp2(powers).view(-1, 1, 1).cuda())
+        check_rows(ops, layer, q, [0], [n - 2], [2], 0.125, 0)
+
+
 # ---- windows ------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows_tokens", [64, 1])
