@@ -51,8 +51,8 @@ class LayerCache:
     exclusive: bool = False               # no page is in the tables of two sequences (bounds what is read back of an 8-bit cache)
 
     def quant_layer(self) -> QuantLayer:
-        """The pools of an 8-bit cache as the kernels take them, checked when first asked for (and again where a tensor of
-        the layer has been exchanged)."""
+        """The pools of an 8-bit cache as the kernels take them, checked when this view is first asked for them (and again where
+        a tensor of the layer has been exchanged)."""
         layer = self.__dict__.get("_quant")
         if layer is None or not layer.made_of(self):
             layer = self.__dict__["_quant"] = QuantLayer(self)

@@ -1,7 +1,7 @@
 // Writing the 8-bit key/value cache and reading it back (the format: kv_quant.cuh).
 //
-// Both are bound by memory: a thread takes 8 values of a row at a time (16 or 32 bytes in, 8 out, or the other way) and
-// several rows at once; the lanes that share a row find its largest magnitude with shuffles, so a value is read once and
+// Both are bound by memory: a thread takes 8 or 16 values of a row at a time (16 or 32 bytes in, 8 or 16 out, or the other way)
+// and several rows at once; the lanes that share a row find its largest magnitude with shuffles, so a value is read once and
 // written once.
 #include <stdexcept>
 #include <string>

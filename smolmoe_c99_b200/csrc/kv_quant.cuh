@@ -5,11 +5,12 @@
 // the largest magnitude of the row (1 <= m < 2), the exponent is
 //   e = E - 8 + [m > 1.75]  or  E - 6 + [m > 1.984375], at least kLeastExponent,
 // the smallest for which no code overflows; code = round to nearest even of x * 2^-e, value = code * 2^e.
-// Why a power of two: e4m3 is a floating-point format, so a finer scale would give it nothing; x * 2^-e and code * 2^e are
-// exact; and a code of at most 7 significant bits times a power of two is a bfloat16 number, so a kernel that reads the
+// Why a power of two: e4m3 is a floating-point format, so a finer scale would give it nothing (int8, whose steps are even, loses
+// up to a bit against a scale that takes the row's largest value to 127); x * 2^-e and code * 2^e are exact; and a code of at most 7 significant bits times a power of two is a bfloat16 number, so a kernel that reads the
 // cache as bfloat16 and one that multiplies codes see the same values.
 // A row with an infinity or a NaN has no scale: its byte is kNoScale, its codes are 0, and it reads back as NaN whole (the
-// byte's bits as a float are infinity, times 0). Codes that were written are therefore always finite.
+// byte's bits as a float are infinity, times 0). Codes that were written are therefore always finite. (A value that rounds up to
+// 2^128, from 1.9375 * 2^127 in e4m3 and 1.984375 * 2^127 in int8, has no float and reads back as infinity.)
 //
 // Pools, per layer: codes [pages, kv_heads, kPageSize, head_dim], exponents [pages, kv_heads, kPageSize] (one each for
 // keys and values); position p of a sequence lies on page page_table[slot][p / kPageSize]. Every position is kept.

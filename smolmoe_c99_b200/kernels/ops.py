@@ -105,7 +105,8 @@ class QuantPools(ctypes.Structure):
 
 
 class QuantLayer:
-    """The pools of an 8-bit layer cache, checked once, with the record that the kernels take."""
+    """The pools of an 8-bit layer cache, checked, with the record that the kernels take. Kept on the ``LayerCache`` it is made of
+    (a ``SequenceCache`` makes those anew for every eager step; a captured step's launches hold its contents)."""
 
     __slots__ = ("tensors", "pointers", "record", "address", "pages", "kv_heads", "head_dim", "slots", "table_stride", "device")
 
@@ -823,17 +824,21 @@ class Ops:
             return None
         group, limit, blocks, chunk_floats = heads // kv_heads, max(lens), 0, 0
         # Sequences that bring up to this many tokens attend straight from the codes, the others through pages read back and
-        # the tcgen05 kernel. Measured on a B200, us a call, codes against pages: 14 heads on 2 of 64, 64 tokens onto 1,000
-        # 10 / 18, 32 onto 8,000 22 / 21, 32 onto 32,000 52 / 31; 28 heads on 4 of 128, 32 onto 1,000 12 / 26, 16 onto 8,000
-        # 22 / 28, 32 onto 8,000 36 / 33, 16 onto 32,000 58 / 52, 32 onto 32,000 95 / 58. So: rows of queries (tokens times
+        # the tcgen05 kernel. Measured on a B200, one sequence, us a call, codes against pages: 14 heads on 2 of 64, 64 tokens onto
+        # 1,000 10 / 19, 32 onto 8,000 22 / 22, 32 onto 32,000 50 / 33; 28 heads on 4 of 128, 32 onto 1,000 11 / 27, 16 onto 8,000
+        # 20 / 29, 32 onto 8,000 35 / 34, 16 onto 32,000 55 / 53, 32 onto 32,000 92 / 59. So: rows of queries (tokens times
         # heads of a group) against the positions they see, and a few rows whatever those are (reading pages back costs the
-        # more the longer the sequence is).
+        # more the longer the sequence is). The positions are the longest sequence's, in a captured step the longest that it is
+        # kept for, so a step may go one way when it is first seen and the other when it is replayed; both are right, and differ
+        # by where weights are rounded.
         few_tokens = self.quant_rows_tokens
         if few_tokens is None:
             most, rows_by_positions = (448, 2_240_000) if head_dim <= 64 else (256, 1_600_000)
             seen = max_len if not window else min(max_len, window + most // group)
             few_tokens = max(1, min(most, max(96, rows_by_positions // seen)) // group)
         if limit > few_tokens and self.use_tcgen05_attention:
+            # (it takes 1,024 sequences and 2,048 blocks, about 74,000 tokens of 7 heads a kv head; a step past that goes straight
+            # from the codes, where keys are read again for every 8 to 32 rows of queries)
             many = 2 * (128 // group)     # tokens of a block of the tcgen05 kernel
             blocks = sum(-(-n // many) for n in lens if n > few_tokens)
             if self.lib.sm_attention_chunk_supports(heads, kv_heads, head_dim, len(lens) * layer.table_stride, len(lens), blocks):
@@ -878,7 +883,7 @@ class Ops:
         if pairs * tiles > 8192:
             return 0
         cluster = 1
-        # (clusters of 8 large CTAs do not pack every SM: more than 14 of them would take a second turn)
+        # (a B200's 148 SMs, one CTA each; clusters of 8 do not pack every SM: more than 14 of them would take a second turn)
         while cluster < 8 and 2 * cluster * pairs <= (148 if cluster < 4 else 112) and tiles > 8 * cluster:
             cluster *= 2
         return cluster
